@@ -109,7 +109,8 @@ int b200q_timer_stop(b200q_ctx* ctx, float* elapsed_ms);                        
  * and its duration added to the sum of its family.  Families (the `kind` argument):
  * 0 quantize_per_token, 1 dequantize_per_token, 2 quantize_static, 3 dequantize_static,
  * 4 weight preparation, 5 tensor-core GEMM (+ fused tail), 6 CUDA-core GEMM, 7 separate tail, 8 embedding,
- * 9 LayerNorm + quantize, 10 attention, 11 residual add.  While profiling is on, the events sit between the kernels, so
+ * 9 LayerNorm + quantize, 10 attention, 11 residual add, 12 cache append, 13 cache read, 14 attention over the cache,
+ * 15 cache keep.  While profiling is on, the events sit between the kernels, so
  * the dependent launches that let one kernel's set-up overlap the previous kernel's tail are switched off.
  * (No counterpart in the reference, whose runtime only offers measureCudaKernel.) */
 int b200q_profile_enable(b200q_ctx* ctx, int on);
@@ -319,6 +320,50 @@ int b200q_layernorm_quantize(b200q_ctx* ctx, const float* x, const float* residu
 int b200q_set_sdpa_variant(b200q_ctx* ctx, int variant);
 int b200q_sdpa_f32(b200q_ctx* ctx, const float* q, const float* k, const float* v, int64_t ld_q, int64_t ld_k, int64_t ld_v,
                    int64_t B, int64_t H, int64_t S, int64_t head_dim, float scale, int causal, float* out, int64_t ld_out);
+
+/* ---- int8 key/value cache and the attention that reads it ----
+ * The reference's attention takes whole K and V on every call (src/nn/functional/attention.ts:42-74) and keeps nothing
+ * between calls, so these entry points have no counterpart in it; a row enters the cache by its per-token quantization
+ * (quantization_types.ts:299-317, 118-130) with one row = one head of one token.
+ *
+ * A cache is `pages` pages of page_tokens tokens (16, 32, 64, 128 or 256) for `heads` heads of head_dim (64 or 128) in four
+ * buffers of the caller's, each starting on a 16-byte boundary: codes int8 [pages][heads][page_tokens][head_dim] and scales
+ * f32 [pages][heads][page_tokens], for K and for V.  Their contents need no initialisation: what no call has written is
+ * never visible.  The handle holds geometry and addresses only; it must not outlive its context or the buffers.
+ *
+ * Every call works on a batch of B sequences with T new rows each.  DEVICE arrays say which: page_table int32 [B, max_pages]
+ * (position p of sequence b is token p mod page_tokens of page page_table[b][p / page_tokens]; max_pages is the table's
+ * row length), start int32 [B] (positions held before the call: row t of the call is position start[b] + t) and count
+ * int32 [B] (rows in use, held to 0..T; null: T).  f32 operands: row (b, t) of head h starts at
+ * base + (b * T + t) * ld + h * head_dim, on a 16-byte boundary (ld a multiple of 4).  Rows t >= count[b] of outputs are
+ * left as they were.  A position outside the table, or on a page outside the cache, sets status bit 5 and is not
+ * written (append, keep), reads as zeros (read) or is not visible (attention).  Pages may be shared between sequences
+ * for reading; a position that two sequences of one call write is undefined.  All four calls are stream-ordered, need no
+ * workspace that grows, and may be recorded (b200q_graph_begin): lengths and pages are read when the recording runs. */
+typedef struct b200q_kv_cache b200q_kv_cache;
+int b200q_kv_create(b200q_ctx* ctx, int64_t pages, int64_t page_tokens, int64_t heads, int64_t head_dim, int8_t* k_codes,
+                    int8_t* v_codes, float* k_scales, float* v_scales, b200q_kv_cache** out);
+int b200q_kv_destroy(b200q_ctx* ctx, b200q_kv_cache* cache);
+/* Quantizes the new rows k and v (f32, `heads` heads) into the cache: the codes and scales b200q_quantize_per_token
+ * gives for rows of head_dim elements. */
+int b200q_kv_append(b200q_ctx* ctx, b200q_kv_cache* cache, const float* k, const float* v, int64_t ld_k, int64_t ld_v, int64_t B,
+                    int64_t T, const int32_t* page_table, int64_t max_pages, const int32_t* start, const int32_t* count);
+/* fround(code * scale) of positions start[b] + t, as b200q_dequantize_per_token. */
+int b200q_kv_read(b200q_ctx* ctx, b200q_kv_cache* cache, int64_t B, int64_t T, const int32_t* page_table, int64_t max_pages,
+                  const int32_t* start, const int32_t* count, float* k_out, float* v_out, int64_t ld_k, int64_t ld_v);
+/* out = softmax(scale * q K^T) V over the cached rows for H query heads (a multiple of the cache's heads: H / heads
+ * neighbouring heads share one), binary32 accuracy.  Row t sees every position below start[b] and, of the new ones (which
+ * b200q_kv_append has written), j <= t when tree is null -- T = 1 is a decoding step, T > 1 a chunk of a prompt -- or those
+ * j < count[b] whose bit is set in tree[b * T + t]: a drafted tree of at most 64 tokens, each row the set of its ancestors
+ * and itself.  A row that sees nothing is zero. */
+int b200q_kv_attention(b200q_ctx* ctx, b200q_kv_cache* cache, const float* q, int64_t ld_q, int64_t B, int64_t T, int64_t H,
+                       const int32_t* page_table, int64_t max_pages, const int32_t* start, const int32_t* count, const uint64_t* tree,
+                       float scale, float* out, int64_t ld_out);
+/* Keeps the accepted rows of a drafted tree: position start[b] + keep[b * T + i] moves to start[b] + i for i < count[b]
+ * (T at most 64; sources in any order, read before anything is written; keep values 0 .. T-1, another one is dropped and
+ * sets status bit 5). */
+int b200q_kv_keep(b200q_ctx* ctx, b200q_kv_cache* cache, int64_t B, int64_t T, const int32_t* page_table, int64_t max_pages,
+                  const int32_t* start, const int32_t* keep, const int32_t* count);
 
 /* ---- captured steps ----
  * A sequence of calls on a context recorded once and replayed with one launch (the reference's CUDA runtime replays

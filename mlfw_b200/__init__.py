@@ -6,6 +6,7 @@ object layer, and the mirror of the reference's backend interface
 (:mod:`mlfw_b200.backend`).  There is no CPU fallback.
 """
 from ._lib import B200QError, LIB_PATH
+from .kv_cache import KVCache
 from .device import ACT, Context, DeviceBuffer, Group, PinnedArray, W_KN, W_NK
 
-__all__ = ["B200QError", "LIB_PATH", "ACT", "Context", "DeviceBuffer", "Group", "PinnedArray", "W_KN", "W_NK"]
+__all__ = ["B200QError", "LIB_PATH", "ACT", "Context", "DeviceBuffer", "Group", "KVCache", "PinnedArray", "W_KN", "W_NK"]

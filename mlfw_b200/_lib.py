@@ -82,6 +82,12 @@ PROTOTYPES = {
     "b200q_layernorm_quantize": (c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, C.c_float, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp]),
     "b200q_set_sdpa_variant": (c_int, [c_vp, c_int]),
     "b200q_sdpa_f32": (c_int, [c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, C.c_float, c_int, c_vp, c_i64]),
+    "b200q_kv_create": (c_int, [c_vp, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp, C.POINTER(c_vp)]),
+    "b200q_kv_destroy": (c_int, [c_vp, c_vp]),
+    "b200q_kv_append": (c_int, [c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_vp, c_i64, c_vp, c_vp]),
+    "b200q_kv_read": (c_int, [c_vp, c_vp, c_i64, c_i64, c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64]),
+    "b200q_kv_attention": (c_int, [c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_vp, c_i64, c_vp, c_vp, c_vp, C.c_float, c_vp, c_i64]),
+    "b200q_kv_keep": (c_int, [c_vp, c_vp, c_i64, c_i64, c_vp, c_i64, c_vp, c_vp, c_vp]),
     "b200q_graph_begin": (c_int, [c_vp]),
     "b200q_graph_end": (c_int, [c_vp, C.POINTER(c_vp)]),
     "b200q_graph_launch": (c_int, [c_vp, c_vp]),

@@ -12,6 +12,9 @@ turned the four ``Linear`` modules into quantize -> quantized_dot -> per-channel
     y = x + (gelu(LayerNorm2(x) W1^T + b1) W2^T + b2)    the residual sum x is formed inside the LayerNorm2 launch; the
                                                          requantization of W2's input starts in W1's epilogue
 
+With a key/value cache (``forward_cached``) the attention reads int8 rows that earlier calls have appended, so a token is
+computed once.
+
 Weights are quantized per output channel on the device when the block is built and stay resident.
 """
 from __future__ import annotations
@@ -22,6 +25,7 @@ from typing import Dict, Optional
 import numpy as np
 
 from .device import Context, DeviceBuffer, W_NK
+from .kv_cache import KVCache
 
 
 @dataclass
@@ -78,28 +82,37 @@ class GPTBlock:
         self.fc2 = QuantLinear.from_float(ctx, params["w2"], params["b2"])
         self._bufs: Dict[str, DeviceBuffer] = {}
         self._M = -1
+        self._cached_bufs: Dict[int, Dict[str, DeviceBuffer]] = {}
 
     def _reserve(self, M: int) -> Dict[str, DeviceBuffer]:
         if M != self._M:
-            c, D, FF = self.ctx, self.D, self.FF
-            self._bufs = {
-                "n1_q": c.empty((M, D), np.int8), "n1_s": c.empty((M,), np.float32), "qkv": c.empty((M, 3 * D), np.float32),
-                "attn": c.empty((M, D), np.float32), "o": c.empty((M, D), np.float32), "x": c.empty((M, D), np.float32),
-                "n2_q": c.empty((M, D), np.int8), "n2_s": c.empty((M,), np.float32), "f1": c.empty((M, FF), np.float32),
-                "f1_q": c.empty((M, FF), np.int8), "f1_s": c.empty((M,), np.float32), "f2": c.empty((M, D), np.float32),
-            }
+            self._bufs = self._buffers(M)
             self._M = M
         return self._bufs
 
+    def _buffers(self, M: int) -> Dict[str, DeviceBuffer]:
+        c, D, FF = self.ctx, self.D, self.FF
+        return {
+            "n1_q": c.empty((M, D), np.int8), "n1_s": c.empty((M,), np.float32), "qkv": c.empty((M, 3 * D), np.float32),
+            "attn": c.empty((M, D), np.float32), "o": c.empty((M, D), np.float32), "x": c.empty((M, D), np.float32),
+            "n2_q": c.empty((M, D), np.int8), "n2_s": c.empty((M,), np.float32), "f1": c.empty((M, FF), np.float32),
+            "f1_q": c.empty((M, FF), np.int8), "f1_s": c.empty((M,), np.float32), "f2": c.empty((M, D), np.float32),
+        }
+
     def forward(self, h: DeviceBuffer, B: int, S: int, out: DeviceBuffer, causal: bool = True) -> Dict[str, DeviceBuffer]:
         """h, out: f32 [B*S, D].  Returns the intermediate buffers (reused by the next call with the same size)."""
-        c, D, H, FF = self.ctx, self.D, self.H, self.FF
+        c, D, H = self.ctx, self.D, self.H
         M = B * S
         t = self._reserve(M)
         c.layernorm_quantize(h, None, self.g1, self.b1, self.eps, M, D, None, None, t["n1_q"], t["n1_s"])
         c.int8_linear(t["n1_q"], t["n1_s"], self.qkv.w, self.qkv.scales, self.qkv.bias, "none", M, 3 * D, D, t["qkv"])
         base = t["qkv"].ptr
         c.sdpa_f32(base, base + D * 4, base + 2 * D * 4, 3 * D, 3 * D, 3 * D, B, H, S, 64, 1.0 / np.sqrt(64.0), causal, t["attn"], D)
+        self._after_attention(h, M, t, out)
+        return t
+
+    def _after_attention(self, h: DeviceBuffer, M: int, t: Dict[str, DeviceBuffer], out: DeviceBuffer) -> None:
+        c, D, FF = self.ctx, self.D, self.FF
         c.linear_f32(t["attn"], self.wo.w, self.wo.scales, self.wo.bias, "none", M, D, D, t["o"])
         c.layernorm_quantize(t["o"], h, self.g2, self.b2, self.eps, M, D, t["x"], None, t["n2_q"], t["n2_s"])
         # FC1 with the requantization of FC2's input behind it: the rows' ranges come out of FC1's epilogue, one pass encodes
@@ -107,6 +120,29 @@ class GPTBlock:
                                         t["f1"], t["f1_q"], t["f1_s"])
         c.int8_linear(t["f1_q"], t["f1_s"], self.fc2.w, self.fc2.scales, self.fc2.bias, "none", M, D, FF, t["f2"])
         c.add_f32(t["x"], t["f2"], M * D, out)
+
+    def forward_cached(self, h: DeviceBuffer, B: int, T: int, cache: KVCache, page_table, max_pages: int, start, out: DeviceBuffer,
+                       count=None, tree=None) -> Dict[str, DeviceBuffer]:
+        """The block for T new tokens of each of B sequences whose earlier ones are in ``cache`` (one cache per block): K and V of
+        the new tokens are appended, attention reads the cache.  h, out: f32 [B*T, D], row b*T + t.  A prompt's chunk (T tokens),
+        a decoding step (T = 1) or, with ``tree`` (uint64 [B*T]), drafted tokens; after a verification
+        :meth:`KVCache.keep` drops the refused ones.  Every row is computed, rows from count[b] on without attention.
+        Returns the intermediate buffers; those of every B*T it was called with stay with the block, so that a recorded step
+        remains valid while prompts of other lengths pass in between."""
+        c, D, H = self.ctx, self.D, self.H
+        assert cache.heads == H and cache.head_dim == 64, "the cache has another shape than the block's heads"
+        M = B * T
+        if M not in self._cached_bufs:
+            self._cached_bufs[M] = self._buffers(M)
+        t = self._cached_bufs[M]
+        c.layernorm_quantize(h, None, self.g1, self.b1, self.eps, M, D, None, None, t["n1_q"], t["n1_s"])
+        c.int8_linear(t["n1_q"], t["n1_s"], self.qkv.w, self.qkv.scales, self.qkv.bias, "none", M, 3 * D, D, t["qkv"])
+        base = t["qkv"].ptr
+        cache.append(base + D * 4, base + 2 * D * 4, 3 * D, 3 * D, B, T, page_table, max_pages, start, count)
+        if count is not None:
+            t["attn"].fill_bytes(0)     # rows from count[b] on are not written by the attention
+        cache.attention(base, 3 * D, B, T, H, page_table, max_pages, start, count, tree, 1.0 / np.sqrt(64.0), t["attn"], D)
+        self._after_attention(h, M, t, out)
         return t
 
 

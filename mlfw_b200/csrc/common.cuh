@@ -36,14 +36,15 @@ enum StatusBits : uint32_t {
   STATUS_EPI_WAIT_TIMEOUT = 1u << 2,   // epilogue gave up waiting for an accumulator
   STATUS_BAD_TMEM_ALLOC = 1u << 3,     // tensor-memory allocation returned an unexpected address
   STATUS_QUANT_WAIT_TIMEOUT = 1u << 4, // the staged quantize kernel gave up waiting for a row chunk or a free slot
-  STATUS_BAD_INDEX = 1u << 5,          // an embedding lookup met a token outside its table (the row is zero)
+  STATUS_BAD_INDEX = 1u << 5,          // an embedding lookup met a token outside its table (the row is zero), or a cache position is outside its pages
   STATUS_SDPA_WAIT_TIMEOUT = 1u << 7,  // the tensor-core attention kernel gave up waiting for its MMAs
   STATUS_SELFTEST_WAIT_TIMEOUT = 1u << 6, // b200q_selftest_bounded_wait: the wait on a barrier nothing signals gave up, as it must
 };
 
 // Kernel families timed separately when profiling is on (b200q_profile_*).
 enum KernelKind : int { KK_QUANT_TOKEN = 0, KK_DEQUANT_TOKEN, KK_QUANT_STATIC, KK_DEQUANT_STATIC, KK_WEIGHTS, KK_GEMM_UMMA,
-                        KK_GEMM_SIMT, KK_EPILOGUE, KK_EMBEDDING, KK_LAYERNORM, KK_SDPA, KK_ADD, KK_COUNT };
+                        KK_GEMM_SIMT, KK_EPILOGUE, KK_EMBEDDING, KK_LAYERNORM, KK_SDPA, KK_ADD, KK_KV_APPEND,
+                        KK_KV_READ, KK_KV_ATTENTION, KK_KV_KEEP, KK_COUNT };
 constexpr int PROFILE_RING = 256;
 constexpr int HOST_CHUNKS = 16;   // most pieces a host-buffer call is split into
 

@@ -18,7 +18,7 @@ W_NK, W_KN = 0, 1
 KIND = {np.dtype(np.int8): 0, np.dtype(np.uint8): 1, np.dtype(np.int32): 2}
 
 STATUS_BITS = {1: "TMA producer wait ran out", 2: "MMA issuer wait ran out", 4: "epilogue wait ran out",
-               8: "unexpected tensor-memory allocation", 16: "staged quantize wait ran out", 32: "embedding index outside its table",
+               8: "unexpected tensor-memory allocation", 16: "staged quantize wait ran out", 32: "embedding index outside its table, or cache position outside its pages",
                64: "self test: the wait on a barrier nothing signals gave up (as it must)", 128: "attention kernel's wait for its MMAs ran out"}
 
 
@@ -219,7 +219,8 @@ class Context:
         return ms.value
 
     KERNEL_KINDS = ("quantize_per_token", "dequantize_per_token", "quantize_static", "dequantize_static", "weights",
-                    "gemm_tensor_core", "gemm_cuda_core", "tail", "embedding", "layernorm_quantize", "sdpa", "add")
+                    "gemm_tensor_core", "gemm_cuda_core", "tail", "embedding", "layernorm_quantize", "sdpa", "add", "kv_append",
+                    "kv_read", "kv_attention", "kv_keep")
 
     def profile_enable(self, on: bool = True):
         check(self.lib.b200q_profile_enable(self.handle, int(on)), "b200q_profile_enable")

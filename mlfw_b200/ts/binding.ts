@@ -83,6 +83,12 @@ function bind(path: string) {
     layernormQuantize: f('int b200q_layernorm_quantize(void *ctx, const void *x, const void *residual, const void *gamma, const void *beta, float eps, int64_t M, int64_t D, void *sum_out, void *y_out, void *q_out, void *scales_out)'),
     setSdpaVariant: f('int b200q_set_sdpa_variant(void *ctx, int variant)'),
     sdpaF32: f('int b200q_sdpa_f32(void *ctx, const void *q, const void *k, const void *v, int64_t ld_q, int64_t ld_k, int64_t ld_v, int64_t B, int64_t H, int64_t S, int64_t head_dim, float scale, int causal, void *out, int64_t ld_out)'),
+    kvCreate: f('int b200q_kv_create(void *ctx, int64_t pages, int64_t page_tokens, int64_t heads, int64_t head_dim, void *k_codes, void *v_codes, void *k_scales, void *v_scales, _Out_ void **out)'),
+    kvDestroy: f('int b200q_kv_destroy(void *ctx, void *cache)'),
+    kvAppend: f('int b200q_kv_append(void *ctx, void *cache, const void *k, const void *v, int64_t ld_k, int64_t ld_v, int64_t B, int64_t T, const void *page_table, int64_t max_pages, const void *start, const void *count)'),
+    kvRead: f('int b200q_kv_read(void *ctx, void *cache, int64_t B, int64_t T, const void *page_table, int64_t max_pages, const void *start, const void *count, void *k_out, void *v_out, int64_t ld_k, int64_t ld_v)'),
+    kvAttention: f('int b200q_kv_attention(void *ctx, void *cache, const void *q, int64_t ld_q, int64_t B, int64_t T, int64_t H, const void *page_table, int64_t max_pages, const void *start, const void *count, const void *tree, float scale, void *out, int64_t ld_out)'),
+    kvKeep: f('int b200q_kv_keep(void *ctx, void *cache, int64_t B, int64_t T, const void *page_table, int64_t max_pages, const void *start, const void *keep, const void *count)'),
     graphBegin: f('int b200q_graph_begin(void *ctx)'),
     graphEnd: f('int b200q_graph_end(void *ctx, _Out_ void **out)'),
     graphLaunch: f('int b200q_graph_launch(void *ctx, void *graph)'),

@@ -1,0 +1,99 @@
+"""Host checks of the key/value cache's index rules and refusals (mlfw_b200/csrc/kv_layout.h), the very functions the kernels
+and the C entry points call, compiled with g++; and of the entry points' refusals that need no GPU."""
+import ctypes as C
+import os
+import subprocess
+
+import numpy as np
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+SOURCE = r"""
+#include "kv_layout.h"
+using namespace b200q;
+extern "C" {
+int64_t row(int64_t pages, int64_t max_pages, int shift, int heads, const int32_t* table, int64_t b, int head, int64_t pos) {
+  return kv_row(KvGeom{pages, max_pages, shift, heads}, table, b, head, pos);
+}
+int in_use(const int32_t* count, int64_t b, int T) { return kv_rows_in_use(count, b, T); }
+const char* geometry(int64_t p, int64_t t, int64_t h, int64_t d) { return kv_refuse_geometry(p, t, h, d); }
+const char* batch(int64_t B, int64_t T, int64_t h, const void* table, int64_t mp, const void* start) { return kv_refuse_batch(B, T, h, table, mp, start); }
+const char* rows(const void* base, int64_t ld, int64_t h, int64_t d) { return kv_refuse_rows(base, ld, h, d); }
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def host(tmp_path_factory):
+    d = tmp_path_factory.mktemp("kv")
+    (d / "h.cpp").write_text(SOURCE)
+    so = str(d / "h.so")
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-shared", "-fPIC", "-I", os.path.join(ROOT, "mlfw_b200", "csrc"), str(d / "h.cpp"), "-o", so],
+                   check=True)
+    lib = C.CDLL(so)
+    i64, vp = C.c_int64, C.c_void_p
+    lib.row.restype, lib.row.argtypes = i64, [i64, i64, C.c_int, C.c_int, vp, i64, C.c_int, i64]
+    lib.in_use.argtypes = [vp, i64, C.c_int]
+    for f, a in (("geometry", [i64] * 4), ("batch", [i64, i64, i64, vp, i64, vp]), ("rows", [vp, i64, i64, i64])):
+        getattr(lib, f).restype, getattr(lib, f).argtypes = C.c_char_p, a
+    return lib
+
+
+def test_rows_of_positions(host):
+    rng = np.random.default_rng(0)
+    for shift, heads, pages, per in ((4, 1, 9, 3), (6, 12, 40, 5), (8, 3, 7, 2)):
+        P = 1 << shift
+        table = np.ascontiguousarray(rng.permutation(pages)[: 2 * per].reshape(2, per) if 2 * per <= pages else rng.integers(0, pages, (2, per)), np.int32)
+        for b in range(2):
+            for pos in range(per * P):
+                for head in {0, heads - 1}:
+                    want = (int(table[b, pos // P]) * heads + head) * P + pos % P
+                    assert host.row(pages, per, shift, heads, table.ctypes.data, b, head, pos) == want
+
+
+def test_positions_outside_have_no_row(host):
+    table = np.array([[0, -1, 5, 4]], np.int32)     # a cache of five pages: -1 and 5 are not among them
+    row = lambda pos: host.row(5, 4, 4, 2, table.ctypes.data, 0, 1, pos)  # noqa: E731
+    assert [row(p) for p in (-1, -17, 16, 31, 32, 47, 64, 1 << 40)] == [-1] * 8
+    assert row(15) == 16 + 15 and row(48) == (4 * 2 + 1) * 16 and row(63) == (4 * 2 + 1) * 16 + 15
+    big = np.array([[2**31 - 2]], np.int32)          # rows past 2^31 and codes past 2^38
+    assert host.row(2**31 - 1, 1, 8, 64, big.ctypes.data, 0, 63, 255) == ((2**31 - 2) * 64 + 63) * 256 + 255
+
+
+def test_rows_in_use(host):
+    c = np.array([-3, 0, 2, 9], np.int32)
+    assert [host.in_use(c.ctypes.data, b, 4) for b in range(4)] == [0, 0, 2, 4] and host.in_use(None, 7, 4) == 4
+
+
+def test_refusals(host):
+    assert host.geometry(1, 16, 1, 64) is None and host.geometry(1000, 256, 65535, 128) is None
+    for bad in ((0, 64, 1, 64), (-1, 64, 1, 64), (2**31, 64, 1, 64), (4, 8, 1, 64), (4, 48, 1, 64), (4, 512, 1, 64), (4, 0, 1, 64), (4, 64, 0, 64),
+                (4, 64, 65536, 64), (4, 64, 2, 32), (4, 64, 2, 96), (2**31 - 1, 256, 65535, 128)):
+        assert host.geometry(*bad), bad
+    p = 4096
+    assert host.batch(3, 5, 8, p, 7, p) is None and host.batch(0, 5, 8, None, 0, None) is None and host.batch(3, 5, 8, None, 0, p) is None
+    for bad in ((-1, 5, 8, p, 7, p), (3, -5, 8, p, 7, p), (3, 5, 8, p, -7, p), (3, 5, 8, None, 7, p), (3, 5, 8, p, 7, None), (2**16, 2**15, 1, p, 7, p),
+                (2**62, 2**62, 1, p, 7, p), (1, 2**25, 1, p, 7, p), (1, 1, 1, p, 2**31, p)):
+        assert host.batch(*bad), bad
+    assert host.rows(p, 128, 2, 64) is None and host.rows(p, 400, 3, 128) is None
+    for bad in ((None, 128, 2, 64), (p + 4, 128, 2, 64), (p, 130, 2, 64), (p, 124, 2, 64), (p, -128, 2, 64)):
+        assert host.rows(*bad), bad
+
+
+def test_entry_points_refuse_without_a_gpu():
+    from mlfw_b200 import _lib
+    from mlfw_b200 import build
+    build.build()
+    lib = _lib.lib()
+    message = lambda: lib.b200q_last_error().decode()  # noqa: E731
+    out = C.c_void_p(1)
+    assert lib.b200q_kv_create(None, 4, 48, 2, 64, 4096, 4096, 4096, 4096, C.byref(out)) != 0 and "a page holds" in message() and out.value is None
+    assert lib.b200q_kv_create(None, 4, 64, 2, 64, 4096, None, 4096, 4096, C.byref(out)) != 0 and "null pointer" in message()
+    assert lib.b200q_kv_create(None, 4, 64, 2, 64, 4096, 4100, 4096, 4096, C.byref(out)) != 0 and "16-byte" in message()
+    assert lib.b200q_kv_create(None, 4, 64, 2, 64, 4096, 4096, 4096, 4096, C.byref(out)) != 0 and "null context" in message()
+    assert lib.b200q_kv_create(None, 4, 64, 2, 64, 4096, 4096, 4096, 4096, None) != 0 and "out pointer" in message()
+    assert lib.b200q_kv_destroy(None, None) == 0
+    for name, n in (("append", 12), ("read", 12), ("attention", 15), ("keep", 9)):
+        args = [None if t is C.c_void_p else t(0) for t in _lib.PROTOTYPES["b200q_kv_" + name][1]]
+        assert len(args) == n
+        assert getattr(lib, "b200q_kv_" + name)(*args) != 0 and "null context" in message()
