@@ -179,7 +179,7 @@ void b200q_destroy(b200q_ctx* ctx) {
   if (!ctx) return;
   cudaSetDevice(ctx->device);
   if (ctx->stream) cudaStreamSynchronize(ctx->stream);
-  Workspace* all[] = {&ctx->ws_q, &ctx->ws_scales, &ctx->ws_acc, &ctx->ws_stage_in, &ctx->ws_stage_out, &ctx->ws_range};
+  Workspace* all[] = {&ctx->ws_q, &ctx->ws_scales, &ctx->ws_acc, &ctx->ws_stage_in, &ctx->ws_stage_out, &ctx->ws_range, &ctx->ws_kv};
   for (Workspace* w : all)
     if (w->ptr) cudaFree(w->ptr);
   if (ctx->status_dev) cudaFree(ctx->status_dev);

@@ -84,6 +84,7 @@ struct b200q_ctx {
   b200q::Workspace ws_acc;               // int32 / f32 intermediates of the unfused paths
   b200q::Workspace ws_stage_in, ws_stage_out;  // device staging of the host-buffer entry points
   b200q::Workspace ws_range;             // row-range keys of the two-step per-token requantization (2 words per row)
+  b200q::Workspace ws_kv;                // joins of the attention over the cache: fixed size, made with the first cache
   int requant_variant = 0;               // 0: ranges published by the GEMM epilogue + one-pass encode; 1: f32 result + full per-token quantize
   double wait_limit_s = 2.0;             // bound of every device-side wait
   int gemm_variant = 0;                  // 0 auto, 1 CUDA-core kernel only, 2 tensor cores with one CTA per tile, 3 with CTA pairs

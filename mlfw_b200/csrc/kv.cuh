@@ -22,6 +22,12 @@ struct KvBatch {
   const int32_t *start, *count;
 };
 
+// Workspace of the attention: one counter per block of the largest grid, then two slots per block for pieces of items.
+// Its size depends on the GPU only, so a recording never finds it moved.
+constexpr int KV_BLOCKS_PER_SM = 2, KV_SLOT_FLOATS = 16 * (128 + 2);
+inline size_t kv_counter_bytes(const b200q_ctx* ctx) { return ((size_t)ctx->sm_count * KV_BLOCKS_PER_SM * sizeof(uint32_t) + 255) & ~size_t(255); }
+int kv_workspace(b200q_ctx* ctx);
+
 int launch_kv_append(b200q_ctx* ctx, const b200q_kv_cache& c, const KvBatch& s, const float* k, const float* v, int64_t ld_k, int64_t ld_v);
 int launch_kv_read(b200q_ctx* ctx, const b200q_kv_cache& c, const KvBatch& s, float* k_out, float* v_out, int64_t ld_k, int64_t ld_v);
 int launch_kv_keep(b200q_ctx* ctx, const b200q_kv_cache& c, const KvBatch& s, const int32_t* keep);

@@ -2,6 +2,18 @@
 //
 // Row t of sequence b sees the start[b] positions cached before and, of the count[b] new ones, those up to itself (no
 // tree) or those whose bit is set in its row of ancestors.  Query heads h of a group H / heads share cache head h / (H / heads).
+//
+// The arithmetic.  A cached value is code * scale with an integer |code| <= 128, which binary16 holds exactly.  A query
+// row is written in fixed point against its largest element, x = q * 2^(22 - e) with 2^e <= max|q| < 2^(e+1), and split
+// x = hi * 2^12 + lo, |hi| <= 2^11 an integer, |lo| <= 2^11: two binary16 numbers that keep 23 bits.  Then
+//     sum_d q_d code_d = 2^(e-22) * (2^12 * sum hi code + sum lo code),
+// two binary16 products with binary32 sums; the first is a sum of integers below 2^25 at worst and below 2^24 for all
+// ordinary rows, so it is exact, and a score carries the rounding of q (2^-23 of the row's largest element) and the one
+// of adding the two.  The weights p * scale_v are split the same way against their running maximum of the row.  So the
+// cache's codes go into the tensor cores as they are, and the result has binary32 accuracy at two binary16 products per
+// contraction.
+#include <cuda_fp16.h>
+
 #include "kernels.cuh"
 #include "kv.cuh"
 
@@ -19,73 +31,501 @@ struct AttnArgs {
   float* out;
   int64_t ld_q, ld_o;
   int B, T, H, group;
-  float scale;
+  float scale_log2e;       // scale * log2(e): scores are kept in units of log2
   uint32_t* status;
+  uint32_t* counters;      // pieces of an item that have arrived, by the run the item begins in; zero between launches
+  float* slots;
 };
 
-// One block per (sequence, row, query head), one warp per cached token: the plain formula in one pass over the cache.
-template <int D>
-__global__ void __launch_bounds__(128) kv_attention_kernel(const AttnArgs a) {
-  constexpr int E = D / 32;
-  __shared__ float part[4][D + 2];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t bt = blockIdx.x / a.H;
-  const int h = blockIdx.x % a.H, b = (int)(bt / a.T), t = (int)(bt % a.T);
-  const int n = kv_rows_in_use(a.count, b, a.T);
-  if (t >= n) return;
-  const int64_t first = a.start[b];
-  const uint64_t seen = a.tree ? a.tree[bt] : 0;
-  float q[E], o[E];
+constexpr float NEG_INF = -__builtin_huge_valf();
+
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 r;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a));
+  return r;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+  uint2 r;
+  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(a));
+  return r;
+}
+__device__ __forceinline__ float2 lds_f2(uint32_t a) {
+  const uint2 r = lds64(a);
+  return make_float2(__uint_as_float(r.x), __uint_as_float(r.y));
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+// Bytes 0 and 2 (even) or 1 and 3 (odd) of a word of codes as two binary16 numbers: the byte with its sign bit flipped
+// under the exponent of 1024 is 1024 + 128 + code; subtracting 1152 is exact.
+__device__ __forceinline__ uint32_t codes_even(uint32_t x) {
+  const uint32_t y = (x & 0x00ff00ffu) ^ 0x64806480u;
+  uint32_t r;
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(y), "r"(0x64806480u));
+  return r;
+}
+__device__ __forceinline__ uint32_t codes_odd(uint32_t x) { return codes_even(x >> 8); }
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {   // lo in the low half
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// x = hi * 2^12 + lo for |x| < 2^23: hi an integer (1.5 * 2^23 trick), lo exact.
+__device__ __forceinline__ void split12(float x, float& hi, float& lo) {
+  hi = __fsub_rn(fmaf(x, 0x1p-12f, 12582912.0f), 12582912.0f);
+  lo = fmaf(hi, -4096.0f, x);
+}
+__device__ __forceinline__ float pow2(int e) {   // 2^e for -126 <= e <= 127
+  return __int_as_float((e + 127) << 23);
+}
+
+// Where a query row comes from and its result goes: row R of the sequence (R = t * group + head within the group).
+__device__ __forceinline__ int64_t row_offset(const AttnArgs& a, int b, int head, int R, int64_t ld, int D, int& t) {
+  t = R / a.group;
+  return ((int64_t)b * a.T + t) * ld + (int64_t)(head * a.group + (R - t * a.group)) * D;
+}
+
+// The run of 16-token tiles this block works on: total tiles, the item its first tile belongs to (e = sequence * row
+// blocks + row block, head) and the tile inside it.  All threads take part and get the same answer.
+struct Run {
+  int64_t total, begin, end;
+  int runs, e, head, tile;
+};
+template <int ROWS>
+__device__ __forceinline__ Run find_run(const AttnArgs& a, int row_blocks, int warps) {
+  __shared__ int64_t warp_sum[33];
+  __shared__ int found[3];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int E = a.B * row_blocks, per = (E + blockDim.x - 1) / blockDim.x;
+  const int e0 = min(E, tid * per), e1 = min(E, e0 + per);
+  auto tiles = [&](int e) {
+    const int b = e / row_blocks;
+    return (int64_t)kv_tiles(a.g, a.start[b], kv_rows_in_use(a.count, b, a.T), a.group, ROWS, e - b * row_blocks, a.tree != nullptr, KV_TILE) * a.g.heads;
+  };
+  int64_t mine = 0;
+  for (int e = e0; e < e1; e++) mine += tiles(e);
+  int64_t incl = mine;
 #pragma unroll
-  for (int e = 0; e < E; e++) { q[e] = a.q[bt * a.ld_q + (int64_t)h * D + lane * E + e] * a.scale; o[e] = 0.0f; }
-  float m = __int_as_float(0xff800000), l = 0.0f;
-  for (int64_t pos = warp; pos < first + (a.tree ? n : t + 1); pos += 4) {
-    if (pos >= first && a.tree && !((seen >> (pos - first)) & 1)) continue;
-    const int64_t row = kv_row(a.g, a.page_table, b, h / a.group, pos);
-    if (row < 0) {
-      if (lane == 0) atomicOr(a.status, STATUS_BAD_INDEX);
-      continue;
-    }
-    float z = 0.0f;
-#pragma unroll
-    for (int e = 0; e < E; e++) z = fmaf(q[e], (float)a.k[row * D + lane * E + e], z);
-#pragma unroll
-    for (int s = 16; s > 0; s >>= 1) z += __shfl_xor_sync(0xffffffffu, z, s);
-    z *= a.ks[row];
-    const float top = fmaxf(m, z), old = expf(m - top), p = expf(z - top);
-    l = l * old + p;
-#pragma unroll
-    for (int e = 0; e < E; e++) o[e] = fmaf(p * a.vs[row], (float)a.v[row * D + lane * E + e], o[e] * old);
-    m = top;
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t x = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += x;
   }
-#pragma unroll
-  for (int e = 0; e < E; e++) part[warp][lane * E + e] = o[e];
-  if (lane == 0) { part[warp][D] = m; part[warp][D + 1] = l; }
+  if (lane == 31) warp_sum[warp] = incl;
   __syncthreads();
-  float top = part[0][D];
-  for (int w = 1; w < 4; w++) top = fmaxf(top, part[w][D]);
-  if (threadIdx.x < D) {
-    float sum = 0.0f, val = 0.0f;
-    for (int w = 0; w < 4; w++) {
-      if (part[w][D + 1] == 0.0f) continue;
-      const float f = expf(part[w][D] - top);
-      sum += f * part[w][D + 1];
-      val += f * part[w][threadIdx.x];
+  if (tid == 0) {
+    int64_t s = 0;
+    for (int w = 0; w < warps; w++) { const int64_t x = warp_sum[w]; warp_sum[w] = s; s += x; }
+    warp_sum[32] = s;
+  }
+  __syncthreads();
+  Run r;
+  r.total = warp_sum[32];
+  // at least one tile per warp of a block: a shorter run costs more in joining than it saves
+  const int64_t want = r.total / warps;
+  r.runs = (int)(want < 1 ? 1 : (want < (int64_t)gridDim.x ? want : (int64_t)gridDim.x));
+  if ((int)blockIdx.x >= r.runs || r.total == 0) { r.begin = r.end = 0; return r; }
+  r.begin = kv_run_begin(r.total, r.runs, blockIdx.x);
+  r.end = kv_run_begin(r.total, r.runs, blockIdx.x + 1);
+  int64_t at = warp_sum[warp] + incl - mine;
+  if (r.begin >= at && r.begin < at + mine) {
+    int e = e0;
+    int64_t n = tiles(e);
+    while (r.begin >= at + n) { at += n; n = tiles(++e); }
+    const int64_t per_head = n / a.g.heads, in = r.begin - at;
+    found[0] = e; found[1] = (int)(in / per_head); found[2] = (int)(in % per_head);
+  }
+  __syncthreads();
+  r.e = found[0]; r.head = found[1]; r.tile = found[2];
+  return r;
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Few rows (a decoding step: 1 .. 16 query rows share a cache head).  Bound by reading the cache: 2 (D + 4) bytes per token
+// and head.  Warp-level binary16 products (m16n8k16): the sixteen rows of the A operand are eight query rows' hi and the
+// same rows' lo parts, so one instruction does both parts and a thread finds the two sums of its score in its own
+// accumulators.  B operands come straight from rows of codes: a lane's 16 bytes of a key row are four k-steps (which head
+// dimensions make up a k-step is free as long as q follows), and of V a lane takes the same 16 dimensions of four tokens.
+//
+// Each warp works on 16-token tiles of its own through a ring of its own in shared memory (cp.async, no block-wide
+// barrier inside a piece); eight warps of a block join their results at the end of a piece.
+// ---------------------------------------------------------------------------------------------------------------
+constexpr int FEW_WARPS = 8;
+template <int D>
+struct Few {
+  static constexpr int STAGES = D == 128 ? 3 : 6;              // about 100 KB of ring per block: two blocks per SM
+  static constexpr int TILE = 2 * KV_TILE * D + 2 * KV_TILE * 4;   // K and V codes, K and V scales
+  static constexpr int RING = FEW_WARPS * STAGES * TILE;
+  static constexpr int Q_BYTES(int rg) { return rg * (D / 16) * 512; }
+};
+// Byte offset of 16-byte piece c of token t in a tile of [16][D]: swizzled so that neither the reads of K (eight tokens'
+// rows, four neighbouring pieces each) nor those of V (a piece of every second token) meet in a bank.
+template <int D>
+__device__ __forceinline__ uint32_t k_at(int t, int c) {
+  if (D == 128) return (uint32_t)(t * 128 + ((c ^ ((t & 1) << 2)) << 4));
+  return (uint32_t)((t >> 1) * 128 + (((((t & 1) << 2) | c) ^ (((t >> 1) & 3) << 1)) << 4));
+}
+template <int D>
+__device__ __forceinline__ uint32_t v_at(int t, int c) {
+  if (D == 128) return (uint32_t)(t * 128 + ((c ^ (((t >> 1) & 3) << 1)) << 4));
+  return k_at<64>(t, c);
+}
+
+// RG groups of eight query rows.
+template <int D, int RG>
+__global__ void __launch_bounds__(32 * FEW_WARPS, 2) kv_attention_few_kernel(const AttnArgs a, int row_blocks) {
+  using C = Few<D>;
+  constexpr int ROWS = 8 * RG, NT = D / 8, KS = D / 16, CH = D / 8;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float join_m[FEW_WARPS][ROWS], join_l[FEW_WARPS][ROWS];
+  __shared__ uint32_t arrived;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, t4 = lane & 3;
+  const uint32_t ring = smem_u32(smem) + warp * (C::STAGES * C::TILE), q_smem = smem_u32(smem) + C::RING;
+  float* join_o = reinterpret_cast<float*>(smem);               // [warp][row][D], over the rings between pieces
+
+  const Run run = find_run<ROWS>(a, row_blocks, FEW_WARPS);
+  int64_t left = run.end - run.begin;
+  int e = run.e, head = run.head, tile0 = run.tile;
+  int64_t at = run.begin;                                       // first tile of the piece among all tiles
+
+  while (left > 0) {
+    const int b = e / row_blocks, rb = e - b * row_blocks;
+    const int64_t first = a.start[b];
+    const int n = kv_rows_in_use(a.count, b, a.T);
+    const int tiles = kv_tiles(a.g, first, n, a.group, ROWS, rb, a.tree != nullptr, KV_TILE);
+    if (tiles == 0) { e++; head = 0; tile0 = 0; continue; }
+    const int64_t vis = kv_visible(a.g, first, n, a.group, ROWS, rb, a.tree != nullptr);
+    const int tile1 = (int)min((int64_t)tiles, tile0 + left);
+    const int rows_here = min(ROWS, n * a.group - rb * ROWS);
+    if (tid == 0 && (first < 0 || first + n > (a.g.max_pages << a.g.page_shift))) atomicOr(a.status, STATUS_BAD_INDEX);
+
+    // ---- the ring: tile i of the item into slot s
+    const int32_t* table = a.page_table + (int64_t)b * a.g.max_pages;
+    const int per_page = a.g.page_shift - 4;                    // log2 tiles per page
+    auto page_of = [&](int i) -> int { return (i < tile1 && ((int64_t)i >> per_page) < a.g.max_pages) ? __ldg(table + (i >> per_page)) : -1; };
+    auto fetch = [&](int i, int page, int s) {
+      if (i < tile1 && page >= 0 && page < a.g.pages) {
+        const int64_t row = (((int64_t)page * a.g.heads + head) << a.g.page_shift) + ((i & ((1 << per_page) - 1)) << 4);
+        const uint32_t dst = ring + s * C::TILE;
+#pragma unroll
+        for (int x = 0; x < D / 32; x++) {
+          const int c = x * 32 + lane, t = c / (D / 16), p = c % (D / 16);
+          cp16(dst + k_at<D>(t, p), a.k + row * D + c * 16);
+        }
+#pragma unroll
+        for (int x = 0; x < D / 32; x++) {
+          const int c = x * 32 + lane, t = c / (D / 16), p = c % (D / 16);
+          cp16(dst + KV_TILE * D + v_at<D>(t, p), a.v + row * D + c * 16);
+        }
+        if (lane < 8) cp16(dst + 2 * KV_TILE * D + lane * 16, (lane < 4 ? a.ks : a.vs) + row + (lane & 3) * 4);
+      }
+      cp_commit();
+    };
+    int page_q[C::STAGES];                                      // pages of the tiles in the ring
+#pragma unroll
+    for (int s = 0; s < C::STAGES - 1; s++) page_q[s] = page_of(tile0 + warp + s * FEW_WARPS);
+#pragma unroll
+    for (int s = 0; s < C::STAGES - 1; s++) fetch(tile0 + warp + s * FEW_WARPS, page_q[s], s);
+    int page_next = page_of(tile0 + warp + (C::STAGES - 1) * FEW_WARPS);
+
+    // ---- the query rows: this lane's row of every group, dimensions 64 m + 16 t4 + 0..15
+    float row_scale[RG];
+    int row_t[RG];
+    uint64_t row_seen[RG];
+#pragma unroll
+    for (int r = 0; r < RG; r++) {
+      const int R = rb * ROWS + r * 8 + g8;
+      const bool used = r * 8 + g8 < rows_here;
+      int t = 0;
+      const float* src = a.q + row_offset(a, b, head, used ? R : rb * ROWS, a.ld_q, D, t);
+      row_t[r] = used ? t : -1;
+      row_seen[r] = used && a.tree ? a.tree[(int64_t)b * a.T + t] : 0;
+      float4 x[KS];
+      uint32_t top = 0;
+#pragma unroll
+      for (int s = 0; s < KS; s++) {
+        x[s] = used ? __ldg(reinterpret_cast<const float4*>(src + (s >> 2) * 64 + t4 * 16 + (s & 3) * 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        top = max(max(top, max(__float_as_uint(x[s].x) & 0x7fffffffu, __float_as_uint(x[s].y) & 0x7fffffffu)),
+                  max(__float_as_uint(x[s].z) & 0x7fffffffu, __float_as_uint(x[s].w) & 0x7fffffffu));
+      }
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const bool finite = top < 0x7f800000u;
+      const int ex = max((int)(top >> 23), 24) - 127;           // exponent of the row's largest element; tiny rows keep fewer bits
+      const float up = pow2(22 - ex);                           // -105 .. 125
+      row_scale[r] = finite ? a.scale_log2e * pow2(ex - 22) : __int_as_float(0x7fc00000);   // a NaN or an infinity in the row: every score NaN
+      if (warp == 0) {
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+          float h0, h1, h2, h3, l0, l1, l2, l3;
+          const float4 y = finite ? x[s] : make_float4(0.f, 0.f, 0.f, 0.f);
+          split12(y.x * up, h0, l0); split12(y.y * up, h1, l1); split12(y.z * up, h2, l2); split12(y.w * up, h3, l3);
+          // k-step s of the key row's word: its even bytes are k = 2 t4, 2 t4 + 1, the odd ones k + 8
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(q_smem + (r * KS + s) * 512 + lane * 16), "r"(pack_f16(h0, h2)),
+                         "r"(pack_f16(l0, l2)), "r"(pack_f16(h1, h3)), "r"(pack_f16(l1, l3)) : "memory");
+        }
+      }
     }
-    a.out[bt * a.ld_o + (int64_t)h * D + threadIdx.x] = sum == 0.0f ? 0.0f : val / sum;
+    __syncthreads();
+
+    float o[RG][NT][2], m[RG], l[RG], xr[RG];
+    int ex_w[RG];                                               // weights are held as w * 2^(22 - ex_w)
+#pragma unroll
+    for (int r = 0; r < RG; r++) {
+      m[r] = NEG_INF; l[r] = 0.0f; xr[r] = 0.0f; ex_w[r] = -103;
+#pragma unroll
+      for (int i = 0; i < NT; i++) o[r][i][0] = o[r][i][1] = 0.0f;
+    }
+
+    int slot = 0;
+#pragma unroll 1
+    for (int i = tile0 + warp; i < tile1; i += FEW_WARPS) {
+      cp_wait<C::STAGES - 2>();
+      __syncwarp();
+      const int page = page_q[0];
+#pragma unroll
+      for (int s = 0; s + 2 < C::STAGES; s++) page_q[s] = page_q[s + 1];
+      page_q[C::STAGES - 2] = page_next;
+      fetch(i + (C::STAGES - 1) * FEW_WARPS, page_next, slot == 0 ? C::STAGES - 1 : slot - 1);
+      page_next = page_of(i + C::STAGES * FEW_WARPS);
+      const uint32_t kt = ring + slot * C::TILE, vt = kt + KV_TILE * D, sc = vt + KV_TILE * D;
+      slot = slot + 1 == C::STAGES ? 0 : slot + 1;
+      if (page < 0 || page >= a.g.pages) {                      // no such page: nothing of the tile is visible
+        if (lane == 0 && (int64_t)i * KV_TILE < vis) atomicOr(a.status, STATUS_BAD_INDEX);
+        continue;
+      }
+
+      // ---- scores: two blocks of eight tokens
+      float acc[RG][2][4];
+#pragma unroll
+      for (int r = 0; r < RG; r++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) acc[r][j][0] = acc[r][j][1] = acc[r][j][2] = acc[r][j][3] = 0.0f;
+#pragma unroll
+      for (int mm = 0; mm < D / 64; mm++) {
+        const uint4 x0 = lds128(kt + k_at<D>(g8, mm * 4 + t4)), x1 = lds128(kt + k_at<D>(8 + g8, mm * 4 + t4));
+        const uint32_t w0[4] = {x0.x, x0.y, x0.z, x0.w}, w1[4] = {x1.x, x1.y, x1.z, x1.w};
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+          const uint32_t b00 = codes_even(w0[w]), b01 = codes_odd(w0[w]), b10 = codes_even(w1[w]), b11 = codes_odd(w1[w]);
+#pragma unroll
+          for (int r = 0; r < RG; r++) {
+            const uint4 qa = lds128(q_smem + (r * KS + mm * 4 + w) * 512 + lane * 16);
+            mma16816(acc[r][0], qa, b00, b01);
+            mma16816(acc[r][1], qa, b10, b11);
+          }
+        }
+      }
+      const float2 ks0 = lds_f2(sc + t4 * 8), ks1 = lds_f2(sc + 32 + t4 * 8);
+      float2 vs0 = lds_f2(sc + 64 + t4 * 8), vs1 = lds_f2(sc + 96 + t4 * 8);
+      const int64_t pos = (int64_t)i * KV_TILE;
+      const bool edge = pos + KV_TILE > first;                  // some position of the tile is among the new rows or behind them
+      uint4 pa[RG];
+      float fold[RG];
+#pragma unroll
+      for (int r = 0; r < RG; r++) {
+        float z[4];
+        z[0] = fmaf(acc[r][0][0], 4096.0f, acc[r][0][2]) * (ks0.x * row_scale[r]);
+        z[1] = fmaf(acc[r][0][1], 4096.0f, acc[r][0][3]) * (ks0.y * row_scale[r]);
+        z[2] = fmaf(acc[r][1][0], 4096.0f, acc[r][1][2]) * (ks1.x * row_scale[r]);
+        z[3] = fmaf(acc[r][1][1], 4096.0f, acc[r][1][3]) * (ks1.y * row_scale[r]);
+        if (edge) {
+#pragma unroll
+          for (int c = 0; c < 4; c++) {
+            const int64_t j = pos + (c >> 1) * 8 + t4 * 2 + (c & 1) - first;
+            const bool seen = j < 0 ? pos + (c >> 1) * 8 + t4 * 2 + (c & 1) < vis : (j < n && (a.tree ? (row_seen[r] >> j) & 1 : j <= row_t[r]) && first + j < vis);
+            if (!seen) z[c] = NEG_INF;
+            if (j >= n || first + j >= vis) (c == 0 ? vs0.x : c == 1 ? vs0.y : c == 2 ? vs1.x : vs1.y) = 0.0f;   // unwritten: may be anything
+          }
+        }
+        float mx = fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3]));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const float m_new = fmaxf(m[r], mx), m_use = m_new == NEG_INF ? 0.0f : m_new;   // nothing visible yet: p = 0 throughout
+        const float alpha = ex2(m[r] - m_use);
+        m[r] = m_new;
+        const float p0 = ex2(z[0] - m_use), p1 = ex2(z[1] - m_use), p2 = ex2(z[2] - m_use), p3 = ex2(z[3] - m_use);
+        l[r] = fmaf(l[r], alpha, (p0 + p1) + (p2 + p3));
+        // weights p * scale_v in fixed point against the row's largest so far
+        float x0 = p0 * vs0.x, x1 = p1 * vs0.y, x2 = p2 * vs1.x, x3 = p3 * vs1.y;
+        float xm = fmaxf(fmaxf(x0, x1), fmaxf(x2, x3));
+        xm = fmaxf(xm, __shfl_xor_sync(0xffffffffu, xm, 1));
+        xm = fmaxf(xm, __shfl_xor_sync(0xffffffffu, xm, 2));
+        xr[r] = fmaxf(xr[r] * alpha, xm);
+        const int ex = max(__float_as_int(xr[r]) >> 23, 24) - 127;   // -103 .. 128
+        const float up = pow2(22 - ex);
+        const int d = ex_w[r] - ex;
+        fold[r] = alpha * pow2(d > 126 ? 126 : (d < -126 ? -126 : d));
+        ex_w[r] = ex;
+        float h0, h1, h2, h3, l0, l1, l2, l3;
+        split12(x0 * up, h0, l0); split12(x1 * up, h1, l1); split12(x2 * up, h2, l2); split12(x3 * up, h3, l3);
+        pa[r] = make_uint4(pack_f16(h0, h1), pack_f16(l0, l1), pack_f16(h2, h3), pack_f16(l2, l3));
+      }
+
+      // ---- o = o * fold + P V: dimension CH * g8 + d of the 16 tokens
+      {
+        uint32_t y[4][D / 32];
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+          const int t = 2 * t4 + (c & 1) + (c >> 1) * 8;
+          if (D == 128) {
+            const uint4 w = lds128(vt + v_at<D>(t, g8));
+            y[c][0] = w.x; y[c][1] = w.y; y[c][D / 32 - 2] = w.z; y[c][D / 32 - 1] = w.w;
+          } else {
+            const uint2 w = lds64(vt + v_at<D>(t, g8 >> 1) + (g8 & 1) * 8);
+            y[c][0] = w.x; y[c][1] = w.y;
+          }
+        }
+#pragma unroll
+        for (int w = 0; w < D / 32; w++)
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            const uint32_t lo = __byte_perm(y[0][w], y[1][w], h ? 0x7632 : 0x5410), hi = __byte_perm(y[2][w], y[3][w], h ? 0x7632 : 0x5410);
+#pragma unroll
+            for (int odd = 0; odd < 2; odd++) {
+              const int d = w * 4 + h * 2 + odd;
+              const uint32_t b0 = odd ? codes_odd(lo) : codes_even(lo), b1 = odd ? codes_odd(hi) : codes_even(hi);
+#pragma unroll
+              for (int r = 0; r < RG; r++) {
+                float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                mma16816(c, pa[r], b0, b1);
+                o[r][d][0] = fmaf(o[r][d][0], fold[r], fmaf(c[0], 4096.0f, c[2]));
+                o[r][d][1] = fmaf(o[r][d][1], fold[r], fmaf(c[1], 4096.0f, c[3]));
+              }
+            }
+          }
+      }
+    }
+    cp_wait<0>();
+
+    // ---- the eight warps' results of the piece
+#pragma unroll
+    for (int r = 0; r < RG; r++) {
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+      if (t4 == 0) { join_m[warp][r * 8 + g8] = m[r]; join_l[warp][r * 8 + g8] = l[r]; }
+    }
+    __syncthreads();                                            // every ring is drained
+#pragma unroll
+    for (int r = 0; r < RG; r++) {
+      const int row = r * 8 + g8;
+      float top = join_m[0][row];
+#pragma unroll
+      for (int w = 1; w < FEW_WARPS; w++) top = fmaxf(top, join_m[w][row]);
+      // the row's weights back from fixed point, relative to the block's maximum
+      const float f = ex2(m[r] - (top == NEG_INF ? 0.0f : top)) * pow2(ex_w[r] - 22);
+      float* dst = join_o + (warp * ROWS + row) * D + t4 * 2 * CH;
+#pragma unroll
+      for (int c = 0; c < 2; c++)
+#pragma unroll
+        for (int i = 0; i < CH; i += 4)
+          *reinterpret_cast<float4*>(dst + c * CH + i) = make_float4(o[r][i][c] * f, o[r][i + 1][c] * f, o[r][i + 2][c] * f, o[r][i + 3][c] * f);
+    }
+    __syncthreads();
+    const bool whole = tile0 == 0 && tile1 == tiles;
+    const int64_t item0 = at - tile0;                           // first tile of the item among all tiles
+    const int run0 = whole ? 0 : (int)kv_run_of(run.total, run.runs, item0), run1 = whole ? 0 : (int)kv_run_of(run.total, run.runs, item0 + tiles - 1);
+    float* mine = a.slots + (int64_t)(2 * blockIdx.x + (tile0 == 0 ? 1 : 0)) * KV_SLOT_FLOATS;
+#pragma unroll
+    for (int x = 0; x < ROWS * D / (32 * FEW_WARPS); x++) {
+      const int row = (x * 32 * FEW_WARPS + tid) / D, d = tid % D;
+      float top = join_m[0][row], sum = 0.0f, val = 0.0f;
+#pragma unroll
+      for (int w = 1; w < FEW_WARPS; w++) top = fmaxf(top, join_m[w][row]);
+#pragma unroll
+      for (int w = 0; w < FEW_WARPS; w++) {
+        const float lw = join_l[w][row];
+        sum += lw == 0.0f ? 0.0f : lw * ex2(join_m[w][row] - (top == NEG_INF ? 0.0f : top));
+        val += join_o[(w * ROWS + row) * D + d];
+      }
+      if (!whole) {
+        __stcg(mine + row * D + d, val);
+        if (d == 0) { __stcg(mine + ROWS * D + row, top); __stcg(mine + ROWS * D + ROWS + row, sum); }
+      } else if (row < rows_here) {
+        int t;
+        a.out[row_offset(a, b, head, rb * ROWS + row, a.ld_o, D, t) + d] = sum == 0.0f ? 0.0f : val / sum;
+      }
+    }
+    // ---- the last piece of an item to arrive joins all of them, in the order of the runs
+    if (!whole) {
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) arrived = atomicAdd(a.counters + run0, 1u);
+      __syncthreads();
+      if (arrived == (uint32_t)(run1 - run0)) {
+        __threadfence();
+        if (tid == 0) a.counters[run0] = 0;
+#pragma unroll 1
+        for (int x = 0; x < ROWS * D / (32 * FEW_WARPS); x++) {
+          const int row = (x * 32 * FEW_WARPS + tid) / D, d = tid % D;
+          if (row >= rows_here) continue;
+          auto piece = [&](int c) { return a.slots + (int64_t)(2 * c + (c == run0 ? 1 : 0)) * KV_SLOT_FLOATS; };
+          float top = NEG_INF, sum = 0.0f, val = 0.0f;
+          for (int c = run0; c <= run1; c++) top = fmaxf(top, __ldcg(piece(c) + ROWS * D + row));
+          for (int c = run0; c <= run1; c++) {
+            const float* p = piece(c);
+            const float lc = __ldcg(p + ROWS * D + ROWS + row);
+            if (lc == 0.0f) continue;
+            const float f = ex2(__ldcg(p + ROWS * D + row) - (top == NEG_INF ? 0.0f : top));
+            sum = fmaf(lc, f, sum);
+            val = fmaf(__ldcg(p + row * D + d), f, val);
+          }
+          int t;
+          a.out[row_offset(a, b, head, rb * ROWS + row, a.ld_o, D, t) + d] = sum == 0.0f ? 0.0f : val / sum;
+        }
+      }
+    }
+    __syncthreads();                                            // the rings are about to be filled again
+    at += tile1 - tile0;
+    left -= tile1 - tile0;
+    tile0 = 0;
+    if (++head == a.g.heads) { head = 0; e++; }
   }
 }
 
+template <int D, int RG>
+int launch_few(b200q_ctx* ctx, const AttnArgs& a) {
+  const int smem = Few<D>::RING + Few<D>::Q_BYTES(RG);
+  B200Q_CHECK_CUDA(cudaFuncSetAttribute(kv_attention_few_kernel<D, RG>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  const int row_blocks = (int)(((int64_t)a.T * a.group + 8 * RG - 1) / (8 * RG));
+  kv_attention_few_kernel<D, RG><<<ctx->sm_count * KV_BLOCKS_PER_SM, 32 * FEW_WARPS, smem, ctx->stream>>>(a, row_blocks);
+  return 0;
+}
+
 }  // namespace
+
+int kv_workspace(b200q_ctx* ctx) {
+  if (ctx->ws_kv.ptr) return 0;
+  const size_t bytes = kv_counter_bytes(ctx) + (size_t)ctx->sm_count * KV_BLOCKS_PER_SM * 2 * KV_SLOT_FLOATS * sizeof(float);
+  if (int e = ws_reserve(ctx, ctx->ws_kv, bytes)) return e;
+  B200Q_CHECK_CUDA(cudaMemsetAsync(ctx->ws_kv.ptr, 0, kv_counter_bytes(ctx), ctx->stream));
+  return 0;
+}
 
 int launch_kv_attention(b200q_ctx* ctx, const b200q_kv_cache& c, const KvBatch& s, const float* q, int64_t ld_q, int H, const uint64_t* tree,
                         float scale, float* out, int64_t ld_o) {
   ProfScope prof(ctx, KK_KV_ATTENTION);
   const AttnArgs a{KvGeom{c.pages, s.max_pages, c.page_shift, c.heads}, c.k, c.v, c.ks, c.vs, s.page_table, s.start, s.count, tree, q, out,
-                   ld_q, ld_o, s.B, s.T, H, H / c.heads, scale, ctx->status_dev};
-  const unsigned grid = (unsigned)s.B * (unsigned)s.T * (unsigned)H;
-  if (c.head_dim == 64) kv_attention_kernel<64><<<grid, 128, 0, ctx->stream>>>(a);
-  else kv_attention_kernel<128><<<grid, 128, 0, ctx->stream>>>(a);
+                   ld_q, ld_o, s.B, s.T, H, H / c.heads, scale * 1.4426950408889634f, ctx->status_dev, (uint32_t*)ctx->ws_kv.ptr,
+                   (float*)((uint8_t*)ctx->ws_kv.ptr + kv_counter_bytes(ctx))};
+  const int64_t rows = (int64_t)s.T * a.group;
+  int e;
+  if (c.head_dim == 64) e = rows <= 8 ? launch_few<64, 1>(ctx, a) : launch_few<64, 2>(ctx, a);
+  else e = rows <= 8 ? launch_few<128, 1>(ctx, a) : launch_few<128, 2>(ctx, a);
+  if (e) return e;
   ctx->launches++;
   B200Q_CHECK_CUDA(cudaGetLastError());
   return 0;

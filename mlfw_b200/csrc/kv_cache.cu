@@ -250,6 +250,9 @@ int b200q_kv_create(b200q_ctx* ctx, int64_t pages, int64_t page_tokens, int64_t 
   B200Q_REQUIRE(kv_aligned(k_codes, 16) && kv_aligned(v_codes, 16) && kv_aligned(k_scales, 16) && kv_aligned(v_scales, 16),
                 "b200q_kv_create: the cache's buffers must start on 16-byte boundaries");
   B200Q_REQUIRE(ctx != nullptr, "b200q_kv_create: null context");
+  B200Q_REQUIRE(!ctx->capturing, "b200q_kv_create is not allowed between b200q_graph_begin and b200q_graph_end");
+  B200Q_CHECK_CUDA(cudaSetDevice(ctx->device));
+  if (int e = kv_workspace(ctx)) return e;
   b200q_kv_cache* c = new (std::nothrow) b200q_kv_cache();
   B200Q_REQUIRE(c != nullptr, "b200q_kv_create: out of host memory");
   c->ctx = ctx;

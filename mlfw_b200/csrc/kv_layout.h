@@ -45,6 +45,29 @@ B200Q_HD int kv_rows_in_use(const int32_t* count, int64_t b, int T) {
   return c < 0 ? 0 : (c > T ? T : c);
 }
 
+// ---------------------------------------------------------------------------------------------- work of the attention
+// An item is one block of `rows` query rows (row R = t * group + query head within the group) of one sequence and one cache head; its
+// work is the 16-token tiles of the positions any of its rows sees.  All items' tiles, in the order (sequence, row block,
+// head, tile), are cut into equal runs, one per block of the grid.  An item that spans several runs is joined from its pieces.
+constexpr int KV_TILE = 16;
+
+// Positions visible to row block rb of a sequence with `n` rows in use: [0, result).
+B200Q_HD int64_t kv_visible(const KvGeom& g, int64_t start, int n, int group, int rows, int rb, bool tree) {
+  const int64_t last = (int64_t)(rb + 1) * rows - 1;                       // last row of the block
+  const int64_t t = last / group + 1;                                     // new tokens its rows reach without a tree
+  const int64_t vis = start + (tree || t > n ? n : t), most = g.max_pages << g.page_shift;
+  return vis < 0 ? 0 : (vis > most ? most : vis);
+}
+// Tiles of that block: none when it has no row in use, else at least one (a block that sees nothing still writes zeros).
+B200Q_HD int kv_tiles(const KvGeom& g, int64_t start, int n, int group, int rows, int rb, bool tree, int tile) {
+  if ((int64_t)rb * rows >= (int64_t)n * group) return 0;
+  const int64_t vis = kv_visible(g, start, n, group, rows, rb, tree);
+  return vis <= tile ? 1 : (int)((vis + tile - 1) / tile);
+}
+// Runs: the first tile of run c of `runs` (runs <= total), and the run that holds a tile.
+B200Q_HD int64_t kv_run_begin(int64_t total, int64_t runs, int64_t c) { return total * c / runs; }
+B200Q_HD int64_t kv_run_of(int64_t total, int64_t runs, int64_t tile) { return ((tile + 1) * runs - 1) / total; }
+
 // ---------------------------------------------------------------------------------------------- refusals (host)
 // Each returns null when the call is in order, else the reason.
 inline const char* kv_refuse_geometry(int64_t pages, int64_t page_tokens, int64_t heads, int64_t head_dim) {

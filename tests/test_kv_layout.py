@@ -9,15 +9,63 @@ import pytest
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 SOURCE = r"""
+#include <vector>
 #include "kv_layout.h"
 using namespace b200q;
 extern "C" {
 int64_t row(int64_t pages, int64_t max_pages, int shift, int heads, const int32_t* table, int64_t b, int head, int64_t pos) {
   return kv_row(KvGeom{pages, max_pages, shift, heads}, table, b, head, pos);
 }
+int64_t visible(int64_t mp, int shift, int64_t start, int n, int group, int rows, int rb, int tree) { return kv_visible(KvGeom{1, mp, shift, 1}, start, n, group, rows, rb, tree); }
+int tiles(int64_t mp, int shift, int64_t start, int n, int group, int rows, int rb, int tree, int tile) { return kv_tiles(KvGeom{1, mp, shift, 1}, start, n, group, rows, rb, tree, tile); }
 int in_use(const int32_t* count, int64_t b, int T) { return kv_rows_in_use(count, b, T); }
 const char* geometry(int64_t p, int64_t t, int64_t h, int64_t d) { return kv_refuse_geometry(p, t, h, d); }
 const char* batch(int64_t B, int64_t T, int64_t h, const void* table, int64_t mp, const void* start) { return kv_refuse_batch(B, T, h, table, mp, start); }
+// The walk of the attention kernels over a batch, block by block as the device does it: every (item, tile) an owner, every slot of the
+// join written once, every item's pieces as many as its last one expects.  Returns 0, or which of these fails.
+int walk(int B, int T, int heads, int group, int rows, int warps, int grid, int64_t max_pages, int shift, const int32_t* start, const int32_t* count,
+         int tree, int tile_tokens, int64_t* total_out) {
+  const KvGeom g{1, max_pages, shift, heads};
+  const int rbs = (int)(((int64_t)T * group + rows - 1) / rows);
+  std::vector<int64_t> begin;                      // first tile of (e, head)
+  std::vector<int> tiles;
+  int64_t total = 0;
+  for (int e = 0; e < B * rbs; e++) {
+    const int n = kv_tiles(g, start[e / rbs], kv_rows_in_use(count, e / rbs, T), group, rows, e % rbs, tree, tile_tokens);
+    for (int h = 0; h < heads; h++) { begin.push_back(total); tiles.push_back(n); total += n; }
+  }
+  *total_out = total;
+  if (total == 0) return 0;
+  int64_t want = total / warps;
+  const int64_t runs = want < 1 ? 1 : (want < grid ? want : grid);
+  std::vector<int> slot(2 * grid, 0), pieces(begin.size(), 0), expected(begin.size(), 0), counter(grid, -1);
+  size_t item = 0;
+  int64_t covered = 0;
+  for (int64_t c = 0; c < runs; c++) {
+    int64_t at = kv_run_begin(total, runs, c), end = kv_run_begin(total, runs, c + 1);
+    if (at != covered || end <= at) return 1;
+    covered = end;
+    while (at < end) {
+      while (tiles[item] == 0 || begin[item] + tiles[item] <= at) item++;
+      const int64_t t0 = at - begin[item], t1 = tiles[item] < t0 + end - at ? tiles[item] : t0 + end - at;
+      if (t0 < 0 || t1 <= t0) return 2;
+      if (!(t0 == 0 && t1 == tiles[item])) {
+        const int64_t r0 = kv_run_of(total, runs, begin[item]), r1 = kv_run_of(total, runs, begin[item] + tiles[item] - 1);
+        if (r0 > c || r1 < c || r0 < 0 || r1 >= runs || (t0 == 0) != (r0 == c)) return 3;
+        if (slot[2 * c + (t0 == 0 ? 1 : 0)]++) return 4;
+        if (counter[r0] >= 0 && counter[r0] != (int)item) return 5;
+        counter[r0] = (int)item;
+        pieces[item]++;
+        expected[item] = (int)(r1 - r0 + 1);
+      }
+      at += t1 - t0;
+    }
+  }
+  if (covered != total) return 6;
+  for (size_t i = 0; i < begin.size(); i++)
+    if (pieces[i] != expected[i]) return 7;
+  return 0;
+}
 const char* rows(const void* base, int64_t ld, int64_t h, int64_t d) { return kv_refuse_rows(base, ld, h, d); }
 }
 """
@@ -34,6 +82,9 @@ def host(tmp_path_factory):
     i64, vp = C.c_int64, C.c_void_p
     lib.row.restype, lib.row.argtypes = i64, [i64, i64, C.c_int, C.c_int, vp, i64, C.c_int, i64]
     lib.in_use.argtypes = [vp, i64, C.c_int]
+    lib.walk.argtypes = [C.c_int] * 7 + [i64, C.c_int, vp, vp, C.c_int, C.c_int, C.POINTER(i64)]
+    lib.visible.restype, lib.visible.argtypes = i64, [i64, C.c_int, i64] + [C.c_int] * 5
+    lib.tiles.argtypes = [i64, C.c_int, i64] + [C.c_int] * 6
     for f, a in (("geometry", [i64] * 4), ("batch", [i64, i64, i64, vp, i64, vp]), ("rows", [vp, i64, i64, i64])):
         getattr(lib, f).restype, getattr(lib, f).argtypes = C.c_char_p, a
     return lib
@@ -63,6 +114,45 @@ def test_positions_outside_have_no_row(host):
 def test_rows_in_use(host):
     c = np.array([-3, 0, 2, 9], np.int32)
     assert [host.in_use(c.ctypes.data, b, 4) for b in range(4)] == [0, 0, 2, 4] and host.in_use(None, 7, 4) == 4
+
+
+def test_the_runs_cover_every_tile_once(host):
+    rng = np.random.default_rng(5)
+    total = C.c_int64()
+    seen = 0
+    for _ in range(3000):
+        B, T, heads, group = (int(rng.integers(1, m)) for m in (9, 70, 5, 9))
+        rows, warps, grid = int(rng.choice([8, 16, 128])), int(rng.choice([1, 8])), int(rng.choice([1, 7, 148, 296]))
+        shift, tile = int(rng.integers(4, 9)), int(rng.choice([16, 64]))
+        most = int(rng.choice([1, 40, 3000]))
+        max_pages = -(-(most + T) // (1 << shift)) if rng.random() < 0.9 else int(rng.integers(0, 3))
+        start = rng.integers(0, most + 1, B).astype(np.int32)
+        if rng.random() < 0.1:
+            start[rng.integers(0, B)] = rng.choice([-5, -(2**31), 2**31 - 1])
+        count = rng.integers(-1, T + 2, B).astype(np.int32)
+        code = host.walk(B, T, heads, group, rows, warps, grid, max_pages, shift, start.ctypes.data, count.ctypes.data if rng.random() < 0.8 else None,
+                         int(T <= 64 and rng.random() < 0.5), tile, C.byref(total))
+        assert code == 0, (code, B, T, heads, group, rows, warps, grid, max_pages, shift, start, count)
+        seen += total.value > 8 * grid
+    assert seen > 100
+
+
+def test_visible_positions(host):
+    """kv_visible against the rule, row by row: the largest position any row of a block sees."""
+    rng = np.random.default_rng(6)
+    for _ in range(500):
+        T, group, rows = (int(rng.integers(1, m)) for m in (50, 9, 33))
+        start, n, tree = int(rng.integers(0, 100)), 0, bool(rng.integers(0, 2))
+        n = int(rng.integers(1, T + 1))
+        for rb in range(-(-n * group // rows)):
+            used = range(rb * rows, min((rb + 1) * rows, n * group))
+            want = start + (n if tree else max(R // group for R in used) + 1)
+            assert host.visible(64, 4, start, n, group, rows, rb, tree) == want
+            assert host.tiles(64, 4, start, n, group, rows, rb, tree, 16) == -(-want // 16)
+        past = -(-n * group // rows)
+        assert host.tiles(64, 4, start, n, group, rows, past, tree, 16) == 0
+    assert host.visible(2, 4, 100, 3, 1, 8, 0, False) == 32 and host.visible(2, 4, -100, 3, 1, 8, 0, False) == 0
+    assert host.tiles(2, 4, -100, 3, 1, 8, 0, False, 16) == 1 and host.tiles(0, 4, 0, 3, 1, 8, 0, True, 16) == 1
 
 
 def test_refusals(host):
