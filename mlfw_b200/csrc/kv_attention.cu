@@ -9,9 +9,12 @@
 //     sum_d q_d code_d = 2^(e-22) * (2^12 * sum hi code + sum lo code),
 // two binary16 products with binary32 sums; the first is a sum of integers below 2^25 at worst and below 2^24 for all
 // ordinary rows, so it is exact, and a score carries the rounding of q (2^-23 of the row's largest element) and the one
-// of adding the two.  The weights p * scale_v are split the same way against their running maximum of the row.  So the
-// cache's codes go into the tensor cores as they are, and the result has binary32 accuracy at two binary16 products per
-// contraction.
+// of adding the two.  The weights are split the same way: with z the score in units of log2 and the row's running
+//     c = max over the keys of (z + log2 scale_v) - 22,      p = 2^(z - c),      w = p * scale_v <= 2^22 (1 + 2^-20),
+// the row's result is sum w code / sum p, so one running number per row replaces the softmax's maximum and the weights'
+// exponent, and a key whose score is high but whose scale is small (or the other way round) costs no precision.  log2 of
+// the scale only steers c, so the approximate one does; it is held above -78, which keeps p below 2^100.  So the cache's
+// codes go into the tensor cores as they are, and the result has binary32 accuracy at two binary16 products per contraction.
 #include <cuda_fp16.h>
 
 #include "kernels.cuh"
@@ -38,11 +41,17 @@ struct AttnArgs {
 };
 
 constexpr float NEG_INF = -__builtin_huge_valf();
+constexpr float C_NONE = -3.0e38f;       // c of a row that has seen nothing: finite, so that differences with it are numbers
 
 __device__ __forceinline__ float ex2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
+}
+__device__ __forceinline__ float log2_scale(float s) {
+  float r;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
+  return fmaxf(r, -78.0f);
 }
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
@@ -66,9 +75,14 @@ __device__ __forceinline__ float2 lds_f2(uint32_t a) {
   return make_float2(__uint_as_float(r.x), __uint_as_float(r.y));
 }
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint4& a, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-               : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma16816_first(float (&c)[4], const uint4& a, uint32_t b0, uint32_t b1) {   // c = a b
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "f"(0.0f));
 }
 // Bytes 0 and 2 (even) or 1 and 3 (odd) of a word of codes as two binary16 numbers: the byte with its sign bit flipped
 // under the exponent of 1024 is 1024 + 128 + code; subtracting 1152 is exact.
@@ -190,11 +204,18 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, 2) kv_attention_few_kernel(con
   using C = Few<D>;
   constexpr int ROWS = 8 * RG, NT = D / 8, KS = D / 16, CH = D / 8;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float join_m[FEW_WARPS][ROWS], join_l[FEW_WARPS][ROWS];
+  __shared__ float join_c[FEW_WARPS][ROWS], join_l[FEW_WARPS][ROWS];
   __shared__ uint32_t arrived;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, t4 = lane & 3;
   const uint32_t ring = smem_u32(smem) + warp * (C::STAGES * C::TILE), q_smem = smem_u32(smem) + C::RING;
   float* join_o = reinterpret_cast<float*>(smem);               // [warp][row][D], over the rings between pieces
+
+  // Places of a lane's pieces in a slot.  Of the swizzle only a flip of 64 bytes depends on more than the lane: pieces 32 lanes
+  // apart are 512 bytes apart (V, D = 128: every second one flipped), tokens eight apart half a tile of rows apart.
+  const uint32_t k_dst = ring + k_at<D>(lane / (D / 16), lane % (D / 16)), v_dst = ring + KV_TILE * D + v_at<D>(lane / (D / 16), lane % (D / 16));
+  const uint32_t k_src = ring + k_at<D>(g8, t4);
+  const uint32_t v_src = ring + KV_TILE * D + (D == 128 ? v_at<D>(2 * t4, g8) : v_at<D>(2 * t4, g8 >> 1) + (g8 & 1) * 8);
+  const uint32_t q_src = q_smem + lane * 16;
 
   const Run run = find_run<ROWS>(a, row_blocks, FEW_WARPS);
   int64_t left = run.end - run.begin;
@@ -215,22 +236,19 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, 2) kv_attention_few_kernel(con
     // ---- the ring: tile i of the item into slot s
     const int32_t* table = a.page_table + (int64_t)b * a.g.max_pages;
     const int per_page = a.g.page_shift - 4;                    // log2 tiles per page
-    auto page_of = [&](int i) -> int { return (i < tile1 && ((int64_t)i >> per_page) < a.g.max_pages) ? __ldg(table + (i >> per_page)) : -1; };
+    const int in_table = (int)min((int64_t)tile1, a.g.max_pages << per_page);
+    auto page_of = [&](int i) -> int { return i < in_table ? __ldg(table + (i >> per_page)) : -1; };
     auto fetch = [&](int i, int page, int s) {
-      if (i < tile1 && page >= 0 && page < a.g.pages) {
+      if ((uint32_t)page < (uint32_t)a.g.pages) {               // -1 behind the piece's end
         const int64_t row = (((int64_t)page * a.g.heads + head) << a.g.page_shift) + ((i & ((1 << per_page) - 1)) << 4);
-        const uint32_t dst = ring + s * C::TILE;
+        const uint32_t slot_at = s * C::TILE;
+        const int64_t off = row * D + lane * 16;
+        const int8_t *kp = a.k + off, *vp = a.v + off;
 #pragma unroll
-        for (int x = 0; x < D / 32; x++) {
-          const int c = x * 32 + lane, t = c / (D / 16), p = c % (D / 16);
-          cp16(dst + k_at<D>(t, p), a.k + row * D + c * 16);
-        }
+        for (int x = 0; x < D / 32; x++) cp16(k_dst + slot_at + x * 512, kp + x * 512);
 #pragma unroll
-        for (int x = 0; x < D / 32; x++) {
-          const int c = x * 32 + lane, t = c / (D / 16), p = c % (D / 16);
-          cp16(dst + KV_TILE * D + v_at<D>(t, p), a.v + row * D + c * 16);
-        }
-        if (lane < 8) cp16(dst + 2 * KV_TILE * D + lane * 16, (lane < 4 ? a.ks : a.vs) + row + (lane & 3) * 4);
+        for (int x = 0; x < D / 32; x++) cp16(((D == 128 && (x & 1)) ? v_dst ^ 64u : v_dst) + slot_at + x * 512, vp + x * 512);
+        if (lane < 8) cp16(ring + 2 * KV_TILE * D + lane * 16 + slot_at, (lane < 4 ? a.ks : a.vs) + row + (lane & 3) * 4);
       }
       cp_commit();
     };
@@ -281,11 +299,10 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, 2) kv_attention_few_kernel(con
     }
     __syncthreads();
 
-    float o[RG][NT][2], m[RG], l[RG], xr[RG];
-    int ex_w[RG];                                               // weights are held as w * 2^(22 - ex_w)
+    float o[RG][NT][2], c_run[RG], l[RG];
 #pragma unroll
     for (int r = 0; r < RG; r++) {
-      m[r] = NEG_INF; l[r] = 0.0f; xr[r] = 0.0f; ex_w[r] = -103;
+      c_run[r] = C_NONE; l[r] = 0.0f;
 #pragma unroll
       for (int i = 0; i < NT; i++) o[r][i][0] = o[r][i][1] = 0.0f;
     }
@@ -301,31 +318,35 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, 2) kv_attention_few_kernel(con
       page_q[C::STAGES - 2] = page_next;
       fetch(i + (C::STAGES - 1) * FEW_WARPS, page_next, slot == 0 ? C::STAGES - 1 : slot - 1);
       page_next = page_of(i + C::STAGES * FEW_WARPS);
-      const uint32_t kt = ring + slot * C::TILE, vt = kt + KV_TILE * D, sc = vt + KV_TILE * D;
+      const uint32_t slot_at = slot * C::TILE, sc = ring + 2 * KV_TILE * D + slot_at;
       slot = slot + 1 == C::STAGES ? 0 : slot + 1;
-      if (page < 0 || page >= a.g.pages) {                      // no such page: nothing of the tile is visible
+      if ((uint32_t)page >= (uint32_t)a.g.pages) {              // no such page: nothing of the tile is visible
         if (lane == 0 && (int64_t)i * KV_TILE < vis) atomicOr(a.status, STATUS_BAD_INDEX);
         continue;
       }
 
       // ---- scores: two blocks of eight tokens
-      float acc[RG][2][4];
-#pragma unroll
-      for (int r = 0; r < RG; r++)
-#pragma unroll
-        for (int j = 0; j < 2; j++) acc[r][j][0] = acc[r][j][1] = acc[r][j][2] = acc[r][j][3] = 0.0f;
+      constexpr int CHAINS = RG == 1 ? D / 64 : 1;              // independent sums, to be added (exactly) at the end
+      float acc[RG][2 * CHAINS][4];
 #pragma unroll
       for (int mm = 0; mm < D / 64; mm++) {
-        const uint4 x0 = lds128(kt + k_at<D>(g8, mm * 4 + t4)), x1 = lds128(kt + k_at<D>(8 + g8, mm * 4 + t4));
+        const uint32_t at_k = (mm ? k_src ^ 64u : k_src) + slot_at;
+        const uint4 x0 = lds128(at_k), x1 = lds128(at_k + 8 * D);
         const uint32_t w0[4] = {x0.x, x0.y, x0.z, x0.w}, w1[4] = {x1.x, x1.y, x1.z, x1.w};
 #pragma unroll
         for (int w = 0; w < 4; w++) {
           const uint32_t b00 = codes_even(w0[w]), b01 = codes_odd(w0[w]), b10 = codes_even(w1[w]), b11 = codes_odd(w1[w]);
 #pragma unroll
           for (int r = 0; r < RG; r++) {
-            const uint4 qa = lds128(q_smem + (r * KS + mm * 4 + w) * 512 + lane * 16);
-            mma16816(acc[r][0], qa, b00, b01);
-            mma16816(acc[r][1], qa, b10, b11);
+            const uint4 qa = lds128(q_src + (r * KS + mm * 4 + w) * 512);
+            const int j = CHAINS == 2 ? 2 * mm : 0;
+            if (w == 0 && (mm == 0 || CHAINS == 2)) {
+              mma16816_first(acc[r][j], qa, b00, b01);
+              mma16816_first(acc[r][j + 1], qa, b10, b11);
+            } else {
+              mma16816(acc[r][j], qa, b00, b01);
+              mma16816(acc[r][j + 1], qa, b10, b11);
+            }
           }
         }
       }
@@ -333,10 +354,20 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, 2) kv_attention_few_kernel(con
       float2 vs0 = lds_f2(sc + 64 + t4 * 8), vs1 = lds_f2(sc + 96 + t4 * 8);
       const int64_t pos = (int64_t)i * KV_TILE;
       const bool edge = pos + KV_TILE > first;                  // some position of the tile is among the new rows or behind them
+      if (edge) {                                               // behind the last row in use anything may stand
+        const int64_t end = min(vis, first + n);
+        vs0.x = pos + t4 * 2 < end ? vs0.x : 0.0f; vs0.y = pos + t4 * 2 + 1 < end ? vs0.y : 0.0f;
+        vs1.x = pos + 8 + t4 * 2 < end ? vs1.x : 0.0f; vs1.y = pos + 8 + t4 * 2 + 1 < end ? vs1.y : 0.0f;
+      }
+      const float lv0 = log2_scale(vs0.x), lv1 = log2_scale(vs0.y), lv2 = log2_scale(vs1.x), lv3 = log2_scale(vs1.y);
       uint4 pa[RG];
       float fold[RG];
 #pragma unroll
       for (int r = 0; r < RG; r++) {
+        if (CHAINS == 2) {
+#pragma unroll
+          for (int c = 0; c < 8; c++) acc[r][c >> 2][c & 3] += acc[r][2 * CHAINS - 2 + (c >> 2)][c & 3];
+        }
         float z[4];
         z[0] = fmaf(acc[r][0][0], 4096.0f, acc[r][0][2]) * (ks0.x * row_scale[r]);
         z[1] = fmaf(acc[r][0][1], 4096.0f, acc[r][0][3]) * (ks0.y * row_scale[r]);
@@ -346,32 +377,20 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, 2) kv_attention_few_kernel(con
 #pragma unroll
           for (int c = 0; c < 4; c++) {
             const int64_t j = pos + (c >> 1) * 8 + t4 * 2 + (c & 1) - first;
-            const bool seen = j < 0 ? pos + (c >> 1) * 8 + t4 * 2 + (c & 1) < vis : (j < n && (a.tree ? (row_seen[r] >> j) & 1 : j <= row_t[r]) && first + j < vis);
+            const bool seen = first + j < vis && (j < 0 || (j < n && (a.tree ? (row_seen[r] >> j) & 1 : j <= row_t[r])));
             if (!seen) z[c] = NEG_INF;
-            if (j >= n || first + j >= vis) (c == 0 ? vs0.x : c == 1 ? vs0.y : c == 2 ? vs1.x : vs1.y) = 0.0f;   // unwritten: may be anything
           }
         }
-        float mx = fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3]));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float m_new = fmaxf(m[r], mx), m_use = m_new == NEG_INF ? 0.0f : m_new;   // nothing visible yet: p = 0 throughout
-        const float alpha = ex2(m[r] - m_use);
-        m[r] = m_new;
-        const float p0 = ex2(z[0] - m_use), p1 = ex2(z[1] - m_use), p2 = ex2(z[2] - m_use), p3 = ex2(z[3] - m_use);
-        l[r] = fmaf(l[r], alpha, (p0 + p1) + (p2 + p3));
-        // weights p * scale_v in fixed point against the row's largest so far
-        float x0 = p0 * vs0.x, x1 = p1 * vs0.y, x2 = p2 * vs1.x, x3 = p3 * vs1.y;
-        float xm = fmaxf(fmaxf(x0, x1), fmaxf(x2, x3));
-        xm = fmaxf(xm, __shfl_xor_sync(0xffffffffu, xm, 1));
-        xm = fmaxf(xm, __shfl_xor_sync(0xffffffffu, xm, 2));
-        xr[r] = fmaxf(xr[r] * alpha, xm);
-        const int ex = max(__float_as_int(xr[r]) >> 23, 24) - 127;   // -103 .. 128
-        const float up = pow2(22 - ex);
-        const int d = ex_w[r] - ex;
-        fold[r] = alpha * pow2(d > 126 ? 126 : (d < -126 ? -126 : d));
-        ex_w[r] = ex;
+        float top = fmaxf(fmaxf(z[0] + lv0, z[1] + lv1), fmaxf(z[2] + lv2, z[3] + lv3));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const float c_new = fmaxf(c_run[r], top - 22.0f);
+        fold[r] = ex2(c_run[r] - c_new);
+        c_run[r] = c_new;
+        const float p0 = ex2(z[0] - c_new), p1 = ex2(z[1] - c_new), p2 = ex2(z[2] - c_new), p3 = ex2(z[3] - c_new);
+        l[r] = fmaf(l[r], fold[r], (p0 + p1) + (p2 + p3));
         float h0, h1, h2, h3, l0, l1, l2, l3;
-        split12(x0 * up, h0, l0); split12(x1 * up, h1, l1); split12(x2 * up, h2, l2); split12(x3 * up, h3, l3);
+        split12(p0 * vs0.x, h0, l0); split12(p1 * vs0.y, h1, l1); split12(p2 * vs1.x, h2, l2); split12(p3 * vs1.y, h3, l3);
         pa[r] = make_uint4(pack_f16(h0, h1), pack_f16(l0, l1), pack_f16(h2, h3), pack_f16(l2, l3));
       }
 
@@ -380,12 +399,11 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, 2) kv_attention_few_kernel(con
         uint32_t y[4][D / 32];
 #pragma unroll
         for (int c = 0; c < 4; c++) {
-          const int t = 2 * t4 + (c & 1) + (c >> 1) * 8;
           if (D == 128) {
-            const uint4 w = lds128(vt + v_at<D>(t, g8));
+            const uint4 w = lds128(v_src + slot_at + (c & 1) * 128 + (c >> 1) * 1024);
             y[c][0] = w.x; y[c][1] = w.y; y[c][D / 32 - 2] = w.z; y[c][D / 32 - 1] = w.w;
           } else {
-            const uint2 w = lds64(vt + v_at<D>(t, g8 >> 1) + (g8 & 1) * 8);
+            const uint2 w = lds64(((c & 1) ? v_src ^ 64u : v_src) + slot_at + (c >> 1) * 512);
             y[c][0] = w.x; y[c][1] = w.y;
           }
         }
@@ -400,8 +418,8 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, 2) kv_attention_few_kernel(con
               const uint32_t b0 = odd ? codes_odd(lo) : codes_even(lo), b1 = odd ? codes_odd(hi) : codes_even(hi);
 #pragma unroll
               for (int r = 0; r < RG; r++) {
-                float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                mma16816(c, pa[r], b0, b1);
+                float c[4];
+                mma16816_first(c, pa[r], b0, b1);
                 o[r][d][0] = fmaf(o[r][d][0], fold[r], fmaf(c[0], 4096.0f, c[2]));
                 o[r][d][1] = fmaf(o[r][d][1], fold[r], fmaf(c[1], 4096.0f, c[3]));
               }
@@ -416,17 +434,16 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, 2) kv_attention_few_kernel(con
     for (int r = 0; r < RG; r++) {
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-      if (t4 == 0) { join_m[warp][r * 8 + g8] = m[r]; join_l[warp][r * 8 + g8] = l[r]; }
+      if (t4 == 0) { join_c[warp][r * 8 + g8] = c_run[r]; join_l[warp][r * 8 + g8] = l[r]; }
     }
     __syncthreads();                                            // every ring is drained
 #pragma unroll
     for (int r = 0; r < RG; r++) {
       const int row = r * 8 + g8;
-      float top = join_m[0][row];
+      float top = join_c[0][row];
 #pragma unroll
-      for (int w = 1; w < FEW_WARPS; w++) top = fmaxf(top, join_m[w][row]);
-      // the row's weights back from fixed point, relative to the block's maximum
-      const float f = ex2(m[r] - (top == NEG_INF ? 0.0f : top)) * pow2(ex_w[r] - 22);
+      for (int w = 1; w < FEW_WARPS; w++) top = fmaxf(top, join_c[w][row]);
+      const float f = ex2(c_run[r] - top);
       float* dst = join_o + (warp * ROWS + row) * D + t4 * 2 * CH;
 #pragma unroll
       for (int c = 0; c < 2; c++)
@@ -442,13 +459,12 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, 2) kv_attention_few_kernel(con
 #pragma unroll
     for (int x = 0; x < ROWS * D / (32 * FEW_WARPS); x++) {
       const int row = (x * 32 * FEW_WARPS + tid) / D, d = tid % D;
-      float top = join_m[0][row], sum = 0.0f, val = 0.0f;
+      float top = join_c[0][row], sum = 0.0f, val = 0.0f;
 #pragma unroll
-      for (int w = 1; w < FEW_WARPS; w++) top = fmaxf(top, join_m[w][row]);
+      for (int w = 1; w < FEW_WARPS; w++) top = fmaxf(top, join_c[w][row]);
 #pragma unroll
       for (int w = 0; w < FEW_WARPS; w++) {
-        const float lw = join_l[w][row];
-        sum += lw == 0.0f ? 0.0f : lw * ex2(join_m[w][row] - (top == NEG_INF ? 0.0f : top));
+        sum = fmaf(join_l[w][row], ex2(join_c[w][row] - top), sum);
         val += join_o[(w * ROWS + row) * D + d];
       }
       if (!whole) {
@@ -473,14 +489,12 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, 2) kv_attention_few_kernel(con
           const int row = (x * 32 * FEW_WARPS + tid) / D, d = tid % D;
           if (row >= rows_here) continue;
           auto piece = [&](int c) { return a.slots + (int64_t)(2 * c + (c == run0 ? 1 : 0)) * KV_SLOT_FLOATS; };
-          float top = NEG_INF, sum = 0.0f, val = 0.0f;
+          float top = C_NONE, sum = 0.0f, val = 0.0f;
           for (int c = run0; c <= run1; c++) top = fmaxf(top, __ldcg(piece(c) + ROWS * D + row));
           for (int c = run0; c <= run1; c++) {
             const float* p = piece(c);
-            const float lc = __ldcg(p + ROWS * D + ROWS + row);
-            if (lc == 0.0f) continue;
-            const float f = ex2(__ldcg(p + ROWS * D + row) - (top == NEG_INF ? 0.0f : top));
-            sum = fmaf(lc, f, sum);
+            const float f = ex2(__ldcg(p + ROWS * D + row) - top);
+            sum = fmaf(__ldcg(p + ROWS * D + ROWS + row), f, sum);
             val = fmaf(__ldcg(p + row * D + d), f, val);
           }
           int t;
