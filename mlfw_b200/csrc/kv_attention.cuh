@@ -1,0 +1,176 @@
+// Attention over the int8 key/value cache: softmax(scale * q k^T) v for new rows of a batch of sequences.
+//
+// Row t of sequence b sees the start[b] positions cached before and, of the count[b] new ones, those up to itself (no
+// tree) or those whose bit is set in its row of ancestors.  Query heads h of a group H / heads share cache head h / (H / heads).
+//
+// The arithmetic.  A cached value is code * scale with an integer |code| <= 128, which binary16 holds exactly.  A query
+// row is written in fixed point against its largest element, x = q * 2^(10 - e) with 2^e <= max|q| < 2^(e+1), and split
+// x = hi + lo, |hi| <= 2^11 an integer, |lo| <= 1/2: two binary16 numbers that keep 23 bits.  Then
+//     sum_d q_d code_d = 2^(e-10) * (sum hi code + sum lo code),
+// two binary16 products with binary32 sums; the first is a sum of integers below 2^25 at worst and below 2^24 for all
+// ordinary rows, so it is exact, and a score carries the rounding of q (2^-23 of the row's largest element) and the one
+// of adding the two.  The weights are split the same way: with z the score in units of log2 and the row's running
+//     c = max over the keys of (z + log2 scale_v) - 10,      p = 2^(z - c),      w = p * scale_v <= 2^10 (1 + 2^-20),
+// the row's result is sum w code / sum p, so one running number per row replaces the softmax's maximum and the weights'
+// exponent, and a key whose score is high but whose scale is small (or the other way round) costs no precision.  log2 of
+// the scale only steers c, so the approximate one does; it is held above -110 (a scale of 1e-33), which keeps p below 2^121; sums of
+// p are kept in units of 2^22.  So the cache's
+// codes go into the tensor cores as they are, and the result has binary32 accuracy at two binary16 products per contraction.
+#pragma once
+#include "kernels.cuh"
+#include "kv.cuh"
+namespace b200q {
+
+struct AttnArgs {
+  KvGeom g;
+  const int8_t *k, *v;
+  const float *ks, *vs;
+  const int32_t *page_table, *start, *count;
+  const uint64_t* tree;
+  const float* q;
+  float* out;
+  int64_t ld_q, ld_o;
+  int B, T, H, group;
+  float scale_log2e;       // scale * log2(e): scores are kept in units of log2
+  uint32_t* status;
+  uint32_t* counters;      // pieces of an item that have arrived, by the run the item begins in; zero between launches
+  float* slots;
+  int4* items;             // the item that begins in a run and goes on behind it: (e, head, last run, 1), else w = 0
+};
+
+int launch_kv_attention_many(b200q_ctx* ctx, const AttnArgs& a, int D);   // kv_attention_umma.cu
+
+namespace {
+
+
+constexpr float NEG_INF = -__builtin_huge_valf();
+constexpr float P_UNIT = 0x1p-22f;       // sums of p are held times this: up to 2^24 keys of weight 2^120 stay finite
+constexpr float C_NONE = -3.0e38f;       // c of a row that has seen nothing: finite, so that differences with it are numbers
+
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float log2_scale(float s) {
+  float r;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
+  return fmaxf(r, -110.0f);
+}
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 r;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a));
+  return r;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+  uint2 r;
+  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(a));
+  return r;
+}
+__device__ __forceinline__ float2 lds_f2(uint32_t a) {
+  const uint2 r = lds64(a);
+  return make_float2(__uint_as_float(r.x), __uint_as_float(r.y));
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma16816_first(float (&c)[4], const uint4& a, uint32_t b0, uint32_t b1) {   // c = a b
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "f"(0.0f));
+}
+// Bytes 0 and 2 (even) or 1 and 3 (odd) of a word of codes as two binary16 numbers: the byte with its sign bit flipped
+// under the exponent of 1024 is 1024 + 128 + code; subtracting 1152 is exact.
+__device__ __forceinline__ uint32_t codes_even(uint32_t x) {
+  const uint32_t y = (x & 0x00ff00ffu) ^ 0x64806480u;
+  uint32_t r;
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(y), "r"(0x64806480u));
+  return r;
+}
+__device__ __forceinline__ uint32_t codes_odd(uint32_t x) { return codes_even(x >> 8); }
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {   // lo in the low half
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// x = hi + lo for |x| <= 2^11: hi an integer (1.5 * 2^23 trick), lo exact.
+__device__ __forceinline__ void split_whole(float x, float& hi, float& lo) {
+  hi = __fsub_rn(__fadd_rn(x, 12582912.0f), 12582912.0f);
+  lo = __fsub_rn(x, hi);
+}
+__device__ __forceinline__ float pow2(int e) {   // 2^e for -126 <= e <= 127
+  return __int_as_float((e + 127) << 23);
+}
+
+// Where a query row comes from and its result goes: row R of the sequence (R = t * group + head within the group).
+__device__ __forceinline__ int64_t row_offset(const AttnArgs& a, int b, int head, int R, int64_t ld, int D, int& t) {
+  t = R / a.group;
+  return ((int64_t)b * a.T + t) * ld + (int64_t)(head * a.group + (R - t * a.group)) * D;
+}
+
+// The run of tiles this block works on: total tiles, the item its first tile belongs to (e = sequence * row
+// blocks + row block, head) and the tile inside it.  All threads take part and get the same answer.
+struct Run {
+  int64_t total, begin, end;
+  int runs, e, head, tile;
+};
+// ROWS query rows per item, TILE tokens per tile, at least LEAST tiles per run (a shorter one costs more in joining than it saves).
+template <int ROWS, int TILE, int LEAST>
+__device__ __forceinline__ Run find_run(const AttnArgs& a, int row_blocks) {
+  __shared__ int64_t warp_sum[33];
+  __shared__ int found[3];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int E = a.B * row_blocks, per = (E + blockDim.x - 1) / blockDim.x;
+  const int e0 = min(E, tid * per), e1 = min(E, e0 + per);
+  auto tiles = [&](int e) {
+    const int b = e / row_blocks;
+    return (int64_t)kv_tiles(a.g, a.start[b], kv_rows_in_use(a.count, b, a.T), a.group, ROWS, e - b * row_blocks, a.tree != nullptr, TILE) * a.g.heads;
+  };
+  int64_t mine = 0;
+  for (int e = e0; e < e1; e++) mine += tiles(e);
+  int64_t incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t x = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += x;
+  }
+  if (lane == 31) warp_sum[warp] = incl;
+  __syncthreads();
+  if (tid == 0) {
+    int64_t s = 0;
+    for (int w = 0; w < (int)blockDim.x / 32; w++) { const int64_t x = warp_sum[w]; warp_sum[w] = s; s += x; }
+    warp_sum[32] = s;
+  }
+  __syncthreads();
+  Run r;
+  r.total = warp_sum[32];
+  const int64_t want = r.total / LEAST;
+  r.runs = (int)(want < 1 ? 1 : (want < (int64_t)gridDim.x ? want : (int64_t)gridDim.x));
+  if ((int)blockIdx.x >= r.runs || r.total == 0) { r.begin = r.end = 0; return r; }
+  r.begin = kv_run_begin(r.total, r.runs, blockIdx.x);
+  r.end = kv_run_begin(r.total, r.runs, blockIdx.x + 1);
+  int64_t at = warp_sum[warp] + incl - mine;
+  if (r.begin >= at && r.begin < at + mine) {
+    int e = e0;
+    int64_t n = tiles(e);
+    while (r.begin >= at + n) { at += n; n = tiles(++e); }
+    const int64_t per_head = n / a.g.heads, in = r.begin - at;
+    found[0] = e; found[1] = (int)(in / per_head); found[2] = (int)(in % per_head);
+  }
+  __syncthreads();
+  r.e = found[0]; r.head = found[1]; r.tile = found[2];
+  return r;
+}
+
+}  // namespace
+
+}  // namespace b200q
