@@ -96,6 +96,7 @@ struct b200q_ctx {
   bool sdpa_umma_ready = false;          // ... and that of the tensor-core attention kernel
   int tail_mode = 0;                     // 0: exact sigmoid tails; 1: hardware exp / reciprocal for f32 outputs (tolerance only)
   int sdpa_variant = 0;                  // 0: tcgen05 with three-way tf32 products when the shape allows; 1: mma.sync, three-way tf32; 2: tcgen05 or fail; 3: CUDA-core binary32 FMA
+  uint32_t kv_ready = 0;                 // kernels of the attention over the cache whose shared-memory sizes have been raised
   uint64_t umma_ready_mask = 0;          // tensor-core kernel variants whose shared-memory attribute is set on this device
   uint64_t launches = 0;                 // kernels launched through this context
   bool capturing = false;                // between b200q_graph_begin and _end: calls are recorded, nothing may allocate or synchronise

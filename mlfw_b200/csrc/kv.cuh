@@ -29,6 +29,32 @@ inline size_t kv_item_bytes(const b200q_ctx* ctx) { return (size_t)ctx->sm_count
 inline size_t kv_counter_bytes(const b200q_ctx* ctx) { return ((size_t)ctx->sm_count * KV_BLOCKS_PER_SM * sizeof(uint32_t) + 255) & ~size_t(255); }
 int kv_workspace(b200q_ctx* ctx);
 
+// The calls on a cache follow one another within microseconds (append, attention, keep), so each kernel is launched as a
+// programmatic dependent of the one before it: its blocks come while that one drains, and kv_after_previous holds back
+// everything until it has completed.  With profiling on, an event sits between the two and the overlap is off.
+#ifdef __CUDACC__
+__device__ __forceinline__ void kv_after_previous() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+template <typename... P, typename... A>
+int kv_launch(b200q_ctx* ctx, void (*kernel)(P...), dim3 grid, int threads, size_t smem, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = ctx->stream;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = ctx->profiling ? 0 : 1;
+  B200Q_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, P(args)...));
+  ctx->launches++;
+  return 0;
+}
+#endif
+
 int launch_kv_append(b200q_ctx* ctx, const b200q_kv_cache& c, const KvBatch& s, const float* k, const float* v, int64_t ld_k, int64_t ld_v);
 int launch_kv_read(b200q_ctx* ctx, const b200q_kv_cache& c, const KvBatch& s, float* k_out, float* v_out, int64_t ld_k, int64_t ld_v);
 int launch_kv_keep(b200q_ctx* ctx, const b200q_kv_cache& c, const KvBatch& s, const int32_t* keep);

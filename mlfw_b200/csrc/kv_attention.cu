@@ -56,6 +56,7 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, 2) kv_attention_few_kernel(con
   const uint32_t v_src = ring + KV_TILE * D + (D == 128 ? v_at<D>(2 * t4, g8) : v_at<D>(2 * t4, g8 >> 1) + (g8 & 1) * 8);
   const uint32_t q_src = q_smem + lane * 16;
 
+  kv_after_previous();
   const Run run = find_run<ROWS, KV_TILE, FEW_WARPS>(a, row_blocks);
   int64_t left = run.end - run.begin;
   int e = run.e, head = run.head, tile0 = run.tile;
@@ -293,7 +294,7 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, 2) kv_attention_few_kernel(con
     __syncthreads();
     const bool whole = tile0 == 0 && tile1 == tiles;
     const int64_t item0 = at - tile0;                           // first tile of the item among all tiles
-    const int run0 = whole ? 0 : (int)kv_run_of(run.total, run.runs, item0), run1 = whole ? 0 : (int)kv_run_of(run.total, run.runs, item0 + tiles - 1);
+    const int run0 = whole ? 0 : kv_run_of(run.all, item0), run1 = whole ? 0 : kv_run_of(run.all, item0 + tiles - 1);
     float* mine = a.slots + (int64_t)(2 * blockIdx.x + (tile0 == 0 ? 1 : 0)) * KV_SLOT_FLOATS;
 #pragma unroll
     for (int x = 0; x < ROWS * D / (32 * FEW_WARPS); x++) {
@@ -352,10 +353,13 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, 2) kv_attention_few_kernel(con
 template <int D, int RG>
 int launch_few(b200q_ctx* ctx, const AttnArgs& a) {
   const int smem = Few<D>::RING + Few<D>::Q_BYTES(RG);
-  B200Q_CHECK_CUDA(cudaFuncSetAttribute(kv_attention_few_kernel<D, RG>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  constexpr uint32_t ready = 1u << ((D == 64 ? 0 : 2) + RG - 1);
+  if (!(ctx->kv_ready & ready)) {
+    B200Q_CHECK_CUDA(cudaFuncSetAttribute(kv_attention_few_kernel<D, RG>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    ctx->kv_ready |= ready;
+  }
   const int row_blocks = (int)(((int64_t)a.T * a.group + 8 * RG - 1) / (8 * RG));
-  kv_attention_few_kernel<D, RG><<<ctx->sm_count * KV_BLOCKS_PER_SM, 32 * FEW_WARPS, smem, ctx->stream>>>(a, row_blocks);
-  return 0;
+  return kv_launch(ctx, kv_attention_few_kernel<D, RG>, dim3(ctx->sm_count * KV_BLOCKS_PER_SM), 32 * FEW_WARPS, smem, a, row_blocks);
 }
 
 }  // namespace
@@ -381,10 +385,7 @@ int launch_kv_attention(b200q_ctx* ctx, const b200q_kv_cache& c, const KvBatch& 
   if (rows > 16) return launch_kv_attention_many(ctx, a, c.head_dim);
   if (c.head_dim == 64) e = rows <= 8 ? launch_few<64, 1>(ctx, a) : launch_few<64, 2>(ctx, a);
   else e = rows <= 8 ? launch_few<128, 1>(ctx, a) : launch_few<128, 2>(ctx, a);
-  if (e) return e;
-  ctx->launches++;
-  B200Q_CHECK_CUDA(cudaGetLastError());
-  return 0;
+  return e;
 }
 
 }  // namespace b200q

@@ -120,8 +120,9 @@ __device__ __forceinline__ int64_t row_offset(const AttnArgs& a, int b, int head
 // The run of tiles this block works on: total tiles, the item its first tile belongs to (e = sequence * row
 // blocks + row block, head) and the tile inside it.  All threads take part and get the same answer.
 struct Run {
-  int64_t total, begin, end;
-  int runs, e, head, tile;
+  KvRuns all;
+  int64_t begin, end;
+  int e, head, tile;
 };
 // ROWS query rows per item, TILE tokens per tile, at least LEAST tiles per run (a shorter one costs more in joining than it saves).
 template <int ROWS, int TILE, int LEAST>
@@ -152,19 +153,19 @@ __device__ __forceinline__ Run find_run(const AttnArgs& a, int row_blocks) {
   }
   __syncthreads();
   Run r;
-  r.total = warp_sum[32];
-  const int64_t want = r.total / LEAST;
-  r.runs = (int)(want < 1 ? 1 : (want < (int64_t)gridDim.x ? want : (int64_t)gridDim.x));
-  if ((int)blockIdx.x >= r.runs || r.total == 0) { r.begin = r.end = 0; return r; }
-  r.begin = kv_run_begin(r.total, r.runs, blockIdx.x);
-  r.end = kv_run_begin(r.total, r.runs, blockIdx.x + 1);
+  r.begin = r.end = 0;
+  if (warp_sum[32] == 0) return r;
+  r.all = kv_runs(warp_sum[32], LEAST, (int)gridDim.x);
+  if ((int)blockIdx.x >= r.all.runs) return r;
+  r.begin = kv_run_begin(r.all, (int)blockIdx.x);
+  r.end = kv_run_begin(r.all, (int)blockIdx.x + 1);
   int64_t at = warp_sum[warp] + incl - mine;
   if (r.begin >= at && r.begin < at + mine) {
     int e = e0;
     int64_t n = tiles(e);
     while (r.begin >= at + n) { at += n; n = tiles(++e); }
-    const int64_t per_head = n / a.g.heads, in = r.begin - at;
-    found[0] = e; found[1] = (int)(in / per_head); found[2] = (int)(in % per_head);
+    const int64_t per_head = kv_div(n, a.g.heads), in = r.begin - at, head = kv_div(in, per_head);
+    found[0] = e; found[1] = (int)head; found[2] = (int)(in - head * per_head);
   }
   __syncthreads();
   r.e = found[0]; r.head = found[1]; r.tile = found[2];

@@ -128,6 +128,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 2) kv_attention_many_kernel(cons
   const int copy = CS == 1 ? 0 : row / ROWS, rq = row % ROWS;    // which copy of which row of the item
   const int col0 = half * 32 + copy * NC;                        // this thread's tokens of a tile: col0 .. col0 + NC - 1
 
+  asm volatile("griddepcontrol.wait;" ::: "memory");             // the previous kernel of the stream wrote what is read here
   const Run run = find_run<ROWS, MT, 2>(a, mp.row_blocks);
   if (tid == 0 && blockIdx.x < gridDim.x) a.items[blockIdx.x] = make_int4(0, 0, 0, 0);
   if (run.begin == run.end) return;
@@ -143,6 +144,9 @@ __global__ void __launch_bounds__(MANY_THREADS, 2) kv_attention_many_kernel(cons
   }
   __syncthreads();
   fence_after();
+  // Only now may the next kernel's blocks come: one that allocates tensor memory before its own wait must not take what
+  // a block of this grid still needs.
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t tmem = tmem_slot, lane_tm = tmem + ((uint32_t)((warp & 3) * 32) << 16);
   const uint32_t bar_addr = smem_u32(&bar);
   uint32_t phase = 0;
@@ -488,7 +492,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 2) kv_attention_many_kernel(cons
     __syncthreads();
     const bool whole = tile0 == 0 && tile1 == tiles;
     if (tile0 == 0 && !whole && tid == 0)
-      a.items[blockIdx.x] = make_int4(e, head, (int)kv_run_of(run.total, run.runs, at + tiles - 1), 1);
+      a.items[blockIdx.x] = make_int4(e, head, kv_run_of(run.all, at + tiles - 1), 1);
     float* slot = a.slots + (int64_t)(2 * blockIdx.x + (tile0 == 0 ? 1 : 0)) * KV_SLOT_FLOATS;
     for (int x = tid; x < rows_here * (D / 4); x += MANY_THREADS) {
       const int r = x / (D / 4), p = x % (D / 4);
@@ -536,7 +540,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 2) kv_attention_many_kernel(cons
 template <int D, int ROWS>
 __global__ void __launch_bounds__(256) kv_attention_join_kernel(const AttnArgs a, int row_blocks) {
   constexpr int P = D / 4;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  kv_after_previous();
   const int run0 = blockIdx.x;
   const int4 item = __ldcg(a.items + run0);
   if (item.w == 0) return;
@@ -564,17 +568,17 @@ __global__ void __launch_bounds__(256) kv_attention_join_kernel(const AttnArgs a
 template <int D, int CS>
 int launch_many(b200q_ctx* ctx, const AttnArgs& a) {
   constexpr int ROWS = LANES / CS;
-  B200Q_CHECK_CUDA(cudaFuncSetAttribute(kv_attention_many_kernel<D, CS>, cudaFuncAttributeMaxDynamicSharedMemorySize, Many<D>::SMEM));
+  constexpr uint32_t ready = 1u << ((D == 64 ? 4 : 8) + CS / 2);   // CS = 1, 2, 4: bits 0, 1, 2 of four
+  if (!(ctx->kv_ready & ready)) {
+    B200Q_CHECK_CUDA(cudaFuncSetAttribute(kv_attention_many_kernel<D, CS>, cudaFuncAttributeMaxDynamicSharedMemorySize, Many<D>::SMEM));
+    ctx->kv_ready |= ready;
+  }
   ManyParams mp;
   mp.row_blocks = (int)(((int64_t)a.T * a.group + ROWS - 1) / ROWS);
   mp.limit_ns = (unsigned long long)(ctx->wait_limit_s * 1e9);
   const unsigned grid = (unsigned)ctx->sm_count * KV_BLOCKS_PER_SM;
-  kv_attention_many_kernel<D, CS><<<grid, MANY_THREADS, Many<D>::SMEM, ctx->stream>>>(a, mp);
-  B200Q_CHECK_CUDA(cudaGetLastError());
-  kv_attention_join_kernel<D, ROWS><<<dim3(grid, (ROWS + 15) / 16), 256, 0, ctx->stream>>>(a, mp.row_blocks);
-  B200Q_CHECK_CUDA(cudaGetLastError());
-  ctx->launches += 2;
-  return 0;
+  if (int e = kv_launch(ctx, kv_attention_many_kernel<D, CS>, dim3(grid), MANY_THREADS, Many<D>::SMEM, a, mp)) return e;
+  return kv_launch(ctx, kv_attention_join_kernel<D, ROWS>, dim3(grid, (ROWS + 15) / 16), 256, 0, a, mp.row_blocks);
 }
 
 }  // namespace

@@ -82,6 +82,7 @@ template <int D>
 __global__ void __launch_bounds__(256) kv_append_kernel(const KvArgs a, const float* __restrict__ k, const float* __restrict__ v, int64_t ld_k,
                                                         int64_t ld_v, uint32_t units, uint32_t chunks) {
   constexpr int V4 = D / 32;
+  kv_after_previous();
   const int lane = threadIdx.x & 31, sub = lane & 7;
   for (uint32_t u = (blockIdx.x * blockDim.x + threadIdx.x) >> 5; u < units; u += (gridDim.x * blockDim.x) >> 5) {
     const uint32_t token = u / chunks, head = (u - token * chunks) * 4 + (lane >> 3);
@@ -113,6 +114,7 @@ template <int D>
 __global__ void __launch_bounds__(256) kv_read_kernel(const KvArgs a, float* __restrict__ k_out, float* __restrict__ v_out, int64_t ld_k,
                                                       int64_t ld_v, uint32_t units, uint32_t chunks) {
   constexpr int V4 = D / 32;
+  kv_after_previous();
   const int lane = threadIdx.x & 31, sub = lane & 7;
   for (uint32_t u = (blockIdx.x * blockDim.x + threadIdx.x) >> 5; u < units; u += (gridDim.x * blockDim.x) >> 5) {
     const uint32_t token = u / chunks, head = (u - token * chunks) * 4 + (lane >> 3);
@@ -145,6 +147,7 @@ template <int D>
 __global__ void __launch_bounds__(128) kv_keep_kernel(const KvArgs a, const int32_t* __restrict__ keep) {
   constexpr int Q = D / 16, PER = KV_MAX_TREE * Q / 128;   // 16-byte pieces of a row; pieces a thread holds of K (and of V)
   __shared__ int64_t from[KV_MAX_TREE], to[KV_MAX_TREE];
+  kv_after_previous();
   const int head = blockIdx.x % a.g.heads, b = blockIdx.x / a.g.heads, tid = threadIdx.x;
   const int n = kv_rows_in_use(a.count, b, a.T);
   if (tid < n) {
@@ -190,33 +193,21 @@ int launch_kv_append(b200q_ctx* ctx, const b200q_kv_cache& c, const KvBatch& s, 
   ProfScope prof(ctx, KK_KV_APPEND);
   const uint32_t chunks = (uint32_t)(c.heads + 3) / 4, units = (uint32_t)s.B * (uint32_t)s.T * chunks;
   const KvArgs a = kv_args(ctx, c, s);
-  if (c.head_dim == 64) kv_append_kernel<64><<<row_grid(ctx, units), 256, 0, ctx->stream>>>(a, k, v, ld_k, ld_v, units, chunks);
-  else kv_append_kernel<128><<<row_grid(ctx, units), 256, 0, ctx->stream>>>(a, k, v, ld_k, ld_v, units, chunks);
-  ctx->launches++;
-  B200Q_CHECK_CUDA(cudaGetLastError());
-  return 0;
+  return kv_launch(ctx, c.head_dim == 64 ? kv_append_kernel<64> : kv_append_kernel<128>, dim3(row_grid(ctx, units)), 256, 0, a, k, v, ld_k, ld_v, units, chunks);
 }
 
 int launch_kv_read(b200q_ctx* ctx, const b200q_kv_cache& c, const KvBatch& s, float* k_out, float* v_out, int64_t ld_k, int64_t ld_v) {
   ProfScope prof(ctx, KK_KV_READ);
   const uint32_t chunks = (uint32_t)(c.heads + 3) / 4, units = (uint32_t)s.B * (uint32_t)s.T * chunks;
   const KvArgs a = kv_args(ctx, c, s);
-  if (c.head_dim == 64) kv_read_kernel<64><<<row_grid(ctx, units), 256, 0, ctx->stream>>>(a, k_out, v_out, ld_k, ld_v, units, chunks);
-  else kv_read_kernel<128><<<row_grid(ctx, units), 256, 0, ctx->stream>>>(a, k_out, v_out, ld_k, ld_v, units, chunks);
-  ctx->launches++;
-  B200Q_CHECK_CUDA(cudaGetLastError());
-  return 0;
+  return kv_launch(ctx, c.head_dim == 64 ? kv_read_kernel<64> : kv_read_kernel<128>, dim3(row_grid(ctx, units)), 256, 0, a, k_out, v_out, ld_k, ld_v, units, chunks);
 }
 
 int launch_kv_keep(b200q_ctx* ctx, const b200q_kv_cache& c, const KvBatch& s, const int32_t* keep) {
   ProfScope prof(ctx, KK_KV_KEEP);
   const KvArgs a = kv_args(ctx, c, s);
   const unsigned grid = (unsigned)s.B * (unsigned)c.heads;
-  if (c.head_dim == 64) kv_keep_kernel<64><<<grid, 128, 0, ctx->stream>>>(a, keep);
-  else kv_keep_kernel<128><<<grid, 128, 0, ctx->stream>>>(a, keep);
-  ctx->launches++;
-  B200Q_CHECK_CUDA(cudaGetLastError());
-  return 0;
+  return kv_launch(ctx, c.head_dim == 64 ? kv_keep_kernel<64> : kv_keep_kernel<128>, dim3(grid), 128, 0, a, keep);
 }
 
 }  // namespace b200q

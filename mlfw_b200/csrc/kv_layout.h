@@ -53,8 +53,8 @@ constexpr int KV_TILE = 16;
 
 // Positions visible to row block rb of a sequence with `n` rows in use: [0, result).
 B200Q_HD int64_t kv_visible(const KvGeom& g, int64_t start, int n, int group, int rows, int rb, bool tree) {
-  const int64_t last = (int64_t)(rb + 1) * rows - 1;                       // last row of the block
-  const int64_t t = last / group + 1;                                     // new tokens its rows reach without a tree
+  const uint32_t last = (uint32_t)(rb + 1) * (uint32_t)rows - 1;           // last row of the block (rows of a sequence are below 2^31)
+  const int64_t t = last / (uint32_t)group + 1;                           // new tokens its rows reach without a tree
   const int64_t vis = start + (tree || t > n ? n : t), most = g.max_pages << g.page_shift;
   return vis < 0 ? 0 : (vis > most ? most : vis);
 }
@@ -64,9 +64,30 @@ B200Q_HD int kv_tiles(const KvGeom& g, int64_t start, int n, int group, int rows
   const int64_t vis = kv_visible(g, start, n, group, rows, rb, tree);
   return vis <= tile ? 1 : (int)((vis + tile - 1) / tile);
 }
-// Runs: the first tile of run c of `runs` (runs <= total), and the run that holds a tile.
-B200Q_HD int64_t kv_run_begin(int64_t total, int64_t runs, int64_t c) { return total * c / runs; }
-B200Q_HD int64_t kv_run_of(int64_t total, int64_t runs, int64_t tile) { return ((tile + 1) * runs - 1) / total; }
+B200Q_HD int64_t kv_div(int64_t a, int64_t b) {   // a >= 0, b > 0: in 32 bits where that does (a 64-bit division is a subroutine)
+  return ((uint64_t)(a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+}
+// `total` > 0 tiles cut into at most `grid` runs of at least `least` tiles (of all there are, when that is fewer): the first
+// `rem` runs hold base + 1, the others base.
+struct KvRuns {
+  int64_t total, base;
+  int runs, rem;
+};
+B200Q_HD KvRuns kv_runs(int64_t total, int least, int grid) {
+  const int64_t want = total / least;
+  KvRuns r;
+  r.total = total;
+  r.runs = want < 1 ? 1 : (want < grid ? (int)want : grid);
+  r.base = kv_div(total, r.runs);
+  r.rem = (int)(total - r.base * r.runs);
+  return r;
+}
+// The first tile of a run, and the run that holds a tile.
+B200Q_HD int64_t kv_run_begin(const KvRuns& r, int c) { return r.base * c + (c < r.rem ? c : r.rem); }
+B200Q_HD int kv_run_of(const KvRuns& r, int64_t tile) {
+  const int64_t cut = (r.base + 1) * r.rem;
+  return tile < cut ? (int)kv_div(tile, r.base + 1) : r.rem + (int)kv_div(tile - cut, r.base);
+}
 
 // ---------------------------------------------------------------------------------------------- refusals (host)
 // Each returns null when the call is in order, else the reason.

@@ -10,7 +10,11 @@ import ctypes as C
 import numpy as np
 
 from ._lib import check
-from .device import Context, _ptr
+from .device import Context, _ptr as _address
+
+
+def _ptr(b):
+    return b if type(b) is int or b is None else _address(b)
 
 
 class KVCache:
@@ -28,6 +32,7 @@ class KVCache:
         h = C.c_void_p()
         check(ctx.lib.b200q_kv_create(ctx.handle, pages, page_tokens, heads, head_dim, *(_ptr(b) for b in buffers), C.byref(h)), "b200q_kv_create")
         self.handle = h.value
+        self._append, self._read, self._attention, self._keep = (getattr(ctx.lib, "b200q_kv_" + n) for n in ("append", "read", "attention", "keep"))
 
     def close(self) -> None:
         if self.handle and self.ctx.handle:
@@ -40,23 +45,29 @@ class KVCache:
         except Exception:
             pass
 
+    # A decoding step is a handful of these calls per layer: the wrappers do as little as they can.
     def append(self, k, v, ld_k, ld_v, B, T, page_table, max_pages, start, count=None):
         """Quantizes rows k, v (f32; row (b, t) of head h at base + (b*T + t)*ld + h*head_dim) into positions start[b] + t."""
-        check(self.ctx.lib.b200q_kv_append(self.ctx.handle, self.handle, _ptr(k), _ptr(v), ld_k, ld_v, B, T, _ptr(page_table), max_pages,
-                                           _ptr(start), _ptr(count)), "b200q_kv_append")
+        code = self._append(self.ctx.handle, self.handle, _ptr(k), _ptr(v), ld_k, ld_v, B, T, _ptr(page_table), max_pages, _ptr(start), _ptr(count))
+        if code:
+            check(code, "b200q_kv_append")
 
     def read(self, B, T, page_table, max_pages, start, count, k_out, v_out, ld_k, ld_v):
         """code * scale of positions start[b] + t, t < count[b], as f32."""
-        check(self.ctx.lib.b200q_kv_read(self.ctx.handle, self.handle, B, T, _ptr(page_table), max_pages, _ptr(start), _ptr(count),
-                                         _ptr(k_out), _ptr(v_out), ld_k, ld_v), "b200q_kv_read")
+        code = self._read(self.ctx.handle, self.handle, B, T, _ptr(page_table), max_pages, _ptr(start), _ptr(count), _ptr(k_out), _ptr(v_out), ld_k, ld_v)
+        if code:
+            check(code, "b200q_kv_read")
 
     def attention(self, q, ld_q, B, T, H, page_table, max_pages, start, count, tree, scale, out, ld_out):
         """softmax(scale q K^T) V for T new rows per sequence; ``tree``: uint64 [B*T], the drafted rows each row sees, or None for
         those up to itself."""
-        check(self.ctx.lib.b200q_kv_attention(self.ctx.handle, self.handle, _ptr(q), ld_q, B, T, H, _ptr(page_table), max_pages, _ptr(start),
-                                              _ptr(count), _ptr(tree), float(scale), _ptr(out), ld_out), "b200q_kv_attention")
+        code = self._attention(self.ctx.handle, self.handle, _ptr(q), ld_q, B, T, H, _ptr(page_table), max_pages, _ptr(start), _ptr(count), _ptr(tree),
+                               scale, _ptr(out), ld_out)
+        if code:
+            check(code, "b200q_kv_attention")
 
     def keep(self, B, T, page_table, max_pages, start, keep, count):
         """Moves the accepted drafted rows start[b] + keep[b*T + i] to start[b] + i, i < count[b]."""
-        check(self.ctx.lib.b200q_kv_keep(self.ctx.handle, self.handle, B, T, _ptr(page_table), max_pages, _ptr(start), _ptr(keep), _ptr(count)),
-              "b200q_kv_keep")
+        code = self._keep(self.ctx.handle, self.handle, B, T, _ptr(page_table), max_pages, _ptr(start), _ptr(keep), _ptr(count))
+        if code:
+            check(code, "b200q_kv_keep")

@@ -36,13 +36,13 @@ int walk(int B, int T, int heads, int group, int rows, int warps, int grid, int6
   }
   *total_out = total;
   if (total == 0) return 0;
-  int64_t want = total / warps;
-  const int64_t runs = want < 1 ? 1 : (want < grid ? want : grid);
+  const KvRuns all = kv_runs(total, warps, grid);
+  const int runs = all.runs;
   std::vector<int> slot(2 * grid, 0), pieces(begin.size(), 0), expected(begin.size(), 0), counter(grid, -1);
   size_t item = 0;
   int64_t covered = 0;
-  for (int64_t c = 0; c < runs; c++) {
-    int64_t at = kv_run_begin(total, runs, c), end = kv_run_begin(total, runs, c + 1);
+  for (int c = 0; c < runs; c++) {
+    int64_t at = kv_run_begin(all, c), end = kv_run_begin(all, c + 1);
     if (at != covered || end <= at) return 1;
     covered = end;
     while (at < end) {
@@ -50,7 +50,7 @@ int walk(int B, int T, int heads, int group, int rows, int warps, int grid, int6
       const int64_t t0 = at - begin[item], t1 = tiles[item] < t0 + end - at ? tiles[item] : t0 + end - at;
       if (t0 < 0 || t1 <= t0) return 2;
       if (!(t0 == 0 && t1 == tiles[item])) {
-        const int64_t r0 = kv_run_of(total, runs, begin[item]), r1 = kv_run_of(total, runs, begin[item] + tiles[item] - 1);
+        const int64_t r0 = kv_run_of(all, begin[item]), r1 = kv_run_of(all, begin[item] + tiles[item] - 1);
         if (r0 > c || r1 < c || r0 < 0 || r1 >= runs || (t0 == 0) != (r0 == c)) return 3;
         if (slot[2 * c + (t0 == 0 ? 1 : 0)]++) return 4;
         if (counter[r0] >= 0 && counter[r0] != (int)item) return 5;
