@@ -107,6 +107,13 @@ __device__ __forceinline__ void split_whole(float x, float& hi, float& lo) {
   hi = __fsub_rn(__fadd_rn(x, 12582912.0f), 12582912.0f);
   lo = __fsub_rn(x, hi);
 }
+// Two weights as binary16 halves: the rounded values and what is left of them (exact before its own rounding).
+__device__ __forceinline__ void split_f16(float x0, float x1, uint32_t& hi, uint32_t& lo) {
+  hi = pack_f16(x0, x1);
+  float y0, y1;
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;\n\t}" : "=f"(y0), "=f"(y1) : "r"(hi));
+  lo = pack_f16(__fsub_rn(x0, y0), __fsub_rn(x1, y1));
+}
 __device__ __forceinline__ float pow2(int e) {   // 2^e for -126 <= e <= 127
   return __int_as_float((e + 127) << 23);
 }

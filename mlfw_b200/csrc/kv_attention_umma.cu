@@ -1,7 +1,6 @@
 // Attention over the int8 key/value cache for many query rows (chunks of a prompt, drafted trees) on the 5th-generation
 // tensor cores.  What is computed and in which arithmetic stands in kv_attention.cuh.
 #include "kv_attention.cuh"
-#include "quant_math.cuh"
 
 namespace b200q {
 
@@ -9,8 +8,9 @@ namespace {
 
 // ---------------------------------------------------------------------------------------------------------------
 // One block per SM walks a run of 64-token tiles; an item is up to 128 rows, the 128 lanes of tensor memory.  Roles:
-//   four staging warps: K and V of a tile from the cache into a ring in shared memory as binary16 tiles of the tensor cores'
-//     layout (V transposed), with the tokens' scales beside them; a warp handles sixteen tokens, which always share a page;
+//   three staging warps: K and V of a tile from the cache into a ring in shared memory as binary16 tiles of the tensor cores'
+//     layout (V transposed), with the tokens' scales beside them, in units of sixteen tokens, which always share a page
+//     (three, so that the block has 20 warps and 96 registers per thread);
 //   one thread issues the products: S_hi = Q_hi K^T and S_lo = Q_lo K^T (tcgen05.mma kind::f16, 128 x 64) of tile j + 1, then
 //     O = P_lo V + P_hi V of tile j with the weights read from tensor memory;
 //   sixteen softmax warps, four threads per row with sixteen tokens of a tile each: scores from tensor memory, the row's c
@@ -29,7 +29,7 @@ namespace {
 // products in flight get 2 ms, tensor memory is freed.  Threads meet at mbarriers only, never at a hardware barrier that
 // a role that has left would keep the others waiting at; the one at the end is reached by all.
 // ---------------------------------------------------------------------------------------------------------------
-constexpr int MT = 64, LANES = 128, SOFT_WARPS = 16, STAGE_WARPS = 4, MANY_THREADS = 32 * (SOFT_WARPS + STAGE_WARPS + 1);
+constexpr int MT = 64, LANES = 128, SOFT_WARPS = 16, STAGE_WARPS = 3, MANY_THREADS = 32 * (SOFT_WARPS + STAGE_WARPS + 1);
 template <int D>
 struct Many {
   static constexpr int Q_BLOCK = LANES * 128, Q_BYTES = (D / 64) * Q_BLOCK;    // K blocks of 64 dimensions: [128 rows][128 B]
@@ -73,23 +73,50 @@ __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::be
 __device__ __forceinline__ void fence_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// N consecutive columns of this warp's lanes; the values may be used after tm_wait_ld on the same registers.
-__device__ __forceinline__ void tm_ld(uint32_t at, uint32_t (&r)[16]) {
+// Loads from tensor memory: consecutive columns of this warp's lanes.  The wait stands in the same statement: registers that a
+// separate one ties to the wait get copied.
+__device__ __forceinline__ void tm_ld2(uint32_t at0, uint32_t at1, uint32_t (&x)[16], uint32_t (&y)[16]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
-        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(at) : "memory");
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%32];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%33];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]), "=r"(x[6]), "=r"(x[7]), "=r"(x[8]), "=r"(x[9]),
+        "=r"(x[10]), "=r"(x[11]), "=r"(x[12]), "=r"(x[13]), "=r"(x[14]), "=r"(x[15]),
+        "=r"(y[0]), "=r"(y[1]), "=r"(y[2]), "=r"(y[3]), "=r"(y[4]), "=r"(y[5]), "=r"(y[6]), "=r"(y[7]), "=r"(y[8]), "=r"(y[9]),
+          "=r"(y[10]), "=r"(y[11]), "=r"(y[12]), "=r"(y[13]), "=r"(y[14]), "=r"(y[15])
+      : "r"(at0), "r"(at1) : "memory");
 }
-__device__ __forceinline__ void tm_ld(uint32_t at, uint32_t (&r)[8]) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(at) : "memory");
+__device__ __forceinline__ void tm_ld2(uint32_t at0, uint32_t at1, uint32_t (&x)[8], uint32_t (&y)[8]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%16];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%8, %9, %10, %11, %12, %13, %14, %15}, [%17];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]), "=r"(x[6]), "=r"(x[7]),
+        "=r"(y[0]), "=r"(y[1]), "=r"(y[2]), "=r"(y[3]), "=r"(y[4]), "=r"(y[5]), "=r"(y[6]), "=r"(y[7])
+      : "r"(at0), "r"(at1) : "memory");
 }
-template <int N>
-__device__ __forceinline__ void tm_wait_ld(uint32_t (&r)[N]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-  for (int i = 0; i < N; i++) asm volatile("" : "+r"(r[i])::"memory");   // no use of a loaded register moves ahead of the wait
+__device__ __forceinline__ void tm_ld2(uint32_t at0, uint32_t at1, uint32_t (&x)[4], uint32_t (&y)[4]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%8];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x4.b32 {%4, %5, %6, %7}, [%9];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]),
+        "=r"(y[0]), "=r"(y[1]), "=r"(y[2]), "=r"(y[3])
+      : "r"(at0), "r"(at1) : "memory");
+}
+__device__ __forceinline__ void tm_ld(uint32_t at, uint32_t (&x)[32]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\ttcgen05.wait::ld.sync.aligned;"
+               : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]), "=r"(x[6]), "=r"(x[7]), "=r"(x[8]), "=r"(x[9]),
+                 "=r"(x[10]), "=r"(x[11]), "=r"(x[12]), "=r"(x[13]), "=r"(x[14]), "=r"(x[15]), "=r"(x[16]), "=r"(x[17]), "=r"(x[18]),
+                 "=r"(x[19]), "=r"(x[20]), "=r"(x[21]), "=r"(x[22]), "=r"(x[23]), "=r"(x[24]), "=r"(x[25]), "=r"(x[26]), "=r"(x[27]),
+                 "=r"(x[28]), "=r"(x[29]), "=r"(x[30]), "=r"(x[31])
+               : "r"(at) : "memory");
+}
+__device__ __forceinline__ void tm_ld(uint32_t at, uint32_t (&x)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\ttcgen05.wait::ld.sync.aligned;"
+               : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]), "=r"(x[6]), "=r"(x[7]), "=r"(x[8]), "=r"(x[9]),
+                 "=r"(x[10]), "=r"(x[11]), "=r"(x[12]), "=r"(x[13]), "=r"(x[14]), "=r"(x[15])
+               : "r"(at) : "memory");
 }
 __device__ __forceinline__ void tm_st(uint32_t at, const uint32_t (&r)[8]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
@@ -99,26 +126,34 @@ __device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint3
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
 
-__device__ __forceinline__ void tm_ld(uint32_t at, uint32_t (&r)[4]) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
-}
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory"); }
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
 
+// Whether the phase is over; suspends the thread for up to a microsecond while it is not.
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tmbarrier.try_wait.parity.shared::cta.b64 q, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(done) : "r"(bar), "r"(parity), "r"(1000u) : "memory");
+  return done != 0;
+}
+
 struct ManyParams {
   int row_blocks;
-  unsigned long long limit_ns;
+  uint32_t polls;          // bound of every wait
 };
 
 // The block's barriers and flags.  Counts: one arrival per warp (after __syncwarp) or per tcgen05.commit.
 template <int STAGES>
 struct ManyShared {
-  uint64_t full[STAGES], empty[STAGES];        // ring slots: staged (4 warps), consumed (commit of the tile's P V)
+  uint64_t full[STAGES], empty[STAGES];        // ring slots: staged (4 units), consumed (commit of the tile's P V)
   uint64_t scores[2], weights[2], outputs[2];  // S ready (commit), P ready (16 warps), O ready (commit)
   uint64_t queries, soft;                      // Q staged (16 warps); meeting of the softmax warps (16 warps)
   uint64_t rows[4];                            // meeting of the four warps that share a quarter of the lanes
   uint32_t tmem;
   int abort;
+  static constexpr uint32_t FULL = 0, EMPTY = 8 * STAGES, SCORES = 16 * STAGES, WEIGHTS = SCORES + 16, OUTPUTS = WEIGHTS + 16, QUERIES = OUTPUTS + 16,
+                            SOFT = QUERIES + 8, ROWS = SOFT + 8;   // places of the members
 };
 
 // Pieces of a block's run, one after another: every role walks them by itself.
@@ -162,6 +197,7 @@ __device__ __forceinline__ int v_row(int L, int q) {
 template <int D, int CS>
 __global__ void __launch_bounds__(MANY_THREADS, 1) kv_attention_many_kernel(const AttnArgs a, const ManyParams mp) {
   using C = Many<D>;
+  using S = ManyShared<C::STAGES>;
   constexpr int ROWS = LANES / CS, NC = 16 / CS, QD = D / 4, ST = C::STAGES;   // rows of an item; tokens of a tile and outputs of a thread
   extern __shared__ uint8_t smem_raw[];
   __shared__ ManyShared<ST> sh;
@@ -178,7 +214,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv_attention_many_kernel(cons
   if (run.begin == run.end) return;
 
   if (tid == 0) {
-    for (int s = 0; s < ST; s++) { mbar_init(smem_u32(&sh.full[s]), STAGE_WARPS); mbar_init(smem_u32(&sh.empty[s]), 1); }
+    for (int s = 0; s < ST; s++) { mbar_init(smem_u32(&sh.full[s]), 4); mbar_init(smem_u32(&sh.empty[s]), 1); }
     for (int s = 0; s < 2; s++) { mbar_init(smem_u32(&sh.scores[s]), 1); mbar_init(smem_u32(&sh.weights[s]), SOFT_WARPS); mbar_init(smem_u32(&sh.outputs[s]), 1); }
     mbar_init(smem_u32(&sh.queries), SOFT_WARPS);
     mbar_init(smem_u32(&sh.soft), SOFT_WARPS);
@@ -198,22 +234,17 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv_attention_many_kernel(cons
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t tmem = sh.tmem;
   volatile int* abort_flag = &sh.abort;
+  const uint32_t sh_base = smem_u32(&sh);
 
-  auto wait = [&](const uint64_t& bar, uint32_t parity) -> bool {
-    const uint32_t addr = smem_u32(&bar);
-    uint32_t done = 0, it = 0;
-    uint64_t t0 = 0;
-    while (true) {
-      asm volatile(
-          "{\n\t.reg .pred q;\n\tmbarrier.try_wait.parity.shared::cta.b64 q, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-          : "=r"(done) : "r"(addr), "r"(parity), "r"(1000u) : "memory");
-      if (done) return true;
-      if ((++it & 7u) == 0u) {
-        if (*abort_flag) return false;
-        if (t0 == 0) t0 = gtimer();
-        else if (gtimer() - t0 > mp.limit_ns) { *abort_flag = 1; return false; }
-      }
+  // Waits for a phase of a barrier (given by its place in `sh`), mp.polls times a microsecond at most.
+  auto wait = [&](uint32_t bar, uint32_t parity) -> bool {
+    if (mbar_try(sh_base + bar, parity)) return true;
+    for (uint32_t n = mp.polls; n != 0; n--) {
+      if (mbar_try(sh_base + bar, parity)) return true;
+      if (*abort_flag) return false;
     }
+    *abort_flag = 1;
+    return false;
   };
 
   Walk<ROWS> w;
@@ -228,9 +259,9 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv_attention_many_kernel(cons
     const int col0 = cg * 16 + copy * NC;                        // this thread's tokens of a tile
     const uint32_t lane_tm = tmem + ((uint32_t)(quarter * 32) << 16);
     uint32_t soft_phase = 0, rows_phase = 0;
-    auto meet = [&](const uint64_t& bar, uint32_t& phase) -> bool {   // all warps of the barrier; shared memory before it is seen after it
+    auto meet = [&](uint32_t bar, uint32_t& phase) -> bool {     // all warps of the barrier; shared memory before it is seen after it
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&bar));
+      if (lane == 0) mbar_arrive(sh_base + bar);
       const bool ok = wait(bar, phase);
       phase ^= 1u;
       return __all_sync(0xffffffffu, ok);
@@ -257,14 +288,15 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv_attention_many_kernel(cons
                     max(__float_as_uint(x[i].z) & 0x7fffffffu, __float_as_uint(x[i].w) & 0x7fffffffu));
         }
         sum_x[cg][row] = __uint_as_float(top);
-        alive = meet(sh.rows[quarter], rows_phase);
+        alive = meet(S::ROWS + 8 * quarter, rows_phase);
         if (!alive) break;
 #pragma unroll
         for (int k = 0; k < 4; k++) top = max(top, __float_as_uint(sum_x[k][row]));
         const bool finite = top < 0x7f800000u;
         const int ex = max((int)(top >> 23), 24) - 127;
-        const float up = pow2(10 - ex);
-        rs = finite ? a.scale_log2e * pow2(ex - 10) : __int_as_float(0x7fc00000);
+        // rs is kept positive, so that a masked x = -Inf stays -Inf: a negative scale turns the query's sign, a zero one zeroes it
+        const float up = a.scale_log2e == 0.0f ? 0.0f : copysignf(pow2(10 - ex), a.scale_log2e);
+        rs = finite ? fmaxf(fabsf(a.scale_log2e) * pow2(ex - 10), 1e-37f) : __int_as_float(0x7fc00000);
 #pragma unroll
         for (int i = 0; i < QD / 4; i += 2) {                    // eight dimensions: 16 bytes of either half, in the order of staged K
           float h[8], l[8];
@@ -278,113 +310,98 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv_attention_many_kernel(cons
         }
         fence_proxy();                                           // the tensor cores read what the threads wrote
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&sh.queries));
+        if (lane == 0) mbar_arrive(sh_base + S::QUERIES);
       }
 
-      uint64_t o2[QD / 2];                                       // pairs of outputs, in the order of the V tile's rows
+      float o[QD];                                               // outputs, in the order of the V tile's rows
 #pragma unroll
-      for (int i = 0; i < QD / 2; i++) o2[i] = 0;
+      for (int i = 0; i < QD; i++) o[i] = 0.0f;
       float c_run = C_NONE, l_run = 0.0f, fold = 0.0f;           // fold: the factor that goes with the latest tile's O
       auto take_outputs = [&](uint32_t t) -> bool {              // o = o * fold + O of tile t
-        if (!__all_sync(0xffffffffu, wait(sh.outputs[t & 1], (t >> 1) & 1))) return false;
+        if (!__all_sync(0xffffffffu, wait(S::OUTPUTS + 8 * (t & 1), (t >> 1) & 1))) return false;
         fence_after();
-        const uint64_t fold2 = f2_dup(fold);
+        uint32_t x[QD];
+        tm_ld(lane_tm + TM_O + (t & 1) * TM_O_STEP + cg * QD, x);
 #pragma unroll
-        for (int c = 0; c < QD; c += 16) {
-          uint32_t x[16];
-          tm_ld(lane_tm + TM_O + (t & 1) * TM_O_STEP + cg * QD + c, x);
-          tm_wait_ld(x);
-#pragma unroll
-          for (int i = 0; i < 16; i += 2)
-            o2[(c + i) / 2] = f2_fma(o2[(c + i) / 2], fold2, f2_pack(__uint_as_float(x[i]), __uint_as_float(x[i + 1])));
-        }
+        for (int i = 0; i < QD; i++) o[i] = fmaf(o[i], fold, __uint_as_float(x[i]));
         return true;
       };
 
-      for (int j = w.tile0; j < w.tile1; j++, it++) {
+      const int j0 = w.tile0, j1 = w.tile1, plain = w.first <= 0 ? 0 : (int)(w.first / MT);   // tiles of cached tokens only
+#pragma unroll 1
+      for (int j = j0; j < j1; j++, it++) {
         const uint32_t buf = it & 1, slot = it % ST;
         const uint32_t s_tm = lane_tm + TM_S + buf * TM_S_STEP;
         // the slot's tokens (the staging warps' stores) and the scores
-        bool ok = wait(sh.full[slot], (it / ST) & 1) && wait(sh.scores[buf], (it >> 1) & 1);
+        bool ok = wait(S::FULL + 8 * slot, (it / ST) & 1) && wait(S::SCORES + 8 * buf, (it >> 1) & 1);
         alive = __all_sync(0xffffffffu, ok);
         if (!alive) break;
         fence_after();
         uint32_t hi[NC], lo[NC];
-        tm_ld(s_tm + col0, hi);
-        tm_ld(s_tm + TM_SLO + col0, lo);
+        tm_ld2(s_tm + col0, s_tm + TM_SLO + col0, hi, lo);
 
         // which of this thread's tokens its row sees
         uint32_t seen = tok_there[slot][cg];
-        const int64_t from = (int64_t)j * MT + cg * 16 - w.first;   // place of the first of the sixteen tokens among the new rows
-        if (from + 16 > 0) {
-          const uint32_t before = from >= 0 ? 0u : (1u << (int)-from) - 1;
-          uint32_t fresh;
-          if (a.tree) fresh = from >= 64 ? 0u : (from >= 0 ? (uint32_t)(row_seen >> (int)from) : (uint32_t)(row_seen << (int)-from));
-          else {
-            const int64_t k = (int64_t)row_t + 1 - from;         // tokens up to the row itself
-            fresh = k <= 0 ? 0u : (k >= 16 ? 0xffffu : (1u << (int)k) - 1);
+        const bool all = j < plain && seen == 0xffffu;           // the same in the whole warp
+        if (!all) {
+          const int64_t from = (int64_t)j * MT + cg * 16 - w.first;   // place of the first of the sixteen tokens among the new rows
+          if (from + 16 > 0) {
+            const uint32_t before = from >= 0 ? 0u : (1u << (int)-from) - 1;
+            uint32_t fresh;
+            if (a.tree) fresh = from >= 64 ? 0u : (from >= 0 ? (uint32_t)(row_seen >> (int)from) : (uint32_t)(row_seen << (int)-from));
+            else {
+              const int64_t k = (int64_t)row_t + 1 - from;       // tokens up to the row itself
+              fresh = k <= 0 ? 0u : (k >= 16 ? 0xffffu : (1u << (int)k) - 1);
+            }
+            seen &= before | fresh;
           }
-          seen &= before | fresh;
+          seen >>= copy * NC;
         }
-        seen >>= copy * NC;
-        const bool all = (seen & ((1u << NC) - 1)) == (1u << NC) - 1;
 
-        // z = (S_hi + S_lo) * scale_k * rs
-        float z[NC], top = NEG_INF;
-        const uint64_t rs2 = f2_dup(rs);
-        tm_wait_ld(hi);
-        tm_wait_ld(lo);
+        // x = (S_hi + S_lo) * scale_k, the score z = x * rs
+        float x[NC], u[NC], top = NEG_INF;
 #pragma unroll
         for (int i = 0; i < NC; i += 4) {
-          const float4 k = *reinterpret_cast<const float4*>(&tok_ks[slot][col0 + i]);
-          const uint64_t s0 = f2_add(f2_pack(__uint_as_float(hi[i]), __uint_as_float(hi[i + 1])), f2_pack(__uint_as_float(lo[i]), __uint_as_float(lo[i + 1])));
-          const uint64_t s1 = f2_add(f2_pack(__uint_as_float(hi[i + 2]), __uint_as_float(hi[i + 3])), f2_pack(__uint_as_float(lo[i + 2]), __uint_as_float(lo[i + 3])));
-          f2_unpack(f2_mul(f2_mul(s0, f2_pack(k.x, k.y)), rs2), z[i], z[i + 1]);
-          f2_unpack(f2_mul(f2_mul(s1, f2_pack(k.z, k.w)), rs2), z[i + 2], z[i + 3]);
+          const float4 k = *reinterpret_cast<const float4*>(&tok_ks[slot][col0 + i]), v = *reinterpret_cast<const float4*>(&tok_lv[slot][col0 + i]);
+          const float kk[4] = {k.x, k.y, k.z, k.w}, vv[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int c = 0; c < 4; c++) {
+            x[i + c] = (__uint_as_float(hi[i + c]) + __uint_as_float(lo[i + c])) * kk[c];
+            u[i + c] = fmaf(x[i + c], rs, vv[c]);
+          }
         }
         if (!all) {
 #pragma unroll
           for (int i = 0; i < NC; i++)
-            if (!((seen >> i) & 1)) z[i] = NEG_INF;
+            if (!((seen >> i) & 1)) x[i] = u[i] = NEG_INF;
         }
 #pragma unroll
-        for (int i = 0; i < NC; i += 4) {
-          const float4 v = *reinterpret_cast<const float4*>(&tok_lv[slot][col0 + i]);
-          top = fmaxf(fmaxf(top, fmaxf(z[i] + v.x, z[i + 1] + v.y)), fmaxf(z[i + 2] + v.z, z[i + 3] + v.w));
-        }
+        for (int i = 0; i < NC; i += 2) top = fmaxf(fmaxf(top, u[i]), u[i + 1]);
         // the row's other tokens: warps with the same lanes (slots alternate, so one meeting per tile does)
         top_x[buf][cg][row] = top;
-        alive = meet(sh.rows[quarter], rows_phase);
+        alive = meet(S::ROWS + 8 * quarter, rows_phase);
         if (!alive) break;
 #pragma unroll
         for (int k = 0; k < 4; k++) top = fmaxf(top, top_x[buf][k][row]);
         const float c_new = fmaxf(c_run, top - 10.0f), fold_new = ex2(c_run - c_new);
         c_run = c_new;
-        uint64_t l2 = 0;
-        const uint64_t c2 = f2_dup(c_new), magic2 = f2_dup(12582912.0f);
+        float sum = 0.0f;
         uint32_t h[NC / 2], l[NC / 2];
 #pragma unroll
         for (int i = 0; i < NC; i += 4) {
           const float4 v = *reinterpret_cast<const float4*>(&tok_vs[slot][col0 + i]);
+          const float vv[4] = {v.x, v.y, v.z, v.w};
+          float wt[4];
 #pragma unroll
-          for (int k = 0; k < 4; k += 2) {
-            float d0, d1, x0, x1, y0, y1;
-            f2_unpack(f2_sub(f2_pack(z[i + k], z[i + k + 1]), c2), d0, d1);
-            const uint64_t p = f2_pack(ex2(d0), ex2(d1));
-            l2 = f2_add(l2, p);
-            const uint64_t x = f2_mul(p, k == 0 ? f2_pack(v.x, v.y) : f2_pack(v.z, v.w));
-            const uint64_t xh = f2_sub(f2_add(x, magic2), magic2);
-            f2_unpack(xh, x0, x1);
-            f2_unpack(f2_sub(x, xh), y0, y1);
-            h[(i + k) / 2] = pack_f16(x0, x1);
-            l[(i + k) / 2] = pack_f16(y0, y1);
+          for (int c = 0; c < 4; c++) {
+            const float p = ex2(fmaf(x[i + c], rs, -c_new));
+            sum += p;
+            wt[c] = p * vv[c];
           }
+          split_f16(wt[0], wt[1], h[i / 2], l[i / 2]);
+          split_f16(wt[2], wt[3], h[i / 2 + 1], l[i / 2 + 1]);
         }
-        {
-          float p0, p1;
-          f2_unpack(l2, p0, p1);
-          l_run = fmaf(l_run, fold_new, (p0 + p1) * P_UNIT);
-        }
+        l_run = fmaf(l_run, fold_new, sum * P_UNIT);
         // the sixteen tokens' weights, zero where another copy has them: 8 + 8 columns over their S_hi
         uint32_t ph[8], pl[8];
 #pragma unroll
@@ -398,9 +415,9 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv_attention_many_kernel(cons
         tm_wait_st();
         fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&sh.weights[buf]));
+        if (lane == 0) mbar_arrive(sh_base + S::WEIGHTS + 8 * buf);
         // the tile before: its O is ready or nearly so
-        if (j > w.tile0) {
+        if (j > j0) {
           alive = take_outputs(it - 1);
           if (!alive) break;
         }
@@ -415,29 +432,26 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv_attention_many_kernel(cons
       float* res = reinterpret_cast<float*>(sm + C::QHI);        // [128][D], 16-byte pieces XOR lane % 8
       sum_x[cg][row] = l_run;
       if (cg == 0) c_x[row] = c_run;
-      alive = meet(sh.soft, soft_phase);
+      alive = meet(S::SOFT, soft_phase);
       if (!alive) break;
       {
         float c_max = c_x[rq];
 #pragma unroll
         for (int k = 1; k < CS; k++) c_max = fmaxf(c_max, c_x[k * ROWS + rq]);
-        const uint64_t f2 = f2_dup(ex2(c_run - c_max));
+        const float f = ex2(c_run - c_max);
 #pragma unroll
         for (int i = 0; i < QD / 4; i++) {
           float v[4];
 #pragma unroll
           for (int q = 0; q < 4; q++) {
             const int k = q * (QD / 4) + i, k2 = D == 64 ? k ^ 4 : k;   // see v_row
-            float x0, x1, y0, y1;
-            f2_unpack(f2_mul(o2[k / 2], f2), x0, x1);
-            f2_unpack(f2_mul(o2[k2 / 2], f2), y0, y1);
-            v[q] = (D == 64 && (cg & 1)) ? ((k2 & 1) ? y1 : y0) : ((k & 1) ? x1 : x0);
+            v[q] = ((D == 64 && (cg & 1)) ? o[k2] : o[k]) * f;
           }
           const int piece = cg * (QD / 4) + i;
           *reinterpret_cast<float4*>(res + row * D + ((piece ^ (row & 7)) << 2)) = make_float4(v[0], v[1], v[2], v[3]);
         }
       }
-      alive = meet(sh.soft, soft_phase);
+      alive = meet(S::SOFT, soft_phase);
       if (!alive) break;
       const bool whole = w.tile0 == 0 && w.tile1 == w.tiles;
       if (w.tile0 == 0 && !whole && tid == 0) a.items[blockIdx.x] = make_int4(w.e, w.head, kv_run_of(run.all, w.at + w.tiles - 1), 1);
@@ -464,123 +478,145 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv_attention_many_kernel(cons
           if (p == 0) { __stcg(slot + ROWS * D + r, c_max); __stcg(slot + ROWS * D + ROWS + r, sum); }
         }
       }
-      alive = meet(sh.soft, soft_phase);                         // Q's tiles are about to be written again
+      alive = meet(S::SOFT, soft_phase);                         // Q's tiles are about to be written again
       w.close(a);
     }
   } else if (warp < SOFT_WARPS + STAGE_WARPS) {
     // ------------------------------------------------------------------------------------------------ staging
-    // Sixteen tokens of a tile per warp: one page, so one run of codes and of scales.  A tile's codes are on their way into
-    // registers while the warp waits for a free slot, and the page of the tile after it is looked up.
+    // Unit u of a piece is sixteen tokens of tile tile0 + u / 4: one page, so one run of codes and of scales.  Units go round the
+    // warps; a unit's codes are on their way into registers while the warp waits for a free slot.
     const int sw = warp - SOFT_WARPS;
     constexpr int KN = D / 32, VN = D / 64;                      // K: 16-byte pieces of a lane; V: (eight tokens x one word) of a lane
     const int v_L = D == 128 ? lane : lane & 15, v_oct = D == 128 ? 0 : lane >> 4;
+    uint32_t k_off[KN], v_off[4];                                // places in the tiles, but for the sixteen tokens' own
+#pragma unroll
+    for (int i = 0; i < KN; i++) {
+      const int c = i * 32 + lane, tok = c / (D / 16), p = c % (D / 16);
+      k_off[i] = (p >> 2) * C::K_BLOCK + sw128(tok, (p & 3) * 32);   // sixteen tokens on: 2048 bytes on, the same swizzle
+    }
+#pragma unroll
+    for (int q = 0; q < 4; q++) v_off[q] = v_row<D>(v_L, q) * 128;
+    uint32_t next = sw;                                          // the next unit of the run for this warp
     while (alive && w.open(a, mp.row_blocks)) {
       const int32_t* table = a.page_table + (int64_t)w.b * a.g.max_pages;
-      const int64_t pages_tokens = a.g.max_pages << a.g.page_shift;
-      auto page_of = [&](int j) -> int {
-        const int64_t pos = (int64_t)j * MT + sw * 16;
-        return (j < w.tile1 && pos < pages_tokens) ? __ldg(table + (pos >> a.g.page_shift)) : -1;
+      const int64_t in_table = min(w.vis, a.g.max_pages << a.g.page_shift);
+      const uint32_t first_unit = it * 4, end_unit = (it + (uint32_t)(w.tile1 - w.tile0)) * 4;
+      const int64_t pos0 = (int64_t)w.tile0 * MT - (int64_t)first_unit * 16;
+      auto page_of = [&](uint32_t u) -> int {                    // -1: nothing of the unit is visible
+        const int64_t pos = pos0 + (int64_t)u * 16;
+        return (u < end_unit && pos < in_table) ? __ldg(table + (pos >> a.g.page_shift)) : -1;
       };
-      struct Raw { uint4 k[KN]; uint32_t v[VN * 8]; float ks, vs; };
-      auto fetch = [&](int j, int page, Raw& r) {
-        const int64_t pos = (int64_t)j * MT + sw * 16;
-        const bool ok = (uint32_t)page < (uint32_t)a.g.pages && pos < w.vis;   // else nothing of the sixteen is visible
+      uint4 rk[KN];
+      uint32_t rv[VN * 8];
+      float ks, vs;
+      auto fetch = [&](uint32_t u, int page) {
+        const int64_t pos = pos0 + (int64_t)u * 16;
+        const bool ok = (uint32_t)page < (uint32_t)a.g.pages;
         const int64_t cell = ok ? (((int64_t)page * a.g.heads + w.head) << a.g.page_shift) + (pos & ((1 << a.g.page_shift) - 1)) : 0;
         const int8_t *kp = a.k + cell * D, *vp = a.v + cell * D;
 #pragma unroll
-        for (int i = 0; i < KN; i++) r.k[i] = ok ? __ldg(reinterpret_cast<const uint4*>(kp) + i * 32 + lane) : make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < KN; i++) rk[i] = ok ? __ldg(reinterpret_cast<const uint4*>(kp) + i * 32 + lane) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-        for (int u = 0; u < VN; u++)
+        for (int o = 0; o < VN; o++)
 #pragma unroll
-          for (int i = 0; i < 8; i++) r.v[u * 8 + i] = ok ? __ldg(reinterpret_cast<const uint32_t*>(vp + ((v_oct + u) * 8 + i) * D) + v_L) : 0u;
-        r.ks = r.vs = 0.0f;
-        if (ok && lane < 16 && pos + lane < w.vis) { r.ks = __ldg(a.ks + cell + lane); r.vs = __ldg(a.vs + cell + lane); }
+          for (int i = 0; i < 8; i++) rv[o * 8 + i] = ok ? __ldg(reinterpret_cast<const uint32_t*>(vp + ((v_oct + o) * 8 + i) * D) + v_L) : 0u;
+        ks = vs = 0.0f;
+        if (ok && lane < 16 && pos + lane < w.vis) { ks = __ldg(a.ks + cell + lane); vs = __ldg(a.vs + cell + lane); }
       };
-      Raw cur;
-      int page = page_of(w.tile0), page_next = page_of(w.tile0 + 1);
-      fetch(w.tile0, page, cur);
-      for (int j = w.tile0; j < w.tile1; j++, it++) {
-        const uint32_t slot = it % ST;
-        alive = __all_sync(0xffffffffu, wait(sh.empty[slot], ((it / ST) & 1) ^ 1u));
+      int page = page_of(next), page_next = page_of(next + STAGE_WARPS);
+      fetch(next, page);
+#pragma unroll 1
+      for (; next < end_unit; next += STAGE_WARPS) {
+        const uint32_t t = next >> 2, slot = t % ST, part = next & 3;
+        alive = __all_sync(0xffffffffu, wait(S::EMPTY + 8 * slot, ((t / ST) & 1) ^ 1u));
         if (!alive) break;
-        const uint32_t kt = sm_base + C::RING + slot * C::STAGE, vt = kt + C::K_BYTES;
+        const uint32_t kt = sm_base + C::RING + slot * C::STAGE + part * 2048, vt = sm_base + C::RING + slot * C::STAGE + C::K_BYTES;
 #pragma unroll
         for (int i = 0; i < KN; i++) {                           // of four neighbouring dimensions the even ones come first
-          const int c = i * 32 + lane, tok = sw * 16 + c / (D / 16), p = c % (D / 16);
-          const uint32_t to = kt + (p >> 2) * C::K_BLOCK;
-          const uint4 x = cur.k[i];
-          sts128(to + sw128(tok, (p & 3) * 32), codes_even(x.x), codes_odd(x.x), codes_even(x.y), codes_odd(x.y));
-          sts128(to + sw128(tok, (p & 3) * 32 + 16), codes_even(x.z), codes_odd(x.z), codes_even(x.w), codes_odd(x.w));
+          const uint32_t to = kt + k_off[i];
+          sts128(to, codes_even(rk[i].x), codes_odd(rk[i].x), codes_even(rk[i].y), codes_odd(rk[i].y));
+          sts128(to ^ 16u, codes_even(rk[i].z), codes_odd(rk[i].z), codes_even(rk[i].w), codes_odd(rk[i].w));
         }
 #pragma unroll
-        for (int u = 0; u < VN; u++)
+        for (int o = 0; o < VN; o++)
 #pragma unroll
           for (int h = 0; h < 2; h++) {
             uint32_t y[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) y[i] = __byte_perm(cur.v[u * 8 + 2 * i], cur.v[u * 8 + 2 * i + 1], h ? 0x7632 : 0x5410);
-            const int col = (sw * 2 + v_oct + u) * 16;           // eight tokens
-            sts128(vt + sw128(v_row<D>(v_L, 2 * h), col), codes_even(y[0]), codes_even(y[1]), codes_even(y[2]), codes_even(y[3]));
-            sts128(vt + sw128(v_row<D>(v_L, 2 * h + 1), col), codes_odd(y[0]), codes_odd(y[1]), codes_odd(y[2]), codes_odd(y[3]));
+            for (int i = 0; i < 4; i++) y[i] = __byte_perm(rv[o * 8 + 2 * i], rv[o * 8 + 2 * i + 1], h ? 0x7632 : 0x5410);
+            const uint32_t col = part * 2 + v_oct + o;           // which eight tokens
+            const uint32_t e = vt + v_off[2 * h], d = vt + v_off[2 * h + 1];
+            sts128(e + ((col ^ ((v_off[2 * h] >> 7) & 7)) << 4), codes_even(y[0]), codes_even(y[1]), codes_even(y[2]), codes_even(y[3]));
+            sts128(d + ((col ^ ((v_off[2 * h + 1] >> 7) & 7)) << 4), codes_odd(y[0]), codes_odd(y[1]), codes_odd(y[2]), codes_odd(y[3]));
           }
-        const int64_t pos = (int64_t)j * MT + sw * 16;
-        const bool there = (uint32_t)page < (uint32_t)a.g.pages && lane < 16 && pos + lane < w.vis;
-        const uint32_t mask = __ballot_sync(0xffffffffu, there);
+        const bool ok = (uint32_t)page < (uint32_t)a.g.pages;
+        const int64_t pos = pos0 + (int64_t)next * 16;
+        const uint32_t mask = __ballot_sync(0xffffffffu, ok && lane < 16 && pos + lane < w.vis);
         if (lane < 16) {
-          tok_ks[slot][sw * 16 + lane] = cur.ks;
-          tok_vs[slot][sw * 16 + lane] = cur.vs;
-          tok_lv[slot][sw * 16 + lane] = log2_scale(cur.vs);
+          tok_ks[slot][part * 16 + lane] = ks;
+          tok_vs[slot][part * 16 + lane] = vs;
+          tok_lv[slot][part * 16 + lane] = log2_scale(vs);
         }
         if (lane == 0) {
-          tok_there[slot][sw] = mask;
-          if ((uint32_t)page >= (uint32_t)a.g.pages && pos < w.vis) atomicOr(a.status, STATUS_BAD_INDEX);
+          tok_there[slot][part] = mask;
+          if (!ok && pos < w.vis) atomicOr(a.status, STATUS_BAD_INDEX);
         }
         fence_proxy();                                           // the tensor cores read what the threads wrote
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&sh.full[slot]));
+        if (lane == 0) mbar_arrive(sh_base + S::FULL + 8 * slot);
         page = page_next;
-        page_next = page_of(j + 2);
-        if (j + 1 < w.tile1) fetch(j + 1, page, cur);
+        page_next = page_of(next + 2 * STAGE_WARPS);
+        if (next + STAGE_WARPS < end_unit) fetch(next + STAGE_WARPS, page);
       }
+      it += (uint32_t)(w.tile1 - w.tile0);
       if (alive) w.close(a);
     }
-  } else if (lane == 0) {
+  } else {
     // ------------------------------------------------------------------------------------------------ products
+    // The whole warp walks and waits; one lane issues.
     uint32_t q_phase = 0;
+    const uint64_t qh_desc = smem_desc(sm_base + C::QHI), ql_desc = smem_desc(sm_base + C::QLO), k_desc = smem_desc(sm_base + C::RING),
+                   v_desc = smem_desc(sm_base + C::RING + C::K_BYTES);
     auto score = [&](uint32_t t) -> bool {                       // S of tile t
       const uint32_t slot = t % ST;
-      if (!wait(sh.full[slot], (t / ST) & 1)) return false;
-      if (t >= 2 && !wait(sh.outputs[t & 1], ((t - 2) >> 1) & 1)) return false;   // P V of tile t - 2 has read the weights that stand there
+      bool ok = wait(S::FULL + 8 * slot, (t / ST) & 1);
+      if (t >= 2) ok = ok && wait(S::OUTPUTS + 8 * (t & 1), ((t - 2) >> 1) & 1);   // P V of tile t - 2 has read the weights that stand there
+      if (!__all_sync(0xffffffffu, ok)) return false;
       fence_after();
       constexpr uint32_t idesc = idesc_f16(LANES, MT);
-      const uint32_t s_tm = tmem + TM_S + (t & 1) * TM_S_STEP, kt = sm_base + C::RING + slot * C::STAGE;
+      const uint32_t s_tm = tmem + TM_S + (t & 1) * TM_S_STEP;
+      const uint64_t kd = k_desc + (uint64_t)(slot * (C::STAGE >> 4));
+      if (lane == 0) {
 #pragma unroll
-      for (int s = 0; s < D / 16; s++) {                         // 16 dimensions = 32 bytes along K per instruction
-        const uint64_t kd = smem_desc(kt + (s >> 2) * C::K_BLOCK) + 2 * (s & 3);
-        const uint32_t q = sm_base + (s >> 2) * C::Q_BLOCK;
-        mma_ss(s_tm, smem_desc(q + C::QHI) + 2 * (s & 3), kd, idesc, s != 0);
-        mma_ss(s_tm + TM_SLO, smem_desc(q + C::QLO) + 2 * (s & 3), kd, idesc, s != 0);
+        for (int s = 0; s < D / 16; s++) {                       // 16 dimensions = 32 bytes along K per instruction
+          mma_ss(s_tm, qh_desc + (s >> 2) * (C::Q_BLOCK >> 4) + 2 * (s & 3), kd + (s >> 2) * (C::K_BLOCK >> 4) + 2 * (s & 3), idesc, s != 0);
+          mma_ss(s_tm + TM_SLO, ql_desc + (s >> 2) * (C::Q_BLOCK >> 4) + 2 * (s & 3), kd + (s >> 2) * (C::K_BLOCK >> 4) + 2 * (s & 3), idesc, s != 0);
+        }
+        mma_commit(sh_base + S::SCORES + 8 * (t & 1));
       }
-      mma_commit(smem_u32(&sh.scores[t & 1]));
+      __syncwarp();
       return true;
     };
     while (alive && w.open(a, mp.row_blocks)) {
-      alive = wait(sh.queries, q_phase);
+      alive = __all_sync(0xffffffffu, wait(S::QUERIES, q_phase));
       q_phase ^= 1u;
       if (alive) { fence_after(); alive = score(it); }
       for (int j = w.tile0; alive && j < w.tile1; j++, it++) {
         if (j + 1 < w.tile1 && !score(it + 1)) { alive = false; break; }
-        if (!wait(sh.weights[it & 1], (it >> 1) & 1)) { alive = false; break; }
+        if (!__all_sync(0xffffffffu, wait(S::WEIGHTS + 8 * (it & 1), (it >> 1) & 1))) { alive = false; break; }
         fence_after();
         constexpr uint32_t idesc = idesc_f16(LANES, D);
         const uint32_t p_tm = tmem + TM_S + (it & 1) * TM_S_STEP, o_tm = tmem + TM_O + (it & 1) * TM_O_STEP;
-        const uint32_t vt = sm_base + C::RING + (it % ST) * C::STAGE + C::K_BYTES;
+        const uint64_t vd = v_desc + (uint64_t)((it % ST) * (C::STAGE >> 4));
+        if (lane == 0) {
 #pragma unroll
-        for (int s = 0; s < 4; s++) mma_ts(o_tm, p_tm + s * 16 + 8, smem_desc(vt) + 2 * s, idesc, s != 0);   // 16 tokens each; the small halves first
+          for (int s = 0; s < 4; s++) mma_ts(o_tm, p_tm + s * 16 + 8, vd + 2 * s, idesc, s != 0);   // 16 tokens each; the small halves first
 #pragma unroll
-        for (int s = 0; s < 4; s++) mma_ts(o_tm, p_tm + s * 16, smem_desc(vt) + 2 * s, idesc, 1);
-        mma_commit(smem_u32(&sh.outputs[it & 1]));
-        mma_commit(smem_u32(&sh.empty[it % ST]));
+          for (int s = 0; s < 4; s++) mma_ts(o_tm, p_tm + s * 16, vd + 2 * s, idesc, 1);
+          mma_commit(sh_base + S::OUTPUTS + 8 * (it & 1));
+          mma_commit(sh_base + S::EMPTY + 8 * (it % ST));
+        }
+        __syncwarp();
       }
       if (alive) w.close(a);
     }
@@ -640,7 +676,7 @@ int launch_many(b200q_ctx* ctx, const AttnArgs& a) {
   }
   ManyParams mp;
   mp.row_blocks = (int)(((int64_t)a.T * a.group + ROWS - 1) / ROWS);
-  mp.limit_ns = (unsigned long long)(ctx->wait_limit_s * 1e9);
+  mp.polls = (uint32_t)(ctx->wait_limit_s * 1e6) + 1000;
   const unsigned grid = (unsigned)ctx->sm_count;
   if (int e = kv_launch(ctx, kv_attention_many_kernel<D, CS>, dim3(grid), MANY_THREADS, Many<D>::SMEM, a, mp)) return e;
   return kv_launch(ctx, kv_attention_join_kernel<D, ROWS>, dim3(grid, (ROWS + 15) / 16), 256, 0, a, mp.row_blocks);
