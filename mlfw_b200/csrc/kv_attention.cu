@@ -37,6 +37,63 @@ __device__ __forceinline__ uint32_t v_at(int t, int c) {
   return k_at<64>(t, c);
 }
 
+// The end of a piece: the block's warps are added up, to the result when the piece is the whole item, else to the block's slot,
+// and the last piece of an item to arrive joins all of them in the order of the runs.  join_o holds outputs relative to the
+// largest of the warps' c.
+template <int D, int ROWS, int WARPS>
+__device__ __forceinline__ void finish_piece(const AttnArgs& a, const Run& run, int b, int rb, int head, int rows_here, int tile0, int tile1, int tiles,
+                                             int64_t at, const float (&join_c)[WARPS][ROWS], const float (&join_l)[WARPS][ROWS], const float* join_o,
+                                             uint32_t* arrived) {
+  const int tid = threadIdx.x;
+  const bool whole = tile0 == 0 && tile1 == tiles;
+  const int64_t item0 = at - tile0;                           // first tile of the item among all tiles
+  const int run0 = whole ? 0 : kv_run_of(run.all, item0), run1 = whole ? 0 : kv_run_of(run.all, item0 + tiles - 1);
+  float* mine = a.slots + (int64_t)(2 * blockIdx.x + (tile0 == 0 ? 1 : 0)) * KV_SLOT_FLOATS;
+  for (int x = tid; x < ROWS * D; x += 32 * WARPS) {
+    const int row = x / D, d = x % D;
+    float top = join_c[0][row], sum = 0.0f, val = 0.0f;
+#pragma unroll
+    for (int w = 1; w < WARPS; w++) top = fmaxf(top, join_c[w][row]);
+#pragma unroll
+    for (int w = 0; w < WARPS; w++) {
+      sum = fmaf(join_l[w][row], ex2(join_c[w][row] - top), sum);
+      val += join_o[(w * ROWS + row) * D + d];
+    }
+    if (!whole) {
+      __stcg(mine + row * D + d, val);
+      if (d == 0) { __stcg(mine + ROWS * D + row, top); __stcg(mine + ROWS * D + ROWS + row, sum); }
+    } else if (row < rows_here) {
+      int t;
+      a.out[row_offset(a, b, head, rb * ROWS + row, a.ld_o, D, t) + d] = sum == 0.0f ? 0.0f : val / sum * P_UNIT;
+    }
+  }
+  // ---- the last piece of an item to arrive joins all of them, in the order of the runs
+  if (!whole) {
+    __threadfence();
+    __syncthreads();
+    if (tid == 0) *arrived = atomicAdd(a.counters + run0, 1u);
+    __syncthreads();
+    if (*arrived == (uint32_t)(run1 - run0)) {
+      __threadfence();
+      if (tid == 0) a.counters[run0] = 0;
+      for (int x = tid; x < rows_here * D; x += 32 * WARPS) {
+        const int row = x / D, d = x % D;
+        auto piece = [&](int c) { return a.slots + (int64_t)(2 * c + (c == run0 ? 1 : 0)) * KV_SLOT_FLOATS; };
+        float top = C_NONE, sum = 0.0f, val = 0.0f;
+        for (int c = run0; c <= run1; c++) top = fmaxf(top, __ldcg(piece(c) + ROWS * D + row));
+        for (int c = run0; c <= run1; c++) {
+          const float* p = piece(c);
+          const float f = ex2(__ldcg(p + ROWS * D + row) - top);
+          sum = fmaf(__ldcg(p + ROWS * D + ROWS + row), f, sum);
+          val = fmaf(__ldcg(p + row * D + d), f, val);
+        }
+        int t;
+        a.out[row_offset(a, b, head, rb * ROWS + row, a.ld_o, D, t) + d] = sum == 0.0f ? 0.0f : val / sum * P_UNIT;
+      }
+    }
+  }
+}
+
 // RG groups of eight query rows.
 template <int D, int RG>
 __global__ void __launch_bounds__(32 * FEW_WARPS, 2) kv_attention_few_kernel(const AttnArgs a, int row_blocks) {
@@ -292,56 +349,313 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, 2) kv_attention_few_kernel(con
           *reinterpret_cast<float4*>(dst + c * CH + i) = make_float4(o[r][i][c] * f, o[r][i + 1][c] * f, o[r][i + 2][c] * f, o[r][i + 3][c] * f);
     }
     __syncthreads();
-    const bool whole = tile0 == 0 && tile1 == tiles;
-    const int64_t item0 = at - tile0;                           // first tile of the item among all tiles
-    const int run0 = whole ? 0 : kv_run_of(run.all, item0), run1 = whole ? 0 : kv_run_of(run.all, item0 + tiles - 1);
-    float* mine = a.slots + (int64_t)(2 * blockIdx.x + (tile0 == 0 ? 1 : 0)) * KV_SLOT_FLOATS;
+    finish_piece<D, ROWS, FEW_WARPS>(a, run, b, rb, head, rows_here, tile0, tile1, tiles, at, join_c, join_l, join_o, &arrived);
+    __syncthreads();                                            // the rings are about to be filled again
+    at += tile1 - tile0;
+    left -= tile1 - tile0;
+    tile0 = 0;
+    if (++head == a.g.heads) { head = 0; e++; }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Up to four rows (decoding with up to four query heads per cache head), on the integer tensor cores: m16n8k32 with the
+// codes as they are, so that K needs no conversion and V a transpose of bytes.  A query row and a row of weights are 32-bit
+// fixed-point numbers in four 8-bit digits, and the sixteen rows of the A operand are four rows times four digits: of row r
+// the rows 2 r and 2 r + 1 hold the digits 3 and 2, the rows 8 + 2 r and 9 + 2 r the digits 1 and 0.  A thread of an even
+// row therefore finds sum d3 code and sum d1 code, its neighbour in the odd row those of d2 and d0; each takes one of their two
+// columns after one exchange, so no score is computed twice.  Sums are 32-bit integers and exact: scores carry the rounding of
+// adding the digits, and the outputs are added up without rounding until a row's c changes (or 2^15 tokens have passed), when
+// they are converted, scaled and moved to binary32.  c = top - 26 leaves 5.5 bits before a larger weight (below 2^32) moves it.
+// Scales of V are taken relative to the power of two of the first tile's largest (kappa), so that tiny values keep their digits.
+//
+// About 310 instructions per warp and 32 tokens of 128 dimensions, where the binary16 form above takes 1300: bound by
+// reading the cache.  Twelve warps (D = 128: 64 integer sums, 32 outputs per thread) or sixteen (D = 64), one block per SM.
+// ---------------------------------------------------------------------------------------------------------------
+constexpr int IT = 32;                                          // tokens of a tile: two runs of sixteen, each in one page
+template <int D>
+struct Four {
+  static constexpr int WARPS = D == 128 ? 12 : 16, STAGES = D == 128 ? 2 : 3;
+  static constexpr int GRAN = 2 * KV_TILE * D + 2 * KV_TILE * 4, TILE = 2 * GRAN;   // sixteen tokens: K and V codes, K and V scales
+  static constexpr int RING = WARPS * STAGES * TILE;
+};
+__device__ __forceinline__ void imma(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {   // s8 x s8
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void imma_first(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+      : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
+}
+__device__ __forceinline__ void imma_u8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {   // u8 x s8
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float lds_f(uint32_t a) {
+  float r;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(r) : "r"(a));
+  return r;
+}
+
+template <int D>
+__global__ void __launch_bounds__(32 * Four<D>::WARPS, 1) kv_attention_four_kernel(const AttnArgs a, int row_blocks) {
+  using C = Four<D>;
+  constexpr int ROWS = 4, WARPS = C::WARPS, ST = C::STAGES, KS = D / 32, CH = D / 8, W = D / 32;
+  constexpr float C_BELOW = 26.0f, C_SLACK = 31.5f;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float join_c[WARPS][ROWS], join_l[WARPS][ROWS];
+  __shared__ uint32_t arrived;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, t4 = lane & 3, r = g8 >> 1, odd = g8 & 1;
+  const uint32_t ring = smem_u32(smem) + warp * (ST * C::TILE);
+  float* join_o = reinterpret_cast<float*>(smem);               // [warp][row][D], over the rings between pieces
+  const uint32_t k_dst = ring + k_at<D>(lane / (D / 16), lane % (D / 16)), v_dst = ring + KV_TILE * D + v_at<D>(lane / (D / 16), lane % (D / 16));
+  const uint32_t k_src = ring + k_at<D>(g8, t4);
+  const uint32_t v_src = ring + KV_TILE * D + (D == 128 ? v_at<D>(2 * t4, g8) : v_at<D>(2 * t4, g8 >> 1) + (g8 & 1) * 8);
+  const uint32_t s_src = ring + 2 * KV_TILE * D + (2 * t4 + odd) * 4;
+  // weights of this thread's two sums; selectors of its two digits among (own, partner's) weights in the order of the tokens
+  const float w0 = odd ? 0x1p16f : 0x1p24f, w2 = odd ? 1.0f : 0x1p8f;
+  const uint32_t sel = odd ? 0x0426u : 0x5173u;
+
+  kv_after_previous();
+  const Run run = find_run<ROWS, IT, WARPS>(a, row_blocks);
+  int64_t left = run.end - run.begin, at = run.begin;
+  int e = run.e, head = run.head, tile0 = run.tile;
+
+  while (left > 0) {
+    const int b = e / row_blocks, rb = e - b * row_blocks;
+    const int64_t first = a.start[b];
+    const int n = kv_rows_in_use(a.count, b, a.T);
+    const int tiles = kv_tiles(a.g, first, n, a.group, ROWS, rb, a.tree != nullptr, IT);
+    if (tiles == 0) { e++; head = 0; tile0 = 0; continue; }
+    const int64_t vis = kv_visible(a.g, first, n, a.group, ROWS, rb, a.tree != nullptr);
+    const int tile1 = (int)min((int64_t)tiles, tile0 + left);
+    const int rows_here = min(ROWS, n * a.group - rb * ROWS);
+    const int plain = first <= 0 ? 0 : (int)(first / IT);       // tiles of cached tokens only
+    if (tid == 0 && (first < 0 || first + n > (a.g.max_pages << a.g.page_shift))) atomicOr(a.status, STATUS_BAD_INDEX);
+
+    // ---- the ring: a tile's two runs of sixteen tokens into slot s
+    const int32_t* table = a.page_table + (int64_t)b * a.g.max_pages;
+    const int64_t in_table = min(vis, a.g.max_pages << a.g.page_shift);
+    auto page_of = [&](int i, int h) -> int {                   // -1: nothing of the run is visible
+      const int64_t pos = (int64_t)i * IT + h * 16;
+      return (i < tile1 && pos < in_table) ? __ldg(table + (pos >> a.g.page_shift)) : -1;
+    };
+    auto fetch = [&](int i, int page, int h, int s) {
+      if ((uint32_t)page < (uint32_t)a.g.pages) {
+        const int64_t row = (((int64_t)page * a.g.heads + head) << a.g.page_shift) + ((i * IT + h * 16) & ((1 << a.g.page_shift) - 1));
+        const uint32_t to = s * C::TILE + h * C::GRAN;
+        const int8_t *kp = a.k + row * D + lane * 16, *vp = a.v + row * D + lane * 16;
 #pragma unroll
-    for (int x = 0; x < ROWS * D / (32 * FEW_WARPS); x++) {
-      const int row = (x * 32 * FEW_WARPS + tid) / D, d = tid % D;
-      float top = join_c[0][row], sum = 0.0f, val = 0.0f;
+        for (int x = 0; x < D / 32; x++) cp16(k_dst + to + x * 512, kp + x * 512);
 #pragma unroll
-      for (int w = 1; w < FEW_WARPS; w++) top = fmaxf(top, join_c[w][row]);
-#pragma unroll
-      for (int w = 0; w < FEW_WARPS; w++) {
-        sum = fmaf(join_l[w][row], ex2(join_c[w][row] - top), sum);
-        val += join_o[(w * ROWS + row) * D + d];
+        for (int x = 0; x < D / 32; x++) cp16(((D == 128 && (x & 1)) ? v_dst ^ 64u : v_dst) + to + x * 512, vp + x * 512);
+        if (lane < 8) cp16(ring + 2 * KV_TILE * D + lane * 16 + to, (lane < 4 ? a.ks : a.vs) + row + (lane & 3) * 4);
       }
-      if (!whole) {
-        __stcg(mine + row * D + d, val);
-        if (d == 0) { __stcg(mine + ROWS * D + row, top); __stcg(mine + ROWS * D + ROWS + row, sum); }
-      } else if (row < rows_here) {
-        int t;
-        a.out[row_offset(a, b, head, rb * ROWS + row, a.ld_o, D, t) + d] = sum == 0.0f ? 0.0f : val / sum * P_UNIT;
+    };
+    int pg[ST][2];                                              // pages of the tiles in the ring, then of the next one
+#pragma unroll
+    for (int s = 0; s < ST; s++) { pg[s][0] = page_of(tile0 + warp + s * WARPS, 0); pg[s][1] = page_of(tile0 + warp + s * WARPS, 1); }
+#pragma unroll
+    for (int s = 0; s < ST - 1; s++) {
+      fetch(tile0 + warp + s * WARPS, pg[s][0], 0, s);
+      fetch(tile0 + warp + s * WARPS, pg[s][1], 1, s);
+      cp_commit();
+    }
+
+    // ---- the query row r: digits of dimensions 64 m + 16 t4 + 8 h + (0..7), k-step 2 m + h
+    float rs;
+    int row_t;
+    uint64_t row_seen;
+    uint32_t qa[KS][4];
+    {
+      const bool used = r < rows_here;
+      int t = 0;
+      const float* src = a.q + row_offset(a, b, head, rb * ROWS + (used ? r : 0), a.ld_q, D, t);
+      row_t = used ? t : -1;
+      row_seen = used && a.tree ? a.tree[(int64_t)b * a.T + t] : 0;
+      float4 x[2 * KS];
+      uint32_t top = 0;
+#pragma unroll
+      for (int s = 0; s < 2 * KS; s++) {
+        x[s] = used ? __ldg(reinterpret_cast<const float4*>(src + (s >> 2) * 64 + t4 * 16 + (s & 3) * 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        top = max(max(top, max(__float_as_uint(x[s].x) & 0x7fffffffu, __float_as_uint(x[s].y) & 0x7fffffffu)),
+                  max(__float_as_uint(x[s].z) & 0x7fffffffu, __float_as_uint(x[s].w) & 0x7fffffffu));
+      }
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const bool finite = top < 0x7f800000u;
+      const int ex = max((int)(top >> 23), 30) - 127;           // exponent of the row's largest element; tiny rows keep fewer digits
+      const float up = finite ? pow2(29 - ex) : 0.0f;           // |x| <= 2^30
+      rs = finite ? a.scale_log2e * pow2(ex - 29) : __int_as_float(0x7fc00000);   // a NaN or an infinity in the row: every score NaN
+#pragma unroll
+      for (int s = 0; s < 2 * KS; s++) {
+        uint32_t d[4];
+        const float y[4] = {x[s].x, x[s].y, x[s].z, x[s].w};
+#pragma unroll
+        for (int c = 0; c < 4; c++) d[c] = ((uint32_t)__float2int_rn(finite ? y[c] * up : 0.0f) + 0x00808080u) ^ 0x00808080u;   // bytes = signed digits
+        const uint32_t hi01 = __byte_perm(d[0], d[1], odd ? 0x0062 : 0x0073), hi23 = __byte_perm(d[2], d[3], odd ? 0x0062 : 0x0073);
+        const uint32_t lo01 = __byte_perm(d[0], d[1], odd ? 0x0040 : 0x0051), lo23 = __byte_perm(d[2], d[3], odd ? 0x0040 : 0x0051);
+        qa[s >> 1][(s & 1) * 2] = __byte_perm(hi01, hi23, 0x5410);
+        qa[s >> 1][(s & 1) * 2 + 1] = __byte_perm(lo01, lo23, 0x5410);
       }
     }
-    // ---- the last piece of an item to arrive joins all of them, in the order of the runs
-    if (!whole) {
-      __threadfence();
-      __syncthreads();
-      if (tid == 0) arrived = atomicAdd(a.counters + run0, 1u);
-      __syncthreads();
-      if (arrived == (uint32_t)(run1 - run0)) {
-        __threadfence();
-        if (tid == 0) a.counters[run0] = 0;
+
+    int acc[CH][4];
+    float o[CH][2], c_run = C_NONE, l = 0.0f, kf = 0.0f;        // kf: 2^-kappa, 0 until a tile has a scale
+#pragma unroll
+    for (int i = 0; i < CH; i++) { acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0; o[i][0] = o[i][1] = 0.0f; }
+    int since = 0;                                              // tiles in the integer sums
+    auto move_sums = [&](float f) {                             // o = (o + the integer sums) * f
+#pragma unroll
+      for (int i = 0; i < CH; i++) {
+        o[i][0] = (o[i][0] + fmaf((float)acc[i][0], w0, (float)acc[i][2] * w2)) * f;
+        o[i][1] = (o[i][1] + fmaf((float)acc[i][1], w0, (float)acc[i][3] * w2)) * f;
+        acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0;
+      }
+      since = 0;
+    };
+
+    int slot = 0;
 #pragma unroll 1
-        for (int x = 0; x < ROWS * D / (32 * FEW_WARPS); x++) {
-          const int row = (x * 32 * FEW_WARPS + tid) / D, d = tid % D;
-          if (row >= rows_here) continue;
-          auto piece = [&](int c) { return a.slots + (int64_t)(2 * c + (c == run0 ? 1 : 0)) * KV_SLOT_FLOATS; };
-          float top = C_NONE, sum = 0.0f, val = 0.0f;
-          for (int c = run0; c <= run1; c++) top = fmaxf(top, __ldcg(piece(c) + ROWS * D + row));
-          for (int c = run0; c <= run1; c++) {
-            const float* p = piece(c);
-            const float f = ex2(__ldcg(p + ROWS * D + row) - top);
-            sum = fmaf(__ldcg(p + ROWS * D + ROWS + row), f, sum);
-            val = fmaf(__ldcg(p + row * D + d), f, val);
-          }
-          int t;
-          a.out[row_offset(a, b, head, rb * ROWS + row, a.ld_o, D, t) + d] = sum == 0.0f ? 0.0f : val / sum * P_UNIT;
+    for (int i = tile0 + warp; i < tile1; i += WARPS) {
+      cp_wait<ST - 2>();
+      __syncwarp();
+      const bool there0 = (uint32_t)pg[0][0] < (uint32_t)a.g.pages, there1 = (uint32_t)pg[0][1] < (uint32_t)a.g.pages;
+      const uint32_t here = slot * C::TILE;
+      {
+        const int s = slot == 0 ? ST - 1 : slot - 1, nx = i + (ST - 1) * WARPS;
+        fetch(nx, pg[ST - 1][0], 0, s);
+        fetch(nx, pg[ST - 1][1], 1, s);
+        cp_commit();
+      }
+#pragma unroll
+      for (int s = 0; s + 1 < ST; s++) { pg[s][0] = pg[s + 1][0]; pg[s][1] = pg[s + 1][1]; }
+      pg[ST - 1][0] = page_of(i + ST * WARPS, 0);
+      pg[ST - 1][1] = page_of(i + ST * WARPS, 1);
+      slot = slot + 1 == ST ? 0 : slot + 1;
+
+      // ---- scores: four blocks of eight tokens; this thread's are 8 j + 2 t4 + odd
+      float z[4], vs[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const uint32_t at_k = k_src + here + (j >> 1) * C::GRAN + (j & 1) * 8 * D;
+        int c[4];
+#pragma unroll
+        for (int mm = 0; mm < D / 64; mm++) {
+          const uint4 x = lds128(mm ? (k_src ^ 64u) + (at_k - k_src) : at_k);
+          if (mm == 0) imma_first(c, qa[0][0], qa[0][1], qa[0][2], qa[0][3], x.x, x.y);
+          else imma(c, qa[2 * mm][0], qa[2 * mm][1], qa[2 * mm][2], qa[2 * mm][3], x.x, x.y);
+          imma(c, qa[2 * mm + 1][0], qa[2 * mm + 1][1], qa[2 * mm + 1][2], qa[2 * mm + 1][3], x.z, x.w);
+        }
+        const float s0 = fmaf((float)c[0], w0, (float)c[2] * w2), s1 = fmaf((float)c[1], w0, (float)c[3] * w2);
+        const float got = __shfl_xor_sync(0xffffffffu, odd ? s0 : s1, 4);
+        const uint32_t at_s = s_src + here + (j >> 1) * C::GRAN + (j & 1) * 32;
+        z[j] = ((odd ? s1 : s0) + got) * (lds_f(at_s) * rs);
+        vs[j] = lds_f(at_s + 64);
+      }
+      const bool all = i < plain && there0 && there1;           // the same in the whole warp
+      if (!all) {
+        const int64_t pos = (int64_t)i * IT, end = min(vis, first + n);
+        if (lane == 0 && ((!there0 && pos < vis) || (!there1 && pos + 16 < vis))) atomicOr(a.status, STATUS_BAD_INDEX);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const int64_t p = pos + 8 * j + 2 * t4 + odd, q = p - first;
+          const bool there = (j < 2 ? there0 : there1) && p < end;
+          if (!there) vs[j] = 0.0f;                             // behind the last row in use anything may stand
+          if (!(there && (q < 0 || (a.tree ? (row_seen >> q) & 1 : q <= row_t)))) z[j] = NEG_INF;
         }
       }
+      if (kf == 0.0f) {                                         // kappa: the power of two of the first scales
+        float big = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
+#pragma unroll
+        for (int x = 1; x < 32; x <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, x));
+        if (big > 0.0f) kf = pow2(127 - min(max(__float_as_int(big) >> 23, 1), 253));
+      }
+      float lv[4], top = NEG_INF;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        vs[j] *= kf;
+        lv[j] = fmaxf(log2_raw(vs[j]), -88.0f);
+        top = fmaxf(top, z[j] + lv[j]);
+      }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+      const bool grow = top > c_run + C_SLACK;
+      if (__any_sync(0xffffffffu, grow) || since == 1024) {
+        const float c_new = grow ? top - C_BELOW : c_run, f = ex2(c_run - c_new);
+        move_sums(f);
+        l *= f;
+        c_run = c_new;
+      }
+      since++;
+      float sum = 0.0f;
+      uint32_t t[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const float p = ex2(z[j] - c_run);
+        sum += p;
+        const uint32_t w = __float2uint_rn(p * vs[j]);
+        t[j] = __byte_perm(w, __shfl_xor_sync(0xffffffffu, w, 4), sel);   // digits (3, 3, 1, 1) or (2, 2, 0, 0) of two neighbouring tokens
+      }
+      l = fmaf(sum, P_UNIT, l);
+      const uint32_t p0 = __byte_perm(t[0], t[1], 0x5410), p1 = __byte_perm(t[0], t[1], 0x7632);
+      const uint32_t p2 = __byte_perm(t[2], t[3], 0x5410), p3 = __byte_perm(t[2], t[3], 0x7632);
+
+      // ---- sums of weight * code: tokens 2 t4, 2 t4 + 1, 8 + 2 t4, 9 + 2 t4 of either run are four neighbouring k
+      uint32_t y[8][W];
+#pragma unroll
+      for (int c = 0; c < 8; c++) {
+        const uint32_t to = here + (c >> 2) * C::GRAN;
+        if (D == 128) {
+          const uint4 x = lds128(v_src + to + (c & 1) * 128 + ((c >> 1) & 1) * 1024);
+          y[c][0] = x.x; y[c][1] = x.y; y[c][W - 2] = x.z; y[c][W - 1] = x.w;
+        } else {
+          const uint2 x = lds64(((c & 1) ? v_src ^ 64u : v_src) + to + ((c >> 1) & 1) * 512);
+          y[c][0] = x.x; y[c][1] = x.y;
+        }
+      }
+#pragma unroll
+      for (int w = 0; w < W; w++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {                           // two dimensions at a time: bytes (0, 1) and (2, 3) of a word
+          const uint32_t s = h ? 0x7362 : 0x5140;
+          const uint32_t u0 = __byte_perm(y[0][w], y[1][w], s), u1 = __byte_perm(y[2][w], y[3][w], s);
+          const uint32_t u2 = __byte_perm(y[4][w], y[5][w], s), u3 = __byte_perm(y[6][w], y[7][w], s);
+          imma_u8(acc[w * 4 + h * 2], p0, p1, p2, p3, __byte_perm(u0, u1, 0x5410), __byte_perm(u2, u3, 0x5410));
+          imma_u8(acc[w * 4 + h * 2 + 1], p0, p1, p2, p3, __byte_perm(u0, u1, 0x7632), __byte_perm(u2, u3, 0x7632));
+        }
     }
+    cp_wait<0>();
+    move_sums(1.0f);
+
+    // ---- the warps' results of the piece
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    l += __shfl_xor_sync(0xffffffffu, l, 4);
+    if (t4 == 0 && !odd) { join_c[warp][r] = c_run; join_l[warp][r] = l * 0x1p-40f; }
+    __syncthreads();                                            // every ring is drained
+    {
+      float top = join_c[0][r];
+#pragma unroll
+      for (int w = 1; w < WARPS; w++) top = fmaxf(top, join_c[w][r]);
+      // 2^-40, as the sums of p, before 2^kappa: huge values of V times weights of 2^31 would leave binary32
+      const float f = ex2(c_run - top) * 0x1p-40f;
+      const float kappa = kf == 0.0f ? 1.0f : pow2(127 - (__float_as_int(kf) >> 23));
+      float* dst = join_o + (warp * ROWS + r) * D + (2 * t4 + odd) * CH;
+#pragma unroll
+      for (int i = 0; i < CH; i += 4) {
+        float v[4];
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+          const float got = __shfl_xor_sync(0xffffffffu, odd ? o[i + c][0] : o[i + c][1], 4);
+          v[c] = ((odd ? o[i + c][1] : o[i + c][0]) + got) * f * kappa;
+        }
+        *reinterpret_cast<float4*>(dst + i) = make_float4(v[0], v[1], v[2], v[3]);
+      }
+    }
+    __syncthreads();
+    finish_piece<D, ROWS, WARPS>(a, run, b, rb, head, rows_here, tile0, tile1, tiles, at, join_c, join_l, join_o, &arrived);
     __syncthreads();                                            // the rings are about to be filled again
     at += tile1 - tile0;
     left -= tile1 - tile0;
@@ -362,6 +676,17 @@ int launch_few(b200q_ctx* ctx, const AttnArgs& a) {
   return kv_launch(ctx, kv_attention_few_kernel<D, RG>, dim3(ctx->sm_count * KV_BLOCKS_PER_SM), 32 * FEW_WARPS, smem, a, row_blocks);
 }
 
+template <int D>
+int launch_four(b200q_ctx* ctx, const AttnArgs& a) {
+  constexpr uint32_t ready = 1u << (D == 64 ? 12 : 13);
+  if (!(ctx->kv_ready & ready)) {
+    B200Q_CHECK_CUDA(cudaFuncSetAttribute(kv_attention_four_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Four<D>::RING));
+    ctx->kv_ready |= ready;
+  }
+  const int row_blocks = (int)(((int64_t)a.T * a.group + 3) / 4);
+  return kv_launch(ctx, kv_attention_four_kernel<D>, dim3(ctx->sm_count), 32 * Four<D>::WARPS, Four<D>::RING, a, row_blocks);
+}
+
 }  // namespace
 
 int kv_workspace(b200q_ctx* ctx) {
@@ -380,6 +705,7 @@ int launch_kv_attention(b200q_ctx* ctx, const b200q_kv_cache& c, const KvBatch& 
                    (float*)((uint8_t*)ctx->ws_kv.ptr + kv_counter_bytes(ctx) + kv_item_bytes(ctx)), (int4*)((uint8_t*)ctx->ws_kv.ptr + kv_counter_bytes(ctx))};
   const int64_t rows = (int64_t)s.T * a.group;
   int e;
+  if (rows <= 4) return c.head_dim == 64 ? launch_four<64>(ctx, a) : launch_four<128>(ctx, a);
   // Measured on both sides of the border: 16 rows (12 heads of 64, 32 sequences of up to 1000 tokens) 61 us here and 88 us
   // there with everything around it; 124 rows (head dimension 128, 8 sequences of up to 5000 tokens) 209 and 129 us.
   if (rows > 16) return launch_kv_attention_many(ctx, a, c.head_dim);
