@@ -377,7 +377,7 @@ template <int D>
 struct Four {
   static constexpr int WARPS = D == 128 ? 12 : 16, STAGES = D == 128 ? 2 : 3;
   static constexpr int GRAN = 2 * KV_TILE * D + 2 * KV_TILE * 4, TILE = 2 * GRAN;   // sixteen tokens: K and V codes, K and V scales
-  static constexpr int RING = WARPS * STAGES * TILE;
+  static constexpr int RING = WARPS * STAGES * TILE, SLOT = 4 * (D + 2) * 4, SMEM = RING + WARPS * SLOT;
 };
 __device__ __forceinline__ void imma(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {   // s8 x s8
   asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -397,17 +397,36 @@ __device__ __forceinline__ float lds_f(uint32_t a) {
   return r;
 }
 
+// One item after another along a run, as a warp walks it.
+struct Item {
+  int e, head, b, rb, n, tiles;
+  int64_t first, vis;
+  template <int ROWS>
+  __device__ __forceinline__ void load(const AttnArgs& a, int row_blocks) {   // skips what has no tile; the caller knows that one follows
+    while (true) {
+      b = e / row_blocks; rb = e - b * row_blocks;
+      first = a.start[b];
+      n = kv_rows_in_use(a.count, b, a.T);
+      tiles = kv_tiles(a.g, first, n, a.group, ROWS, rb, a.tree != nullptr, IT);
+      if (tiles != 0) break;
+      e++;
+    }
+    vis = kv_visible(a.g, first, n, a.group, ROWS, rb, a.tree != nullptr);
+  }
+};
+
+// Every warp has a run of its own, a part of the block's, and a ring that it keeps full across the items of its run; the warps
+// never wait for one another.  Results of an item that several warps of the block worked on are joined by the last of them
+// through shared memory, and those of an item that several blocks worked on by the last warp of the last block.
 template <int D>
 __global__ void __launch_bounds__(32 * Four<D>::WARPS, 1) kv_attention_four_kernel(const AttnArgs a, int row_blocks) {
   using C = Four<D>;
   constexpr int ROWS = 4, WARPS = C::WARPS, ST = C::STAGES, KS = D / 32, CH = D / 8, W = D / 32;
   constexpr float C_BELOW = 26.0f, C_SLACK = 31.5f;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float join_c[WARPS][ROWS], join_l[WARPS][ROWS];
-  __shared__ uint32_t arrived;
+  __shared__ int arrived[WARPS];                                // pieces of an item within the block, by the first warp that has it
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, t4 = lane & 3, r = g8 >> 1, odd = g8 & 1;
   const uint32_t ring = smem_u32(smem) + warp * (ST * C::TILE);
-  float* join_o = reinterpret_cast<float*>(smem);               // [warp][row][D], over the rings between pieces
   const uint32_t k_dst = ring + k_at<D>(lane / (D / 16), lane % (D / 16)), v_dst = ring + KV_TILE * D + v_at<D>(lane / (D / 16), lane % (D / 16));
   const uint32_t k_src = ring + k_at<D>(g8, t4);
   const uint32_t v_src = ring + KV_TILE * D + (D == 128 ? v_at<D>(2 * t4, g8) : v_at<D>(2 * t4, g8 >> 1) + (g8 & 1) * 8);
@@ -417,50 +436,83 @@ __global__ void __launch_bounds__(32 * Four<D>::WARPS, 1) kv_attention_four_kern
   const uint32_t sel = odd ? 0x0426u : 0x5173u;
 
   kv_after_previous();
-  const Run run = find_run<ROWS, IT, WARPS>(a, row_blocks);
-  int64_t left = run.end - run.begin, at = run.begin;
-  int e = run.e, head = run.head, tile0 = run.tile;
+  if (tid < WARPS) arrived[tid] = 0;
+  const Run run = find_run<ROWS, IT, WARPS>(a, row_blocks);     // (its barriers publish `arrived`)
+  if (run.begin == run.end) return;
+  const KvRuns parts = kv_runs(run.end - run.begin, 1, WARPS);
+  if (warp >= parts.runs) return;
+  const int64_t begin = kv_run_begin(parts, warp);
+  int left = (int)(kv_run_begin(parts, warp + 1) - begin);      // this warp's tiles: below 2^31 / 148 blocks / warps
+  int64_t at = run.begin + begin;                               // first tile of the piece among all tiles
 
-  while (left > 0) {
-    const int b = e / row_blocks, rb = e - b * row_blocks;
-    const int64_t first = a.start[b];
-    const int n = kv_rows_in_use(a.count, b, a.T);
-    const int tiles = kv_tiles(a.g, first, n, a.group, ROWS, rb, a.tree != nullptr, IT);
-    if (tiles == 0) { e++; head = 0; tile0 = 0; continue; }
-    const int64_t vis = kv_visible(a.g, first, n, a.group, ROWS, rb, a.tree != nullptr);
-    const int tile1 = (int)min((int64_t)tiles, tile0 + left);
-    const int rows_here = min(ROWS, n * a.group - rb * ROWS);
-    const int plain = first <= 0 ? 0 : (int)(first / IT);       // tiles of cached tokens only
-    if (tid == 0 && (first < 0 || first + n > (a.g.max_pages << a.g.page_shift))) atomicOr(a.status, STATUS_BAD_INDEX);
-
-    // ---- the ring: a tile's two runs of sixteen tokens into slot s
-    const int32_t* table = a.page_table + (int64_t)b * a.g.max_pages;
-    const int64_t in_table = min(vis, a.g.max_pages << a.g.page_shift);
-    auto page_of = [&](int i, int h) -> int {                   // -1: nothing of the run is visible
-      const int64_t pos = (int64_t)i * IT + h * 16;
-      return (i < tile1 && pos < in_table) ? __ldg(table + (pos >> a.g.page_shift)) : -1;
-    };
-    auto fetch = [&](int i, int page, int h, int s) {
-      if ((uint32_t)page < (uint32_t)a.g.pages) {
-        const int64_t row = (((int64_t)page * a.g.heads + head) << a.g.page_shift) + ((i * IT + h * 16) & ((1 << a.g.page_shift) - 1));
-        const uint32_t to = s * C::TILE + h * C::GRAN;
-        const int8_t *kp = a.k + row * D + lane * 16, *vp = a.v + row * D + lane * 16;
-#pragma unroll
-        for (int x = 0; x < D / 32; x++) cp16(k_dst + to + x * 512, kp + x * 512);
-#pragma unroll
-        for (int x = 0; x < D / 32; x++) cp16(((D == 128 && (x & 1)) ? v_dst ^ 64u : v_dst) + to + x * 512, vp + x * 512);
-        if (lane < 8) cp16(ring + 2 * KV_TILE * D + lane * 16 + to, (lane < 4 ? a.ks : a.vs) + row + (lane & 3) * 4);
-      }
-    };
-    int pg[ST][2];                                              // pages of the tiles in the ring, then of the next one
-#pragma unroll
-    for (int s = 0; s < ST; s++) { pg[s][0] = page_of(tile0 + warp + s * WARPS, 0); pg[s][1] = page_of(tile0 + warp + s * WARPS, 1); }
-#pragma unroll
-    for (int s = 0; s < ST - 1; s++) {
-      fetch(tile0 + warp + s * WARPS, pg[s][0], 0, s);
-      fetch(tile0 + warp + s * WARPS, pg[s][1], 1, s);
-      cp_commit();
+  Item it;                                                      // the item of the piece
+  it.e = run.e; it.head = run.head;
+  it.load<ROWS>(a, row_blocks);
+  int tile = run.tile;
+  for (int64_t skip = begin; skip > 0;) {                       // from the block's first tile to the warp's
+    const int64_t rest = (int64_t)(a.g.heads - it.head) * it.tiles - tile;
+    if (skip >= rest) {
+      skip -= rest;
+      it.e++; it.head = 0; tile = 0;
+      it.load<ROWS>(a, row_blocks);
+    } else {
+      const int64_t to = it.head * (int64_t)it.tiles + tile + skip;
+      it.head = (int)kv_div(to, it.tiles);
+      tile = (int)(to - (int64_t)it.head * it.tiles);
+      skip = 0;
     }
+  }
+
+  // ---- the ring: tiles in the order of the run, ST - 1 ahead of their use.  `ahead` walks by itself; page0 and page1 are the
+  // pages of its next tile's two runs of sixteen tokens, -1 where nothing is visible.
+  Item ahead = it;
+  int ahead_tile = tile, ahead_left = left, page0, page1;
+  uint32_t there = 0;                                           // two bits per tile in the ring, the oldest lowest
+  auto pages = [&]() {
+    const int64_t pos = (int64_t)ahead_tile * IT;
+    const int32_t* table = a.page_table + (int64_t)ahead.b * a.g.max_pages;
+    page0 = ahead_left > 0 && pos < ahead.vis ? __ldg(table + (pos >> a.g.page_shift)) : -1;
+    page1 = ahead_left > 0 && pos + 16 < ahead.vis ? __ldg(table + ((pos + 16) >> a.g.page_shift)) : -1;
+  };
+  auto fetch = [&](int s, int place) {
+    if (ahead_left > 0) {
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const int page = h ? page1 : page0;
+        if ((uint32_t)page < (uint32_t)a.g.pages) {
+          const int64_t row = (((int64_t)page * a.g.heads + ahead.head) << a.g.page_shift) + ((ahead_tile * IT + h * 16) & ((1 << a.g.page_shift) - 1));
+          const uint32_t to = s * C::TILE + h * C::GRAN;
+          const int8_t *kp = a.k + row * D + lane * 16, *vp = a.v + row * D + lane * 16;
+#pragma unroll
+          for (int x = 0; x < D / 32; x++) cp16(k_dst + to + x * 512, kp + x * 512);
+#pragma unroll
+          for (int x = 0; x < D / 32; x++) cp16(((D == 128 && (x & 1)) ? v_dst ^ 64u : v_dst) + to + x * 512, vp + x * 512);
+          if (lane < 8) cp16(ring + 2 * KV_TILE * D + lane * 16 + to, (lane < 4 ? a.ks : a.vs) + row + (lane & 3) * 4);
+          there |= (1u + h) << (2 * place);
+        }
+      }
+      ahead_left--;
+      if (++ahead_tile == ahead.tiles) {
+        ahead_tile = 0;
+        if (++ahead.head == a.g.heads) {
+          ahead.head = 0; ahead.e++;
+          if (ahead_left > 0) ahead.load<ROWS>(a, row_blocks);
+        }
+      }
+      pages();
+    }
+    cp_commit();
+  };
+  pages();
+#pragma unroll
+  for (int s = 0; s < ST - 1; s++) fetch(s, s);
+
+  int slot = 0;
+  while (left > 0) {
+    const int tile0 = tile, tile1 = min(it.tiles, tile0 + left), rows_here = min(ROWS, it.n * a.group - it.rb * ROWS);
+    const int64_t first = it.first;
+    const int plain = first <= 0 ? 0 : (int)(first / IT);       // tiles of cached tokens only
+    if (lane == 0 && (first < 0 || first + it.n > (a.g.max_pages << a.g.page_shift))) atomicOr(a.status, STATUS_BAD_INDEX);
 
     // ---- the query row r: digits of dimensions 64 m + 16 t4 + 8 h + (0..7), k-step 2 m + h
     float rs;
@@ -470,9 +522,9 @@ __global__ void __launch_bounds__(32 * Four<D>::WARPS, 1) kv_attention_four_kern
     {
       const bool used = r < rows_here;
       int t = 0;
-      const float* src = a.q + row_offset(a, b, head, rb * ROWS + (used ? r : 0), a.ld_q, D, t);
+      const float* src = a.q + row_offset(a, it.b, it.head, it.rb * ROWS + (used ? r : 0), a.ld_q, D, t);
       row_t = used ? t : -1;
-      row_seen = used && a.tree ? a.tree[(int64_t)b * a.T + t] : 0;
+      row_seen = used && a.tree ? a.tree[(int64_t)it.b * a.T + t] : 0;
       float4 x[2 * KS];
       uint32_t top = 0;
 #pragma unroll
@@ -515,34 +567,25 @@ __global__ void __launch_bounds__(32 * Four<D>::WARPS, 1) kv_attention_four_kern
       since = 0;
     };
 
-    int slot = 0;
 #pragma unroll 1
-    for (int i = tile0 + warp; i < tile1; i += WARPS) {
+    for (int i = tile0; i < tile1; i++) {
       cp_wait<ST - 2>();
       __syncwarp();
-      const bool there0 = (uint32_t)pg[0][0] < (uint32_t)a.g.pages, there1 = (uint32_t)pg[0][1] < (uint32_t)a.g.pages;
+      const bool there0 = there & 1, there1 = there & 2;
+      there >>= 2;
       const uint32_t here = slot * C::TILE;
-      {
-        const int s = slot == 0 ? ST - 1 : slot - 1, nx = i + (ST - 1) * WARPS;
-        fetch(nx, pg[ST - 1][0], 0, s);
-        fetch(nx, pg[ST - 1][1], 1, s);
-        cp_commit();
-      }
-#pragma unroll
-      for (int s = 0; s + 1 < ST; s++) { pg[s][0] = pg[s + 1][0]; pg[s][1] = pg[s + 1][1]; }
-      pg[ST - 1][0] = page_of(i + ST * WARPS, 0);
-      pg[ST - 1][1] = page_of(i + ST * WARPS, 1);
+      fetch(slot == 0 ? ST - 1 : slot - 1, ST - 2);
       slot = slot + 1 == ST ? 0 : slot + 1;
 
       // ---- scores: four blocks of eight tokens; this thread's are 8 j + 2 t4 + odd
       float z[4], vs[4];
 #pragma unroll
       for (int j = 0; j < 4; j++) {
-        const uint32_t at_k = k_src + here + (j >> 1) * C::GRAN + (j & 1) * 8 * D;
+        const uint32_t at_k = here + (j >> 1) * C::GRAN + (j & 1) * 8 * D;
         int c[4];
 #pragma unroll
         for (int mm = 0; mm < D / 64; mm++) {
-          const uint4 x = lds128(mm ? (k_src ^ 64u) + (at_k - k_src) : at_k);
+          const uint4 x = lds128((mm ? k_src ^ 64u : k_src) + at_k);
           if (mm == 0) imma_first(c, qa[0][0], qa[0][1], qa[0][2], qa[0][3], x.x, x.y);
           else imma(c, qa[2 * mm][0], qa[2 * mm][1], qa[2 * mm][2], qa[2 * mm][3], x.x, x.y);
           imma(c, qa[2 * mm + 1][0], qa[2 * mm + 1][1], qa[2 * mm + 1][2], qa[2 * mm + 1][3], x.z, x.w);
@@ -555,14 +598,14 @@ __global__ void __launch_bounds__(32 * Four<D>::WARPS, 1) kv_attention_four_kern
       }
       const bool all = i < plain && there0 && there1;           // the same in the whole warp
       if (!all) {
-        const int64_t pos = (int64_t)i * IT, end = min(vis, first + n);
-        if (lane == 0 && ((!there0 && pos < vis) || (!there1 && pos + 16 < vis))) atomicOr(a.status, STATUS_BAD_INDEX);
+        const int64_t pos = (int64_t)i * IT, end = min(it.vis, first + it.n);
+        if (lane == 0 && ((!there0 && pos < it.vis) || (!there1 && pos + 16 < it.vis))) atomicOr(a.status, STATUS_BAD_INDEX);
 #pragma unroll
         for (int j = 0; j < 4; j++) {
           const int64_t p = pos + 8 * j + 2 * t4 + odd, q = p - first;
-          const bool there = (j < 2 ? there0 : there1) && p < end;
-          if (!there) vs[j] = 0.0f;                             // behind the last row in use anything may stand
-          if (!(there && (q < 0 || (a.tree ? (row_seen >> q) & 1 : q <= row_t)))) z[j] = NEG_INF;
+          const bool held = (j < 2 ? there0 : there1) && p < end;
+          if (!held) vs[j] = 0.0f;                              // behind the last row in use anything may stand
+          if (!(held && (q < 0 || (a.tree ? (row_seen >> q) & 1 : q <= row_t)))) z[j] = NEG_INF;
         }
       }
       if (kf == 0.0f) {                                         // kappa: the power of two of the first scales
@@ -571,12 +614,11 @@ __global__ void __launch_bounds__(32 * Four<D>::WARPS, 1) kv_attention_four_kern
         for (int x = 1; x < 32; x <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, x));
         if (big > 0.0f) kf = pow2(127 - min(max(__float_as_int(big) >> 23, 1), 253));
       }
-      float lv[4], top = NEG_INF;
+      float top = NEG_INF;
 #pragma unroll
       for (int j = 0; j < 4; j++) {
         vs[j] *= kf;
-        lv[j] = fmaxf(log2_raw(vs[j]), -88.0f);
-        top = fmaxf(top, z[j] + lv[j]);
+        top = fmaxf(top, z[j] + fmaxf(log2_raw(vs[j]), -88.0f));
       }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
@@ -626,41 +668,116 @@ __global__ void __launch_bounds__(32 * Four<D>::WARPS, 1) kv_attention_four_kern
           imma_u8(acc[w * 4 + h * 2 + 1], p0, p1, p2, p3, __byte_perm(u0, u1, 0x7632), __byte_perm(u2, u3, 0x7632));
         }
     }
-    cp_wait<0>();
     move_sums(1.0f);
 
-    // ---- the warps' results of the piece
+    // ---- the piece: outputs (2 t4 + odd) * CH .. + CH - 1 of row r, relative to c_run; 2^-40 as the sums of p, before 2^kappa:
+    // huge values of V times weights of 2^31 would leave binary32
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
     l += __shfl_xor_sync(0xffffffffu, l, 4);
-    if (t4 == 0 && !odd) { join_c[warp][r] = c_run; join_l[warp][r] = l * 0x1p-40f; }
-    __syncthreads();                                            // every ring is drained
-    {
-      float top = join_c[0][r];
+    l *= 0x1p-40f;
+    const float kappa = kf == 0.0f ? 1.0f : pow2(127 - (__float_as_int(kf) >> 23));
+    float val[CH];
 #pragma unroll
-      for (int w = 1; w < WARPS; w++) top = fmaxf(top, join_c[w][r]);
-      // 2^-40, as the sums of p, before 2^kappa: huge values of V times weights of 2^31 would leave binary32
-      const float f = ex2(c_run - top) * 0x1p-40f;
-      const float kappa = kf == 0.0f ? 1.0f : pow2(127 - (__float_as_int(kf) >> 23));
-      float* dst = join_o + (warp * ROWS + r) * D + (2 * t4 + odd) * CH;
+    for (int i = 0; i < CH; i++) {
+      const float got = __shfl_xor_sync(0xffffffffu, odd ? o[i][0] : o[i][1], 4);
+      val[i] = ((odd ? o[i][1] : o[i][0]) + got) * 0x1p-40f * kappa;
+    }
+    const int mine = r * D + (2 * t4 + odd) * CH;               // this thread's place in a slot: [row][D], then c and l of the rows
+    bool last = true;
+    if (tile0 != 0 || tile1 != it.tiles) {
+      // other warps of the block that have pieces of the item
+      const int64_t in0 = max(at - tile0 - run.begin, (int64_t)0), in1 = min(at - tile0 + it.tiles, run.end) - 1 - run.begin;
+      const int warp0 = kv_run_of(parts, in0), warp1 = kv_run_of(parts, in1);
+      // a piece that begins in the middle of its item has a slot of its own; one that goes on behind the warp's run is the run's
+      // last, so the ring is free
+      auto slot_of = [&](int w) -> float* {
+        const bool starts = at - tile0 >= run.begin + kv_run_begin(parts, w);
+        return reinterpret_cast<float*>(smem + (starts ? w * (ST * C::TILE) : C::RING + w * C::SLOT));
+      };
+      if (warp0 != warp1) {
+        float* s = slot_of(warp);
+        if (tile0 == 0) { cp_wait<0>(); __syncwarp(); }
 #pragma unroll
-      for (int i = 0; i < CH; i += 4) {
-        float v[4];
+        for (int i = 0; i < CH; i += 4) *reinterpret_cast<float4*>(s + mine + i) = make_float4(val[i], val[i + 1], val[i + 2], val[i + 3]);
+        if (t4 == 0 && !odd) { s[ROWS * D + r] = c_run; s[ROWS * D + ROWS + r] = l; }
+        __threadfence_block();
+        __syncwarp();
+        int before = 0;
+        if (lane == 0) before = atomicAdd(arrived + warp0, 1);
+        last = __shfl_sync(0xffffffffu, before, 0) == warp1 - warp0;
+        if (last) {
+          __threadfence_block();
+          float top = C_NONE, sum = 0.0f;
+          for (int w = warp0; w <= warp1; w++) top = fmaxf(top, slot_of(w)[ROWS * D + r]);
 #pragma unroll
-        for (int c = 0; c < 4; c++) {
-          const float got = __shfl_xor_sync(0xffffffffu, odd ? o[i + c][0] : o[i + c][1], 4);
-          v[c] = ((odd ? o[i + c][1] : o[i + c][0]) + got) * f * kappa;
+          for (int i = 0; i < CH; i++) val[i] = 0.0f;
+          for (int w = warp0; w <= warp1; w++) {
+            const float* x = slot_of(w);
+            const float f = ex2(x[ROWS * D + r] - top);
+            sum = fmaf(x[ROWS * D + ROWS + r], f, sum);
+#pragma unroll
+            for (int i = 0; i < CH; i += 4) {
+              const float4 y = *reinterpret_cast<const float4*>(x + mine + i);
+              val[i] = fmaf(y.x, f, val[i]); val[i + 1] = fmaf(y.y, f, val[i + 1]); val[i + 2] = fmaf(y.z, f, val[i + 2]); val[i + 3] = fmaf(y.w, f, val[i + 3]);
+            }
+          }
+          c_run = top; l = sum;
         }
-        *reinterpret_cast<float4*>(dst + i) = make_float4(v[0], v[1], v[2], v[3]);
+      }
+      // the same between blocks, through memory
+      const bool starts = at - tile0 >= run.begin;
+      if (last && (!starts || at - tile0 + it.tiles > run.end)) {
+        const int run0 = kv_run_of(run.all, at - tile0), run1 = kv_run_of(run.all, at - tile0 + it.tiles - 1);
+        auto piece = [&](int c) { return a.slots + (int64_t)(2 * c + (c == run0 ? 1 : 0)) * KV_SLOT_FLOATS; };
+        float* s = piece((int)blockIdx.x);
+#pragma unroll
+        for (int i = 0; i < CH; i += 4) __stcg(reinterpret_cast<float4*>(s + mine + i), make_float4(val[i], val[i + 1], val[i + 2], val[i + 3]));
+        if (t4 == 0 && !odd) { __stcg(s + ROWS * D + r, c_run); __stcg(s + ROWS * D + ROWS + r, l); }
+        __threadfence();
+        __syncwarp();
+        uint32_t before = 0;
+        if (lane == 0) before = atomicAdd(a.counters + run0, 1u);
+        last = __shfl_sync(0xffffffffu, before, 0) == (uint32_t)(run1 - run0);
+        if (last) {
+          __threadfence();
+          if (lane == 0) a.counters[run0] = 0;
+          float top = C_NONE, sum = 0.0f;
+          for (int c = run0; c <= run1; c++) top = fmaxf(top, __ldcg(piece(c) + ROWS * D + r));
+#pragma unroll
+          for (int i = 0; i < CH; i++) val[i] = 0.0f;
+#pragma unroll 2
+          for (int c = run0; c <= run1; c++) {
+            const float* x = piece(c);
+            const float f = ex2(__ldcg(x + ROWS * D + r) - top);
+            sum = fmaf(__ldcg(x + ROWS * D + ROWS + r), f, sum);
+#pragma unroll
+            for (int i = 0; i < CH; i += 4) {
+              const float4 y = __ldcg(reinterpret_cast<const float4*>(x + mine + i));
+              val[i] = fmaf(y.x, f, val[i]); val[i + 1] = fmaf(y.y, f, val[i + 1]); val[i + 2] = fmaf(y.z, f, val[i + 2]); val[i + 3] = fmaf(y.w, f, val[i + 3]);
+            }
+          }
+          l = sum;
+        }
       }
     }
-    __syncthreads();
-    finish_piece<D, ROWS, WARPS>(a, run, b, rb, head, rows_here, tile0, tile1, tiles, at, join_c, join_l, join_o, &arrived);
-    __syncthreads();                                            // the rings are about to be filled again
+    if (last && r < rows_here) {
+      const float inv = l == 0.0f ? 0.0f : P_UNIT;
+      int t;
+      float* dst = a.out + row_offset(a, it.b, it.head, it.rb * ROWS + r, a.ld_o, D, t) + (2 * t4 + odd) * CH;
+#pragma unroll
+      for (int i = 0; i < CH; i += 4) {
+        const float d = l == 0.0f ? 1.0f : l;
+        *reinterpret_cast<float4*>(dst + i) = make_float4(val[i] / d * inv, val[i + 1] / d * inv, val[i + 2] / d * inv, val[i + 3] / d * inv);
+      }
+    }
     at += tile1 - tile0;
     left -= tile1 - tile0;
-    tile0 = 0;
-    if (++head == a.g.heads) { head = 0; e++; }
+    tile = 0;
+    if (left > 0 && ++it.head == a.g.heads) {
+      it.head = 0; it.e++;
+      it.load<ROWS>(a, row_blocks);
+    }
   }
 }
 
@@ -680,11 +797,11 @@ template <int D>
 int launch_four(b200q_ctx* ctx, const AttnArgs& a) {
   constexpr uint32_t ready = 1u << (D == 64 ? 12 : 13);
   if (!(ctx->kv_ready & ready)) {
-    B200Q_CHECK_CUDA(cudaFuncSetAttribute(kv_attention_four_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Four<D>::RING));
+    B200Q_CHECK_CUDA(cudaFuncSetAttribute(kv_attention_four_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Four<D>::SMEM));
     ctx->kv_ready |= ready;
   }
   const int row_blocks = (int)(((int64_t)a.T * a.group + 3) / 4);
-  return kv_launch(ctx, kv_attention_four_kernel<D>, dim3(ctx->sm_count), 32 * Four<D>::WARPS, Four<D>::RING, a, row_blocks);
+  return kv_launch(ctx, kv_attention_four_kernel<D>, dim3(ctx->sm_count), 32 * Four<D>::WARPS, Four<D>::SMEM, a, row_blocks);
 }
 
 }  // namespace
