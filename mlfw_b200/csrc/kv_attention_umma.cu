@@ -21,9 +21,9 @@ namespace {
 // overlap.  Bound by the instruction issue of the softmax and staging warps, with the products (1024 cycles per tile of
 // 128 rows at head dimension 128) close behind.
 //
-// With 64 or fewer rows (CS = 2) or 32 or fewer (CS = 4) the lanes hold CS copies of the rows, each copy takes 16 / CS of a
-// thread's tokens and has weights of zero elsewhere, and the copies are joined at the end: the softmax work, which
-// would leave lanes idle, shrinks with the rows.
+// With 64 or fewer rows (CS = 2) the lanes hold two copies of the rows, each copy takes half of a thread's tokens and has
+// weights of zero elsewhere, and the copies are joined at the end: the softmax work, which would leave lanes idle,
+// shrinks with the rows.
 //
 // Every wait is bounded: one that runs out raises the block's abort flag and STATUS_SDPA_WAIT_TIMEOUT, all roles leave,
 // products in flight get 2 ms, tensor memory is freed.  Threads meet at mbarriers only, never at a hardware barrier that
@@ -93,15 +93,6 @@ __device__ __forceinline__ void tm_ld2(uint32_t at0, uint32_t at1, uint32_t (&x)
       "tcgen05.wait::ld.sync.aligned;"
       : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]), "=r"(x[6]), "=r"(x[7]),
         "=r"(y[0]), "=r"(y[1]), "=r"(y[2]), "=r"(y[3]), "=r"(y[4]), "=r"(y[5]), "=r"(y[6]), "=r"(y[7])
-      : "r"(at0), "r"(at1) : "memory");
-}
-__device__ __forceinline__ void tm_ld2(uint32_t at0, uint32_t at1, uint32_t (&x)[4], uint32_t (&y)[4]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%8];\n\t"
-      "tcgen05.ld.sync.aligned.32x32b.x4.b32 {%4, %5, %6, %7}, [%9];\n\t"
-      "tcgen05.wait::ld.sync.aligned;"
-      : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]),
-        "=r"(y[0]), "=r"(y[1]), "=r"(y[2]), "=r"(y[3])
       : "r"(at0), "r"(at1) : "memory");
 }
 __device__ __forceinline__ void tm_ld(uint32_t at, uint32_t (&x)[32]) {
@@ -669,7 +660,7 @@ __global__ void __launch_bounds__(256) kv_attention_join_kernel(const AttnArgs a
 template <int D, int CS>
 int launch_many(b200q_ctx* ctx, const AttnArgs& a) {
   constexpr int ROWS = LANES / CS;
-  constexpr uint32_t ready = 1u << ((D == 64 ? 4 : 8) + CS / 2);   // CS = 1, 2, 4: bits 0, 1, 2 of four
+  constexpr uint32_t ready = 1u << ((D == 64 ? 2 : 4) + CS - 1);
   if (!(ctx->kv_ready & ready)) {
     B200Q_CHECK_CUDA(cudaFuncSetAttribute(kv_attention_many_kernel<D, CS>, cudaFuncAttributeMaxDynamicSharedMemorySize, Many<D>::SMEM));
     ctx->kv_ready |= ready;
@@ -686,8 +677,8 @@ int launch_many(b200q_ctx* ctx, const AttnArgs& a) {
 
 int launch_kv_attention_many(b200q_ctx* ctx, const AttnArgs& a, int D) {
   const int64_t rows = (int64_t)a.T * a.group;
-  if (D == 64) return rows <= 32 ? launch_many<64, 4>(ctx, a) : rows <= 64 ? launch_many<64, 2>(ctx, a) : launch_many<64, 1>(ctx, a);
-  return rows <= 32 ? launch_many<128, 4>(ctx, a) : rows <= 64 ? launch_many<128, 2>(ctx, a) : launch_many<128, 1>(ctx, a);
+  if (D == 64) return rows <= 64 ? launch_many<64, 2>(ctx, a) : launch_many<64, 1>(ctx, a);
+  return rows <= 64 ? launch_many<128, 2>(ctx, a) : launch_many<128, 1>(ctx, a);
 }
 
 }  // namespace b200q

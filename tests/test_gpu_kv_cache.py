@@ -341,6 +341,21 @@ def test_attention_is_the_same_every_time(ctx):
             assert (run_attention(S, q, np.full(B, n), None, None, 0.1).view(np.uint32) == first.view(np.uint32)).all()
 
 
+@pytest.mark.parametrize("B,T,H,heads,dim,most", [(40, 1, 16, 16, 64, 420), (24, 1, 32, 8, 128, 900), (20, 3, 12, 4, 64, 700), (12, 9, 8, 8, 64, 900),
+                                                  (6, 24, 16, 16, 64, 1500), (3, 40, 12, 12, 128, 1300), (3, 70, 24, 8, 128, 1100)])
+def test_attention_long_runs(ctx, B, T, H, heads, dim, most):
+    """Enough work that a block has many tiles of several items, of uneven lengths."""
+    S = Setup(ctx, B, most + T, 64, heads, dim)
+    start = S.rng.integers(0, most, B)
+    start[0] = most
+    for i in range(2):
+        S.codes[i] = np.clip(np.round(S.rng.standard_normal(S.codes[i].shape) * 42), -127, 127).astype(np.int8)
+        S.scales[i] = S.rng.uniform(0.01, 0.03, S.scales[i].shape).astype(np.float32)
+    S.upload()
+    q = (S.rng.standard_normal((B, T, H, dim)) * 2).astype(np.float32)
+    check_attention(S, q, start, np.full(B, T), random_tree(S.rng, B, T) if T > 1 and T <= 64 else None, dim ** -0.5)
+
+
 def test_positions_outside_the_cache(ctx):
     """A bad page or a position behind the table: the status bit, no write, zeros, not visible."""
     S = Setup(ctx, 2, 48, 16, 2, 64)
