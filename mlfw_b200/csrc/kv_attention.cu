@@ -126,47 +126,84 @@ __global__ void __launch_bounds__(32 * Four<D>::WARPS, 1) kv_attention_four_kern
     }
   }
 
-  // ---- the ring: tiles in the order of the run, ST - 1 ahead of their use.  `ahead` walks by itself; page0 and page1 are the
-  // pages of its next tile's two runs of sixteen tokens, -1 where nothing is visible.
-  Item ahead = it;
-  int ahead_tile = tile, ahead_left = left, page0, page1;
+  // ---- the ring: tiles in the order of the run, ST - 1 ahead of their use.  `ahead` walks by itself.  A tile of 32 tokens lies in
+  // one page (pages of 32 tokens or more: one address for all of it, looked up when a page begins) or in two of 16; its
+  // pages are looked up a tile early.  -1: nothing there is visible.  Positions fit 32 bits: start is below 2^31, T at most 2^24.
+  const int shift = a.g.page_shift;
+  const bool wide = shift >= 5;
+  const uint32_t in_page = (1u << shift) - 1, page_cells = (uint32_t)a.g.heads << shift;   // < 2^24
+  int ahead_e = it.e, ahead_head = it.head, ahead_tiles = it.tiles, ahead_tile = tile, ahead_left = left, page0 = -1, page1 = -1;
+  uint32_t ahead_vis = (uint32_t)it.vis, ahead_cell = (uint32_t)it.head << shift;   // first cell of the head in a page
+  const int32_t* ahead_table = a.page_table + (int64_t)it.b * a.g.max_pages;
+  const int8_t *k_lane = a.k + lane * 16, *v_lane = a.v + lane * 16;
+  const float* s_lane = (lane < 8 ? a.ks : a.vs) + (lane & 7) * 4;                          // lanes 0 .. 15: scales of K, of V
+  const uint32_t s_dst = ring + 2 * KV_TILE * D + ((lane >> 2) & 1) * C::GRAN + ((lane >> 3) & 1) * 64 + (lane & 3) * 16;
   uint32_t there = 0;                                           // two bits per tile in the ring, the oldest lowest
-  auto pages = [&]() {
-    const int64_t pos = (int64_t)ahead_tile * IT;
-    const int32_t* table = a.page_table + (int64_t)ahead.b * a.g.max_pages;
-    page0 = ahead_left > 0 && pos < ahead.vis ? __ldg(table + (pos >> a.g.page_shift)) : -1;
-    page1 = ahead_left > 0 && pos + 16 < ahead.vis ? __ldg(table + ((pos + 16) >> a.g.page_shift)) : -1;
+  auto look_up = [&](bool anew) {                               // the pages of the tile `ahead`
+    const uint32_t pos = (uint32_t)ahead_tile * IT;
+    if (wide) {
+      if (anew || (pos & in_page) == 0) page0 = pos < ahead_vis ? __ldg(ahead_table + (pos >> shift)) : -1;
+    } else {
+      page0 = pos < ahead_vis ? __ldg(ahead_table + (pos >> 4)) : -1;
+      page1 = pos + 16 < ahead_vis ? __ldg(ahead_table + (pos >> 4) + 1) : -1;
+    }
   };
   auto fetch = [&](int s, int place) {
     if (ahead_left > 0) {
+      const uint32_t pos = (uint32_t)ahead_tile * IT, to = s * C::TILE;
+      if (wide) {
+        if ((uint32_t)page0 < (uint32_t)a.g.pages) {
+          const uint64_t cell = (uint64_t)(uint32_t)page0 * page_cells + (ahead_cell + (pos & in_page));
+          const int8_t *kp = k_lane + cell * D, *vp = v_lane + cell * D;
 #pragma unroll
-      for (int h = 0; h < 2; h++) {
-        const int page = h ? page1 : page0;
-        if ((uint32_t)page < (uint32_t)a.g.pages) {
-          const int64_t row = (((int64_t)page * a.g.heads + ahead.head) << a.g.page_shift) + ((ahead_tile * IT + h * 16) & ((1 << a.g.page_shift) - 1));
-          const uint32_t to = s * C::TILE + h * C::GRAN;
-          const int8_t *kp = a.k + row * D + lane * 16, *vp = a.v + row * D + lane * 16;
+          for (int h = 0; h < 2; h++)
 #pragma unroll
-          for (int x = 0; x < D / 32; x++) cp16(k_dst + to + x * 512, kp + x * 512);
+            for (int x = 0; x < D / 32; x++) {
+              cp16(k_dst + to + h * C::GRAN + x * 512, kp + h * 16 * D + x * 512);
+              cp16(((D == 128 && (x & 1)) ? v_dst ^ 64u : v_dst) + to + h * C::GRAN + x * 512, vp + h * 16 * D + x * 512);
+            }
+          if (lane < 16) cp16(s_dst + to, s_lane + cell);
+          there |= 3u << (2 * place);
+        }
+      } else {
 #pragma unroll
-          for (int x = 0; x < D / 32; x++) cp16(((D == 128 && (x & 1)) ? v_dst ^ 64u : v_dst) + to + x * 512, vp + x * 512);
-          if (lane < 8) cp16(ring + 2 * KV_TILE * D + lane * 16 + to, (lane < 4 ? a.ks : a.vs) + row + (lane & 3) * 4);
-          there |= (1u + h) << (2 * place);
+        for (int h = 0; h < 2; h++) {
+          const int page = h ? page1 : page0;
+          if ((uint32_t)page < (uint32_t)a.g.pages) {
+            const uint64_t cell = (uint64_t)(uint32_t)page * page_cells + ahead_cell;
+            const int8_t *kp = k_lane + cell * D, *vp = v_lane + cell * D;
+#pragma unroll
+            for (int x = 0; x < D / 32; x++) {
+              cp16(k_dst + to + h * C::GRAN + x * 512, kp + x * 512);
+              cp16(((D == 128 && (x & 1)) ? v_dst ^ 64u : v_dst) + to + h * C::GRAN + x * 512, vp + x * 512);
+            }
+            if (lane < 16 && (lane & 4) == 0) cp16(s_dst + to + h * C::GRAN, s_lane + cell);
+            there |= (1u + h) << (2 * place);
+          }
         }
       }
       ahead_left--;
-      if (++ahead_tile == ahead.tiles) {
+      bool anew = false;
+      if (++ahead_tile == ahead_tiles) {
         ahead_tile = 0;
-        if (++ahead.head == a.g.heads) {
-          ahead.head = 0; ahead.e++;
-          if (ahead_left > 0) ahead.load<ROWS>(a, row_blocks);
+        anew = true;
+        ahead_cell += 1u << shift;
+        if (++ahead_head == a.g.heads) {
+          ahead_head = 0; ahead_cell = 0; ahead_e++;
+          if (ahead_left > 0) {
+            Item next;
+            next.e = ahead_e;
+            next.load<ROWS>(a, row_blocks);
+            ahead_e = next.e; ahead_tiles = next.tiles; ahead_vis = (uint32_t)next.vis;
+            ahead_table = a.page_table + (int64_t)next.b * a.g.max_pages;
+          }
         }
       }
-      pages();
+      if (ahead_left > 0) look_up(anew);
     }
     cp_commit();
   };
-  pages();
+  look_up(true);
 #pragma unroll
   for (int s = 0; s < ST - 1; s++) fetch(s, s);
 
@@ -289,7 +326,7 @@ __global__ void __launch_bounds__(32 * Four<D>::WARPS, 1) kv_attention_four_kern
       const bool grow = top > c_run + C_SLACK;
       if (__any_sync(0xffffffffu, grow) || since == 1024) {
         const float c_new = grow ? top - C_BELOW : c_run, f = ex2(c_run - c_new);
-        move_sums(f);
+        if (since != 0) move_sums(f);
         l *= f;
         c_run = c_new;
       }
