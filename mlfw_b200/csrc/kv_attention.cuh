@@ -121,7 +121,7 @@ struct Run {
 // ROWS query rows per item, TILE tokens per tile, at least LEAST tiles per run (a shorter one costs more in joining than it saves).
 template <int ROWS, int TILE, int LEAST>
 __device__ __forceinline__ Run find_run(const AttnArgs& a, int row_blocks) {
-  __shared__ int64_t warp_sum[33];
+  __shared__ int64_t warp_sum[32];
   __shared__ int found[3];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int E = a.B * row_blocks, per = (E + blockDim.x - 1) / blockDim.x;
@@ -140,20 +140,21 @@ __device__ __forceinline__ Run find_run(const AttnArgs& a, int row_blocks) {
   }
   if (lane == 31) warp_sum[warp] = incl;
   __syncthreads();
-  if (tid == 0) {
-    int64_t s = 0;
-    for (int w = 0; w < (int)blockDim.x / 32; w++) { const int64_t x = warp_sum[w]; warp_sum[w] = s; s += x; }
-    warp_sum[32] = s;
+  int64_t before = 0, total = 0;                                // of the warps before this one, and of all
+#pragma unroll 4
+  for (int w = 0; w < (int)blockDim.x / 32; w++) {
+    const int64_t x = warp_sum[w];
+    if (w < warp) before += x;
+    total += x;
   }
-  __syncthreads();
   Run r;
   r.begin = r.end = 0;
-  if (warp_sum[32] == 0) return r;
-  r.all = kv_runs(warp_sum[32], LEAST, (int)gridDim.x);
+  if (total == 0) return r;
+  r.all = kv_runs(total, LEAST, (int)gridDim.x);
   if ((int)blockIdx.x >= r.all.runs) return r;
   r.begin = kv_run_begin(r.all, (int)blockIdx.x);
   r.end = kv_run_begin(r.all, (int)blockIdx.x + 1);
-  int64_t at = warp_sum[warp] + incl - mine;
+  int64_t at = before + incl - mine;
   if (r.begin >= at && r.begin < at + mine) {
     int e = e0;
     int64_t n = tiles(e);
