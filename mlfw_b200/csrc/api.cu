@@ -26,8 +26,15 @@ void set_error(const char* fmt, ...) {
 int ws_reserve(b200q_ctx* ctx, Workspace& ws, size_t bytes) {
   if (bytes <= ws.bytes) return 0;
   B200Q_REQUIRE(!ctx->capturing, "a workspace would have to grow while calls are being recorded: run the same calls once before b200q_graph_begin");
-  // Stream-ordered, so a buffer still read by queued kernels is released after them.
-  if (ws.ptr) B200Q_CHECK_CUDA(cudaFreeAsync(ws.ptr, ctx->stream));
+  if (ws.ptr && ctx->graphs > 0) {
+    // a recording holds the old address and may be replayed after this
+    Retired* r = new (std::nothrow) Retired{ws.ptr, ctx->retired};
+    B200Q_REQUIRE(r != nullptr, "out of host memory");
+    ctx->retired = r;
+  } else if (ws.ptr) {
+    // Stream-ordered, so a buffer still read by queued kernels is released after them.
+    B200Q_CHECK_CUDA(cudaFreeAsync(ws.ptr, ctx->stream));
+  }
   ws.ptr = nullptr;
   ws.bytes = 0;
   size_t want = bytes + bytes / 8;
@@ -47,6 +54,15 @@ int prof_fold(b200q_ctx* ctx) {
   }
   ctx->prof_used = 0;
   return 0;
+}
+
+static void free_retired(b200q_ctx* ctx) {   // nothing queued uses the memory any more
+  while (ctx->retired) {
+    Retired* r = ctx->retired;
+    ctx->retired = r->next;
+    cudaFree(r->ptr);
+    delete r;
+  }
 }
 
 static int use_device(b200q_ctx* ctx) {
@@ -182,6 +198,7 @@ void b200q_destroy(b200q_ctx* ctx) {
   Workspace* all[] = {&ctx->ws_q, &ctx->ws_scales, &ctx->ws_acc, &ctx->ws_stage_in, &ctx->ws_stage_out, &ctx->ws_range, &ctx->ws_kv};
   for (Workspace* w : all)
     if (w->ptr) cudaFree(w->ptr);
+  free_retired(ctx);
   if (ctx->status_dev) cudaFree(ctx->status_dev);
   for (int i = 0; i < PROFILE_RING; i++)
     for (int j = 0; j < 2; j++)
@@ -899,6 +916,7 @@ int b200q_graph_end(b200q_ctx* ctx, b200q_graph** out) {
   g->graph = graph;
   g->exec = exec;
   g->kernels = kernels;
+  ctx->graphs++;
   *out = g;
   return 0;
 }
@@ -919,6 +937,7 @@ int b200q_graph_destroy(b200q_ctx* ctx, b200q_graph* graph) {
   if (graph->exec) cudaGraphExecDestroy(graph->exec);
   if (graph->graph) cudaGraphDestroy(graph->graph);
   delete graph;
+  if (ctx->graphs > 0 && --ctx->graphs == 0) free_retired(ctx);
   return 0;
 }
 

@@ -56,6 +56,12 @@ struct Workspace {
   size_t bytes = 0;
 };
 
+// A workspace that grew while recordings of the context exist: they go on using its old memory.
+struct Retired {
+  void* ptr;
+  Retired* next;
+};
+
 }  // namespace b200q
 
 // The context behind the opaque handle of the C ABI: one per GPU, not thread safe.
@@ -101,6 +107,8 @@ struct b200q_ctx {
   uint64_t launches = 0;                 // kernels launched through this context
   bool capturing = false;                // between b200q_graph_begin and _end: calls are recorded, nothing may allocate or synchronise
   uint64_t capture_launches0 = 0;        // `launches` when the capture began
+  int graphs = 0;                        // recordings that exist
+  b200q::Retired* retired = nullptr;     // memory they may use, until the last of them is destroyed
   // per-kernel CUDA-event timing (off by default): a ring of event pairs, folded into the sums when it wraps or is read
   bool profiling = false;
   cudaEvent_t prof_ev[b200q::PROFILE_RING][2] = {};

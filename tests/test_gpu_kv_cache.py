@@ -607,3 +607,41 @@ def test_block_with_a_cache(ctx):
         assert (again.download().view(np.uint32) == out.download().view(np.uint32)).all()
         length += T if T != 8 else 0                 # the drafted rows are all refused
     cache.close()
+
+
+def test_recorded_block_step_survives_larger_prompts(ctx):
+    """A recorded decoding step of a block, replayed after prompts that made every workspace of the context grow."""
+    import mlfw_b200
+    from mlfw_b200.block import GPTBlock, random_block_params
+    with mlfw_b200.Context(0) as c:
+        D, H, FF, B = 128, 2, 512, 2
+        blk = GPTBlock(c, D, H, FF, random_block_params(D, FF, seed=6, std=0.3))
+        cache = mlfw_b200.KVCache(c, 2 * 8, 64, H, 64)
+        table = c.to_device(np.arange(16, dtype=np.int32).reshape(B, 8))
+        rng = np.random.default_rng(9)
+        step, out, length = c.to_device(rng.standard_normal((B, D)).astype(np.float32)), c.empty((B, D), np.float32), c.to_device(np.array([3, 5], np.int32))
+        first = c.to_device(np.zeros(B, np.int32))
+        prompt = rng.standard_normal((B * 8, D)).astype(np.float32)
+
+        def run(T, h, where, o):
+            blk.forward_cached(h, B, T, cache, table, 8, where, o)
+
+        run(8, c.to_device(prompt), first, c.empty((B * 8, D), np.float32))
+        run(1, step, length, out)
+        c.sync()
+        want = out.download()
+        c.graph_begin()
+        run(1, step, length, out)
+        graph = c.graph_end()
+        big = c.to_device(rng.standard_normal((B * 400, D)).astype(np.float32))
+        run(400, big, first, c.empty((B * 400, D), np.float32))          # the workspaces grow
+        run(8, c.to_device(prompt), first, c.empty((B * 8, D), np.float32))
+        for _ in range(3):
+            out.fill_bytes(0)
+            c.graph_launch(graph)
+            run(400, big, c.to_device(np.array([100, 100], np.int32)), c.empty((B * 400, D), np.float32))
+            c.sync()
+            assert (out.download().view(np.uint32) == want.view(np.uint32)).all()
+        c.graph_destroy(graph)
+        c.check_status()
+        cache.close()
