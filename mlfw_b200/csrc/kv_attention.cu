@@ -31,14 +31,18 @@ __device__ __forceinline__ uint32_t v_at(int t, int c) {
 // they are converted, scaled and moved to binary32.  c = top - 26 leaves 5.5 bits before a larger weight (below 2^32) moves it.
 // Scales of V are taken relative to the power of two of the first tile's largest (kappa), so that tiny values keep their digits.
 //
-// About 650 instructions per warp and 32 tokens of 128 dimensions (conversion of the codes to binary16 for m16n8k16, tried
-// first, took 1300).  Bound by the latency of those instructions with reading the cache close behind: at four rows 4.75 TB/s
-// of the 6.5 measured (48 sequences of up to 6000 tokens, 32 heads on 8, 128 wide: 86.6 us).  Twelve warps (D = 128: 64 integer sums, 32 outputs per thread) or sixteen (D = 64), one block per SM.
+// About 550 instructions per warp and 32 tokens of 128 dimensions, 500 of 64 (conversion of the codes to binary16 for
+// m16n8k16, tried first, took 1300).  Bound by reading the cache: 5.4 TB/s of the 6.5 measured at 48 sequences of up to 6000
+// tokens, 32 heads on 8, 128 wide (75 us; 412 MB), launch, search of the runs and joining included.  One block per SM, eight
+// warps (D = 128: 64 integer sums and 32 outputs per thread, which need more than the 168 registers that twelve warps leave)
+// with two tiles each in flight, or twelve (D = 64) with three.  Same case with 12 x 2: 85 us, 10 x 2: 83, 8 x 3: 77,
+// 6 x 3: 76, 4 x 4: 86; 64 wide, 64 sequences of up to 2000 tokens, 12 heads, 12 x 3: 34.9 us, 16 x 3: 38.9, 8 x 4: 37.1,
+// 12 x 2: 35.1.
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int IT = 32;                                          // tokens of a tile: two runs of sixteen, each in one page
 template <int D>
 struct Four {
-  static constexpr int WARPS = D == 128 ? 12 : 16, STAGES = D == 128 ? 2 : 3;
+  static constexpr int WARPS = D == 128 ? 8 : 12, STAGES = D == 128 ? 2 : 3;
   static constexpr int GRAN = 2 * KV_TILE * D + 2 * KV_TILE * 4, TILE = 2 * GRAN;   // sixteen tokens: K and V codes, K and V scales
   static constexpr int RING = WARPS * STAGES * TILE, SLOT = 4 * (D + 2) * 4, SMEM = RING + WARPS * SLOT;
 };
@@ -100,7 +104,9 @@ __global__ void __launch_bounds__(32 * Four<D>::WARPS, 1) kv_attention_four_kern
 
   kv_after_previous();
   if (tid < WARPS) arrived[tid] = 0;
-  const Run run = find_run<ROWS, IT, WARPS>(a, row_blocks);     // (its barriers publish `arrived`)
+  // At least 8 tiles per run, or whole items: one sequence of 500 tokens, 12 heads of 64, 8.5 us (runs of 8 tiles 9.5), 2000 tokens
+  // 11.5 (whole items 12.6); 4 sequences of 1000 tokens, 32 heads on 8 of 128, 12.0 (12.3).
+  const Run run = find_run<ROWS, IT, 8, true>(a, row_blocks);   // (its barriers publish `arrived`)
   if (run.begin == run.end) return;
   const KvRuns parts = kv_runs(run.end - run.begin, 1, WARPS);
   if (warp >= parts.runs) return;

@@ -118,8 +118,10 @@ struct Run {
   int64_t begin, end;
   int e, head, tile;
 };
-// ROWS query rows per item, TILE tokens per tile, at least LEAST tiles per run (a shorter one costs more in joining than it saves).
-template <int ROWS, int TILE, int LEAST>
+// ROWS query rows per item, TILE tokens per tile, at least LEAST tiles per run: a shorter one costs more in joining than it saves.
+// WHOLE: where an item has at most 32 tiles on average, that many (4 or more), so that with little work items of one length fall
+// into one run each and nothing is joined between blocks.
+template <int ROWS, int TILE, int LEAST, bool WHOLE>
 __device__ __forceinline__ Run find_run(const AttnArgs& a, int row_blocks) {
   __shared__ int64_t warp_sum[32];
   __shared__ int found[3];
@@ -150,7 +152,9 @@ __device__ __forceinline__ Run find_run(const AttnArgs& a, int row_blocks) {
   Run r;
   r.begin = r.end = 0;
   if (total == 0) return r;
-  r.all = kv_runs(total, LEAST, (int)gridDim.x);
+  const int64_t mean = WHOLE ? kv_div(total, (int64_t)E * a.g.heads) : 0;
+  const int least = WHOLE && mean <= 32 ? max((int)mean, 4) : LEAST;
+  r.all = kv_runs(total, least, (int)gridDim.x);
   if ((int)blockIdx.x >= r.all.runs) return r;
   r.begin = kv_run_begin(r.all, (int)blockIdx.x);
   r.end = kv_run_begin(r.all, (int)blockIdx.x + 1);

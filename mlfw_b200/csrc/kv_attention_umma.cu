@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv_attention_many_kernel(cons
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   asm volatile("griddepcontrol.wait;" ::: "memory");             // the previous kernel of the stream wrote what is read here
-  const Run run = find_run<ROWS, MT, 2>(a, mp.row_blocks);
+  const Run run = find_run<ROWS, MT, 2, false>(a, mp.row_blocks);
   if (tid == 0) a.items[blockIdx.x] = make_int4(0, 0, 0, 0);
   if (run.begin == run.end) return;
 
