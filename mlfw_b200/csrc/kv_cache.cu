@@ -84,7 +84,7 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const KvArgs a, const fl
   constexpr int V4 = D / 32;
   kv_after_previous();
   const int lane = threadIdx.x & 31, sub = lane & 7;
-  const uint32_t u = (blockIdx.x * blockDim.x + threadIdx.x) >> 5;
+  const uint32_t u = kv_warp(blockIdx.x, blockDim.x, threadIdx.x);
   if (u >= units) return;
   const uint32_t token = u / chunks, head = (u - token * chunks) * 4 + (lane >> 3);
   const uint32_t b = token / (uint32_t)a.T, t = token - b * (uint32_t)a.T;
@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const KvArgs a, float* __r
   constexpr int V4 = D / 32;
   kv_after_previous();
   const int lane = threadIdx.x & 31, sub = lane & 7;
-  const uint32_t u = (blockIdx.x * blockDim.x + threadIdx.x) >> 5;
+  const uint32_t u = kv_warp(blockIdx.x, blockDim.x, threadIdx.x);
   if (u >= units) return;
   const uint32_t token = u / chunks, head = (u - token * chunks) * 4 + (lane >> 3);
   const uint32_t b = token / (uint32_t)a.T, t = token - b * (uint32_t)a.T;

@@ -45,6 +45,9 @@ B200Q_HD int kv_rows_in_use(const int32_t* count, int64_t b, int T) {
   return c < 0 ? 0 : (c > T ? T : c);
 }
 
+// The warp a thread belongs to, counted over a grid of blocks of whole warps: up to 2^31 - 1, where threads no longer fit 32 bits.
+B200Q_HD uint32_t kv_warp(uint32_t block, uint32_t threads, uint32_t thread) { return block * (threads / 32) + thread / 32; }
+
 // ---------------------------------------------------------------------------------------------- work of the attention
 // An item is one block of `rows` query rows (row R = t * group + query head within the group) of one sequence and one cache head; its
 // work is the 16-token tiles of the positions any of its rows sees.  All items' tiles, in the order (sequence, row block,

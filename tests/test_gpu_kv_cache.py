@@ -452,6 +452,32 @@ def test_offsets_past_31_bits(ctx, orc):
     cache.close()
 
 
+def test_padded_batch_of_many_rows(ctx, orc):
+    """Nine sequences of room for 2^24 rows, of which the last has three in use: more threads than 32 bits count, operands of
+    36 GB of which nothing else is touched."""
+    S = Setup(ctx, 9, 32, 16, 1, 64)
+    T, n = 1 << 24, 3
+    x = ctx.empty((9 * T, 64), np.float32)
+    at = x.ptr + 8 * T * 64 * 4
+    k = S.rng.standard_normal((n, 64)).astype(np.float32)
+    ctx.lib.b200q_upload(ctx.handle, at, k.ctypes.data, k.nbytes)
+    count = [0] * 8 + [n]
+    S.cache.append(x, x, 64, 64, 9, T, S.dtable, S.per, S.dev([14] * 9), S.dev(count))
+    for t in range(n):
+        q, _, s = orc.quantize_per_token(k[t][None])
+        p, r = S.table[8, (14 + t) // 16], (14 + t) % 16
+        for i in range(2):
+            S.codes[i][p, 0, r], S.scales[i][p, 0, r] = q[0], s[0]
+    S.check()
+    S.cache.read(9, T, S.dtable, S.per, S.dev([14] * 9), S.dev(count), x, x, 64, 64)   # K and V are alike, so one operand takes both
+    got = np.empty_like(k)
+    ctx.lib.b200q_download(ctx.handle, got.ctypes.data, at, got.nbytes)
+    c, _, s = orc.quantize_per_token(k)
+    want = c.astype(np.float32) * np.reshape(s, (-1, 1))
+    assert (got.view(np.uint32) == want.view(np.uint32)).all()
+    x.free()
+
+
 def test_refusals(ctx):
     import mlfw_b200
     S = Setup(ctx, 1, 32, 16, 2, 64)

@@ -66,6 +66,7 @@ int walk(int B, int T, int heads, int group, int rows, int warps, int grid, int6
     if (pieces[i] != expected[i]) return 7;
   return 0;
 }
+uint32_t warp(uint32_t block, uint32_t threads, uint32_t thread) { return kv_warp(block, threads, thread); }
 const char* rows(const void* base, int64_t ld, int64_t h, int64_t d) { return kv_refuse_rows(base, ld, h, d); }
 }
 """
@@ -81,6 +82,7 @@ def host(tmp_path_factory):
     lib = C.CDLL(so)
     i64, vp = C.c_int64, C.c_void_p
     lib.row.restype, lib.row.argtypes = i64, [i64, i64, C.c_int, C.c_int, vp, i64, C.c_int, i64]
+    lib.warp.restype, lib.warp.argtypes = C.c_uint32, [C.c_uint32] * 3
     lib.in_use.argtypes = [vp, i64, C.c_int]
     lib.walk.argtypes = [C.c_int] * 7 + [i64, C.c_int, vp, vp, C.c_int, C.c_int, C.POINTER(i64)]
     lib.visible.restype, lib.visible.argtypes = i64, [i64, C.c_int, i64] + [C.c_int] * 5
@@ -153,6 +155,12 @@ def test_visible_positions(host):
         assert host.tiles(64, 4, start, n, group, rows, past, tree, 16) == 0
     assert host.visible(2, 4, 100, 3, 1, 8, 0, False) == 32 and host.visible(2, 4, -100, 3, 1, 8, 0, False) == 0
     assert host.tiles(2, 4, -100, 3, 1, 8, 0, False, 16) == 1 and host.tiles(0, 4, 0, 3, 1, 8, 0, True, 16) == 1
+
+
+def test_warps_of_a_large_grid(host):
+    """A batch of nearly 2^31 rows has as many warps: more threads than 32 bits count."""
+    for block, thread in ((0, 0), (3, 255), (1 << 24, 0), ((1 << 28) - 1, 255)):
+        assert host.warp(block, 256, thread) == (block * 256 + thread) // 32
 
 
 def test_refusals(host):
