@@ -331,15 +331,16 @@ int b200q_sdpa_f32(b200q_ctx* ctx, const float* q, const float* k, const float* 
  * f32 [pages][heads][page_tokens], for K and for V.  Their contents need no initialisation: what no call has written is
  * never visible.  The handle holds geometry and addresses only; it must not outlive its context or the buffers.
  *
- * Every call works on a batch of B sequences with T new rows each.  DEVICE arrays say which: page_table int32 [B, max_pages]
- * (position p of sequence b is token p mod page_tokens of page page_table[b][p / page_tokens]; max_pages is the table's
- * row length), start int32 [B] (positions held before the call: row t of the call is position start[b] + t) and count
- * int32 [B] (rows in use, held to 0..T; null: T).  f32 operands: row (b, t) of head h starts at
- * base + (b * T + t) * ld + h * head_dim, on a 16-byte boundary (ld a multiple of 4).  Rows t >= count[b] of outputs are
- * left as they were.  A position outside the table, or on a page outside the cache, sets status bit 5 and is not
- * written (append, keep), reads as zeros (read) or is not visible (attention).  Pages may be shared between sequences
- * for reading; a position that two sequences of one call write is undefined.  All four calls are stream-ordered, need no
- * workspace that grows, and may be recorded (b200q_graph_begin): lengths and pages are read when the recording runs. */
+ * Every call works on a batch of B sequences with T new rows each.  DEVICE arrays, each at a multiple of its element's
+ * size, say which: page_table int32 [B, max_pages] (position p of sequence b is token p mod page_tokens of page
+ * page_table[b][p / page_tokens]; max_pages is the table's row length), start int32 [B] (positions held before the call:
+ * row t of the call is position start[b] + t) and count int32 [B] (rows in use, held to 0..T; null: T).  f32 operands: row
+ * (b, t) of head h starts at base + (b * T + t) * ld + h * head_dim, on a 16-byte boundary (ld a multiple of 4).  Rows t >=
+ * count[b] of outputs are left as they were.  A position outside the table, or on a page outside the cache, sets status bit
+ * 5 and is not written (append, keep), reads as zeros (read) or is not visible (attention).  Pages may be shared between
+ * sequences for reading; a position that two sequences of one call write is undefined.  All four calls are stream-ordered,
+ * need no workspace that grows, and may be recorded (b200q_graph_begin): lengths and pages are read when the recording
+ * runs. */
 typedef struct b200q_kv_cache b200q_kv_cache;
 int b200q_kv_create(b200q_ctx* ctx, int64_t pages, int64_t page_tokens, int64_t heads, int64_t head_dim, int8_t* k_codes,
                     int8_t* v_codes, float* k_scales, float* v_scales, b200q_kv_cache** out);

@@ -266,6 +266,7 @@ int b200q_kv_append(b200q_ctx* ctx, b200q_kv_cache* cache, const float* k, const
   if (int e = kv_enter("b200q_kv_append", ctx, cache)) return e;
   KV_ORDERLY("b200q_kv_append", kv_refuse_batch(B, T, cache->heads, page_table, max_pages, start));
   if (B * T == 0) return 0;
+  KV_ORDERLY("b200q_kv_append", kv_refuse_array(count, 4));
   KV_ORDERLY("b200q_kv_append", kv_refuse_rows(k, ld_k, cache->heads, cache->head_dim));
   KV_ORDERLY("b200q_kv_append", kv_refuse_rows(v, ld_v, cache->heads, cache->head_dim));
   return launch_kv_append(ctx, *cache, KvBatch{(int)B, (int)T, page_table, max_pages, start, count}, k, v, ld_k, ld_v);
@@ -276,6 +277,7 @@ int b200q_kv_read(b200q_ctx* ctx, b200q_kv_cache* cache, int64_t B, int64_t T, c
   if (int e = kv_enter("b200q_kv_read", ctx, cache)) return e;
   KV_ORDERLY("b200q_kv_read", kv_refuse_batch(B, T, cache->heads, page_table, max_pages, start));
   if (B * T == 0) return 0;
+  KV_ORDERLY("b200q_kv_read", kv_refuse_array(count, 4));
   KV_ORDERLY("b200q_kv_read", kv_refuse_rows(k_out, ld_k, cache->heads, cache->head_dim));
   KV_ORDERLY("b200q_kv_read", kv_refuse_rows(v_out, ld_v, cache->heads, cache->head_dim));
   return launch_kv_read(ctx, *cache, KvBatch{(int)B, (int)T, page_table, max_pages, start, count}, k_out, v_out, ld_k, ld_v);
@@ -291,6 +293,8 @@ int b200q_kv_attention(b200q_ctx* ctx, b200q_kv_cache* cache, const float* q, in
   B200Q_REQUIRE(tree == nullptr || T <= KV_MAX_TREE, "b200q_kv_attention: a tree has at most %d drafted tokens (got %lld)", KV_MAX_TREE, (long long)T);
   B200Q_REQUIRE(std::isfinite(scale), "b200q_kv_attention: the scale must be finite");
   if (B * T == 0) return 0;
+  KV_ORDERLY("b200q_kv_attention", kv_refuse_array(count, 4));
+  KV_ORDERLY("b200q_kv_attention", kv_refuse_array(tree, 8));
   KV_ORDERLY("b200q_kv_attention", kv_refuse_rows(q, ld_q, H, cache->head_dim));
   KV_ORDERLY("b200q_kv_attention", kv_refuse_rows(out, ld_out, H, cache->head_dim));
   return launch_kv_attention(ctx, *cache, KvBatch{(int)B, (int)T, page_table, max_pages, start, count}, q, ld_q, (int)H, tree, scale, out, ld_out);
@@ -302,7 +306,9 @@ int b200q_kv_keep(b200q_ctx* ctx, b200q_kv_cache* cache, int64_t B, int64_t T, c
   KV_ORDERLY("b200q_kv_keep", kv_refuse_batch(B, T, cache->heads, page_table, max_pages, start));
   B200Q_REQUIRE(T <= KV_MAX_TREE, "b200q_kv_keep: at most %d rows per sequence (got %lld)", KV_MAX_TREE, (long long)T);
   if (B * T == 0) return 0;
+  KV_ORDERLY("b200q_kv_keep", kv_refuse_array(count, 4));
   B200Q_REQUIRE(keep != nullptr, "b200q_kv_keep: null pointer");
+  KV_ORDERLY("b200q_kv_keep", kv_refuse_array(keep, 4));
   return launch_kv_keep(ctx, *cache, KvBatch{(int)B, (int)T, page_table, max_pages, start, count}, keep);
 }
 

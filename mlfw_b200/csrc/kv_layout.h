@@ -104,6 +104,8 @@ inline const char* kv_refuse_geometry(int64_t pages, int64_t page_tokens, int64_
 }
 inline bool kv_aligned(const void* p, size_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 
+constexpr const char* kv_misaligned = "an array of integers does not start on a multiple of its element's size";
+
 // B sequences of T rows; `what` holds back the pointer checks when there is nothing to do.
 inline const char* kv_refuse_batch(int64_t B, int64_t T, int64_t heads, const void* page_table, int64_t max_pages, const void* start) {
   if (B < 0 || T < 0 || max_pages < 0) return "negative dimension";
@@ -111,8 +113,11 @@ inline const char* kv_refuse_batch(int64_t B, int64_t T, int64_t heads, const vo
   if (max_pages > INT32_MAX) return "the page table is too wide";
   if (B * T == 0) return nullptr;
   if (start == nullptr || (page_table == nullptr && max_pages > 0)) return "null pointer";
+  if (!kv_aligned(page_table, 4) || !kv_aligned(start, 4)) return kv_misaligned;
   return nullptr;
 }
+// Optional arrays of `element` bytes each: count, tree, keep.
+inline const char* kv_refuse_array(const void* p, size_t element) { return kv_aligned(p, element) ? nullptr : kv_misaligned; }
 // An f32 operand whose row (b, t) of head h starts at base + (b * T + t) * ld + h * head_dim.
 inline const char* kv_refuse_rows(const void* base, int64_t ld, int64_t heads, int64_t head_dim) {
   if (base == nullptr) return "null pointer";

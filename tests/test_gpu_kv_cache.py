@@ -356,6 +356,29 @@ def test_attention_long_runs(ctx, B, T, H, heads, dim, most):
     check_attention(S, q, start, np.full(B, T), random_tree(S.rng, B, T) if T > 1 and T <= 64 else None, dim ** -0.5)
 
 
+@pytest.mark.parametrize("B,T,H,heads,dim", [(3000, 1, 2, 1, 64), (700, 2, 3, 3, 128), (257, 17, 2, 1, 64)])
+def test_attention_many_short_sequences(ctx, B, T, H, heads, dim):
+    """More sequences than threads of a block, of no to three cached tokens, most of them padding."""
+    S = Setup(ctx, B, 3 + T, 16, heads, dim)
+    start = S.rng.integers(0, 4, B)
+    count = np.where(S.rng.random(B) < 0.2, S.rng.integers(0, T + 1, B), 0)
+    for i in range(2):
+        S.codes[i] = np.clip(np.round(S.rng.standard_normal(S.codes[i].shape) * 42), -127, 127).astype(np.int8)
+        S.scales[i] = S.rng.uniform(0.01, 0.03, S.scales[i].shape).astype(np.float32)
+    S.upload()
+    q = (S.rng.standard_normal((B, T, H, dim)) * 2).astype(np.float32)
+    check_attention(S, q, start, count, None, dim ** -0.5)
+
+
+@pytest.mark.parametrize("H,dim,page", [(33, 64, 16), (40, 128, 256), (64, 128, 16), (65, 64, 128), (130, 128, 32)])
+def test_attention_many_heads_on_one(ctx, H, dim, page):
+    """A decoding step whose query heads fill the rows of the kernels for chunks."""
+    S = Setup(ctx, 2, 400, page, 1, dim)
+    S.fill([40, 400])
+    q = (S.rng.standard_normal((2, 1, H, dim)) * 2).astype(np.float32)
+    check_attention(S, q, [39, 399], None, None, dim ** -0.5, ld_pad=8)
+
+
 def test_positions_outside_the_cache(ctx):
     """A bad page or a position behind the table: the status bit, no write, zeros, not visible."""
     S = Setup(ctx, 2, 48, 16, 2, 64)
@@ -504,6 +527,11 @@ def test_refusals(ctx):
             ("below 2\\^31", lambda: c.read(1 << 16, 1 << 15, S.dtable, S.per, s, None, b, b, 128, 128))):
         with pytest.raises(e, match=what):
             call()
+    for call in (lambda: c.append(b, b, 128, 128, 1, 1, S.dtable.ptr + 2, S.per, s), lambda: c.read(1, 1, S.dtable, S.per, s.ptr + 1, None, b, b, 128, 128),
+                 lambda: c.append(b, b, 128, 128, 1, 1, S.dtable, S.per, s, s.ptr + 2), lambda: c.keep(1, 4, S.dtable, S.per, s, b.ptr + 2, None),
+                 lambda: c.attention(b, 128, 1, 1, 2, S.dtable, S.per, s, None, b.ptr + 4, 1.0, b, 128)):
+        with pytest.raises(e, match="multiple of its element"):
+            call()
     before = ctx.launch_count()
     c.append(b, b, 128, 128, 0, 4, None, 0, None)          # nothing to do is not an error
     c.attention(b, 128, 3, 0, 2, None, 0, None, None, None, 1.0, b, 128)
@@ -586,6 +614,66 @@ def test_recorded_step_follows_the_lengths(ctx, orc):
         length += T
     for g in graphs:
         ctx.graph_destroy(g)
+
+
+def test_recordings_and_eager_calls_in_turn(ctx):
+    """Attention of one, 40 and 140 query rows recorded, replayed in turn with eager calls on the same workspace, the pieces of
+    long items among them: every result is bit for bit the first one's."""
+    S = Setup(ctx, 3, 2200, 64, 2, 128)
+    for i in range(2):
+        S.codes[i] = np.clip(np.round(S.rng.standard_normal(S.codes[i].shape) * 42), -127, 127).astype(np.int8)
+        S.scales[i] = S.rng.uniform(0.01, 0.03, S.scales[i].shape).astype(np.float32)
+    S.upload()
+    start, calls = S.dev([2100, 33, 700]), []
+    for T, H in ((1, 4), (20, 4), (70, 4)):
+        q, o = ctx.to_device(S.rng.standard_normal((3 * T, H * 128)).astype(np.float32)), ctx.empty((3 * T, H * 128), np.float32)
+        calls.append((lambda q=q, o=o, T=T, H=H: S.cache.attention(q, H * 128, 3, T, H, S.dtable, S.per, start, None, None, 0.1, o, H * 128), o))
+    want, graphs = [], []
+    for call, o in calls:
+        call()
+        want.append(o.download().view(np.uint32))
+        ctx.graph_begin()
+        call()
+        graphs.append(ctx.graph_end())
+    for i, replay in ((0, 1), (1, 1), (2, 1), (2, 0), (0, 1), (1, 0), (1, 1), (0, 0), (2, 1), (2, 1), (0, 1)):
+        calls[i][1].fill_bytes(0xff)
+        ctx.graph_launch(graphs[i]) if replay else calls[i][0]()
+        for j in range(3):
+            ctx.graph_launch(graphs[j])
+        assert all((calls[j][1].download().view(np.uint32) == want[j]).all() for j in range(3))
+    for g in graphs:
+        ctx.graph_destroy(g)
+
+
+def test_two_contexts_at_once(ctx):
+    """Each context has its stream and its workspace: calls of both under way together give what they give alone."""
+    import mlfw_b200
+    with mlfw_b200.Context(0) as other:
+        both = []
+        for c in (ctx, other):
+            S = Setup(c, 4, 1500, 32, 2, 64, seed=5)
+            for i in range(2):
+                S.codes[i] = np.clip(np.round(S.rng.standard_normal(S.codes[i].shape) * 42), -127, 127).astype(np.int8)
+                S.scales[i] = S.rng.uniform(0.01, 0.03, S.scales[i].shape).astype(np.float32)
+            S.upload()
+            start = S.dev([1400, 0, 900, 77])
+            for T, H in ((1, 6), (24, 4), (65, 4)):
+                q, o = c.to_device(S.rng.standard_normal((4 * T, H * 64)).astype(np.float32)), c.empty((4 * T, H * 64), np.float32)
+                both.append((c, lambda S=S, q=q, o=o, T=T, H=H, start=start: S.cache.attention(q, H * 64, 4, T, H, S.dtable, S.per, start, None, None, 0.1, o, H * 64), o, S))
+        want = []
+        for c, call, o, _ in both:
+            call()
+            want.append(o.download().view(np.uint32))
+            o.fill_bytes(0xff)
+            c.sync()
+        for _ in range(20):
+            for k in (0, 3, 1, 4, 2, 5):
+                both[k][1]()
+        for (c, _, o, _), w in zip(both, want):
+            assert (o.download().view(np.uint32) == w).all()
+        other.check_status()
+        both.clear()
+        del call, o, S, q, start
 
 
 def test_block_with_a_cache(ctx):

@@ -67,6 +67,7 @@ int walk(int B, int T, int heads, int group, int rows, int warps, int grid, int6
   return 0;
 }
 uint32_t warp(uint32_t block, uint32_t threads, uint32_t thread) { return kv_warp(block, threads, thread); }
+const char* array(const void* p, int64_t element) { return kv_refuse_array(p, (size_t)element); }
 const char* rows(const void* base, int64_t ld, int64_t h, int64_t d) { return kv_refuse_rows(base, ld, h, d); }
 }
 """
@@ -87,7 +88,7 @@ def host(tmp_path_factory):
     lib.walk.argtypes = [C.c_int] * 7 + [i64, C.c_int, vp, vp, C.c_int, C.c_int, C.POINTER(i64)]
     lib.visible.restype, lib.visible.argtypes = i64, [i64, C.c_int, i64] + [C.c_int] * 5
     lib.tiles.argtypes = [i64, C.c_int, i64] + [C.c_int] * 6
-    for f, a in (("geometry", [i64] * 4), ("batch", [i64, i64, i64, vp, i64, vp]), ("rows", [vp, i64, i64, i64])):
+    for f, a in (("geometry", [i64] * 4), ("array", [vp, i64]), ("batch", [i64, i64, i64, vp, i64, vp]), ("rows", [vp, i64, i64, i64])):
         getattr(lib, f).restype, getattr(lib, f).argtypes = C.c_char_p, a
     return lib
 
@@ -176,6 +177,15 @@ def test_refusals(host):
     assert host.rows(p, 128, 2, 64) is None and host.rows(p, 400, 3, 128) is None
     for bad in ((None, 128, 2, 64), (p + 4, 128, 2, 64), (p, 130, 2, 64), (p, 124, 2, 64), (p, -128, 2, 64)):
         assert host.rows(*bad), bad
+
+
+def test_refusals_of_integer_arrays(host):
+    """An address that is no multiple of the element's size would fault on the GPU."""
+    assert host.array(None, 8) is None and host.array(4096, 8) is None and host.array(4100, 4) is None
+    assert b"multiple of its element" in host.array(4100, 8) and host.array(4098, 4)
+    for table, start in ((4098, 4096), (4096, 4097)):
+        assert b"multiple of its element" in host.batch(3, 5, 8, table, 7, start)
+    assert host.batch(0, 5, 8, 4098, 7, 4097) is None
 
 
 def test_entry_points_refuse_without_a_gpu():
