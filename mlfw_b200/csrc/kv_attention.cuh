@@ -126,8 +126,8 @@ __device__ __forceinline__ Run find_run(const AttnArgs& a, int row_blocks) {
   __shared__ int64_t warp_sum[32];
   __shared__ int found[3];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int E = a.B * row_blocks, per = (E + blockDim.x - 1) / blockDim.x;
-  const int e0 = min(E, tid * per), e1 = min(E, e0 + per);
+  const uint32_t E = (uint32_t)(a.B * row_blocks), per = (E + blockDim.x - 1) / blockDim.x;   // E < 2^31
+  const int e0 = (int)min(E, (uint32_t)tid * per), e1 = (int)min(E, (uint32_t)(tid + 1) * per);
   auto tiles = [&](int e) {
     const int b = e / row_blocks;
     return (int64_t)kv_tiles(a.g, a.start[b], kv_rows_in_use(a.count, b, a.T), a.group, ROWS, e - b * row_blocks, a.tree != nullptr, TILE) * a.g.heads;
