@@ -515,9 +515,9 @@ int launch_kv_attention(b200q_ctx* ctx, const b200q_kv_cache& c, const KvBatch& 
                    ld_q, ld_o, s.B, s.T, H, H / c.heads, scale * 1.4426950408889634f, ctx->status_dev, (uint32_t*)ctx->ws_kv.ptr,
                    (float*)((uint8_t*)ctx->ws_kv.ptr + kv_counter_bytes(ctx) + kv_item_bytes(ctx)), (int4*)((uint8_t*)ctx->ws_kv.ptr + kv_counter_bytes(ctx))};
   // Query rows per cache head.  Measured on both sides of the border, 8 cache heads, 16 sequences of up to 3000 tokens, here and
-  // there: 24 rows 42 and 63 us (head dimension 64), 63 and 81 us (128); 32 rows 49 and 65, 75 and 84 us; 48 rows 65 and
-  // 67, 102 and 85 us; 124 rows 149 and 73, 237 and 95 us.
-  if ((int64_t)s.T * a.group > 32) return launch_kv_attention_many(ctx, a, c.head_dim);
+  // there: 24 rows 38 and 56 us (head dimension 64), 56 and 76 us (128); 36 rows 51 and 58, 78 and 79; 40 rows 57 and 58, 83 and
+  // 79; 64 rows 83 and 60, 128 and 88.  (With 4 sequences of up to 600 tokens both take 14 to 30 us, here the fewer.)
+  if ((int64_t)s.T * a.group > 36) return launch_kv_attention_many(ctx, a, c.head_dim);
   return c.head_dim == 64 ? launch_four<64>(ctx, a) : launch_four<128>(ctx, a);
 }
 
