@@ -3,19 +3,23 @@
 // Row t of sequence b sees the start[b] positions cached before and, of the count[b] new ones, those up to itself (no
 // tree) or those whose bit is set in its row of ancestors.  Query heads h of a group H / heads share cache head h / (H / heads).
 //
-// The arithmetic.  A cached value is code * scale with an integer |code| <= 128, which binary16 holds exactly.  A query
-// row is written in fixed point against its largest element, x = q * 2^(10 - e) with 2^e <= max|q| < 2^(e+1), and split
-// x = hi + lo, |hi| <= 2^11 an integer, |lo| <= 1/2: two binary16 numbers that keep 23 bits.  Then
-//     sum_d q_d code_d = 2^(e-10) * (sum hi code + sum lo code),
-// two binary16 products with binary32 sums; the first is a sum of integers below 2^25 at worst and below 2^24 for all
-// ordinary rows, so it is exact, and a score carries the rounding of q (2^-23 of the row's largest element) and the one
-// of adding the two.  The weights are split the same way: with z the score in units of log2 and the row's running
-//     c = max over the keys of (z + log2 scale_v) - 10,      p = 2^(z - c),      w = p * scale_v <= 2^10 (1 + 2^-20),
+// The arithmetic.  A cached value is code * scale with an integer |code| <= 128.  The codes go into the tensor cores as they
+// are; queries and weights, which are binary32, are split into parts that the tensor cores take, so the result has binary32
+// accuracy and the cache is never dequantized.  Two forms:
+//   Many rows (kv_attention_umma.cu), binary16 products, two per contraction.  A query row is written in fixed point against
+//   its largest element, x = q * 2^(10 - e) with 2^e <= max|q| < 2^(e+1), and split x = hi + lo, |hi| <= 2^11 an integer,
+//   |lo| <= 1/2: 23 bits.  sum_d q_d code_d = 2^(e-10) * (sum hi code + sum lo code); the first is a sum of integers below
+//   2^25 at worst and below 2^24 for all ordinary rows, so it is exact.  A weight is its rounding to binary16 and the
+//   rounding of what is left: 22 bits.
+//   Few rows (kv_attention.cu), integer products: queries and weights as 32-bit fixed-point numbers in four 8-bit digits, sums
+//   in 32-bit integers, exact.
+// Either way a score carries the rounding of q (2^-23 of the row's largest element or better) and the one of adding the
+// parts.  With z the score in units of log2 and the row's running
+//     c = max over the keys of (z + log2 scale_v) - a constant,      p = 2^(z - c),      w = p * scale_v,
 // the row's result is sum w code / sum p, so one running number per row replaces the softmax's maximum and the weights'
 // exponent, and a key whose score is high but whose scale is small (or the other way round) costs no precision.  log2 of
-// the scale only steers c, so the approximate one does; it is held above -110 (a scale of 1e-33), which keeps p below 2^121; sums of
-// p are kept in units of 2^22.  So the cache's
-// codes go into the tensor cores as they are, and the result has binary32 accuracy at two binary16 products per contraction.
+// the scale only steers c, so the approximate one does; it is held from below (a scale of 1e-33 of the unit), which keeps p
+// below 2^121; sums of p are kept in units of 2^22.
 #pragma once
 #include "kernels.cuh"
 #include "kv.cuh"
@@ -41,7 +45,6 @@ struct AttnArgs {
 int launch_kv_attention_many(b200q_ctx* ctx, const AttnArgs& a, int D);   // kv_attention_umma.cu
 
 namespace {
-
 
 constexpr float NEG_INF = -__builtin_huge_valf();
 constexpr float P_UNIT = 0x1p-22f;       // sums of p are held times this: up to 2^24 keys of weight 2^120 stay finite

@@ -18,8 +18,12 @@ namespace {
 //     quarter of the row's outputs per thread in registers: o = o * 2^(c_old - c_new) + O.  Sums over tiles are binary32
 //     additions, not the tensor core's.
 // Scores and O are double-buffered (512 columns of tensor memory), so products, softmax and staging of neighbouring tiles
-// overlap.  Bound by the instruction issue of the softmax and staging warps, with the products (1024 cycles per tile of
-// 128 rows at head dimension 128) close behind.
+// overlap.  Measured: two prompts' chunks of 512 rows behind up to 4000 cached tokens, 16 heads on 4, 128 wide (26 GFLOP, twice
+// that in binary16 products): 120 us with the join, whose 27 MB between L2 and the SMs take 9; eight drafted trees of 31 over
+// up to 5000 tokens, 32 heads on 8: 81 us.  Bound by the softmax warps: about 3250 cycles per tile of 64 tokens, of which
+// the products need 1200 (tensor pipe 25 % busy): 500 instructions per warp and tile, 0.56 issued per cycle, the rest their
+// latency (the scores' load from tensor memory, the row's meeting, the split and the store of the weights).  Tried and
+// slower, against 110 us on the same box: scores three tiles ahead 136 (the registers spill), Q in tensor memory with a single O 117.
 //
 // With 64 or fewer rows (CS = 2) the lanes hold two copies of the rows, each copy takes half of a thread's tokens and has
 // weights of zero elsewhere, and the copies are joined at the end: the softmax work, which would leave lanes idle,
