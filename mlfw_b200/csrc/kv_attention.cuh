@@ -8,9 +8,9 @@
 // accuracy and the cache is never dequantized.  Two forms:
 //   Many rows (kv_attention_umma.cu), binary16 products, two per contraction.  A query row is written in fixed point against
 //   its largest element, x = q * 2^(10 - e) with 2^e <= max|q| < 2^(e+1), and split x = hi + lo, |hi| <= 2^11 an integer,
-//   |lo| <= 1/2: 23 bits.  sum_d q_d code_d = 2^(e-10) * (sum hi code + sum lo code); the first is a sum of integers below
-//   2^25 at worst and below 2^24 for all ordinary rows, so it is exact.  A weight is its rounding to binary16 and the
-//   rounding of what is left: 22 bits.
+//   |lo| <= 1/2: 23 bits.  sum_d q_d code_d = 2^(e-10) * (sum lo code + sum hi code), in one binary32 sum with the small parts
+//   first: D / 16 steps of integers, whose roundings of the running sum stay below the D that an ordinary binary32 sum has.
+//   A weight is its rounding to binary16 and the rounding of what is left: 22 bits.
 //   Few rows (kv_attention.cu), integer products: queries and weights as 32-bit fixed-point numbers in four 8-bit digits, sums
 //   in 32-bit integers, exact.
 // Either way a score carries the rounding of q (2^-23 of the row's largest element or better) and the one of adding the

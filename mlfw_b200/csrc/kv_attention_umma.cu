@@ -11,19 +11,21 @@ namespace {
 //   three staging warps: K and V of a tile from the cache into a ring in shared memory as binary16 tiles of the tensor cores'
 //     layout (V transposed), with the tokens' scales beside them, in units of sixteen tokens, which always share a page
 //     (three, so that the block has 20 warps and 96 registers per thread);
-//   one thread issues the products: S_hi = Q_hi K^T and S_lo = Q_lo K^T (tcgen05.mma kind::f16, 128 x 64) of tile j + 1, then
+//   one thread issues the products: S = Q_lo K^T + Q_hi K^T (tcgen05.mma kind::f16, 128 x 64) of tile j + 1, then
 //     O = P_lo V + P_hi V of tile j with the weights read from tensor memory;
 //   sixteen softmax warps, four threads per row with sixteen tokens of a tile each: scores from tensor memory, the row's c
 //     agreed on through shared memory, the weights' two halves written over the scores, and tile j - 1's O folded into a
 //     quarter of the row's outputs per thread in registers: o = o * 2^(c_old - c_new) + O.  Sums over tiles are binary32
 //     additions, not the tensor core's.
-// Scores and O are double-buffered (512 columns of tensor memory), so products, softmax and staging of neighbouring tiles
+// Scores and O are double-buffered (384 columns of tensor memory), so products, softmax and staging of neighbouring tiles
 // overlap.  Measured: two prompts' chunks of 512 rows behind up to 4000 cached tokens, 16 heads on 4, 128 wide (26 GFLOP, twice
-// that in binary16 products): 120 us with the join, whose 27 MB between L2 and the SMs take 9; eight drafted trees of 31 over
-// up to 5000 tokens, 32 heads on 8: 81 us.  Bound by the softmax warps: about 3250 cycles per tile of 64 tokens, of which
-// the products need 1200 (tensor pipe 25 % busy): 500 instructions per warp and tile, 0.56 issued per cycle, the rest their
+// that in binary16 products): 107 us with the join, whose 27 MB between L2 and the SMs take 9; eight drafted trees of 31 over
+// up to 5000 tokens, 32 heads on 8: 80 us.  Bound by the softmax warps: about 3150 cycles per tile of 64 tokens, of which
+// the products need 1200 (tensor pipe 25 % busy): 480 instructions per warp and tile, 0.56 issued per cycle, the rest their
 // latency (the scores' load from tensor memory, the row's meeting, the split and the store of the weights).  Tried and
-// slower, against 110 us on the same box: scores three tiles ahead 136 (the registers spill), Q in tensor memory with a single O 117.
+// slower, against 110 us on the same box: scores three tiles ahead 136 (the registers spill), Q in tensor memory with a
+// single O 117; the two parts of the scores in columns of their own, added by the softmax warps, is 110 against 107.7; a
+// hardware barrier for the row's meeting 107.0, not worth a wait without a limit.
 //
 // With 64 or fewer rows (CS = 2) the lanes hold two copies of the rows, each copy takes half of a thread's tokens and has
 // weights of zero elsewhere, and the copies are joined at the end: the softmax work, which would leave lanes idle,
@@ -42,8 +44,8 @@ struct Many {
   static constexpr int QHI = 0, QLO = Q_BYTES, RING = 2 * Q_BYTES, END = RING + STAGES * STAGE;
   static constexpr int SMEM = END + 1024;
 };
-// columns: scores (hi, lo) of even and odd tiles, the weights over them; O of even and odd tiles
-constexpr int TM_S = 0, TM_SLO = 64, TM_S_STEP = 128, TM_O = 256, TM_O_STEP = 128, TM_COLS = 512;
+// columns: scores of even and odd tiles, the weights over them; O of even and odd tiles
+constexpr int TM_S = 0, TM_S_STEP = 64, TM_O = 128, TM_O_STEP = 128, TM_COLS = 512;
 
 __device__ __forceinline__ uint64_t gtimer() {
   uint64_t t;
@@ -79,26 +81,6 @@ __device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sy
 
 // Loads from tensor memory: consecutive columns of this warp's lanes.  The wait stands in the same statement: registers that a
 // separate one ties to the wait get copied.
-__device__ __forceinline__ void tm_ld2(uint32_t at0, uint32_t at1, uint32_t (&x)[16], uint32_t (&y)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%32];\n\t"
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%33];\n\t"
-      "tcgen05.wait::ld.sync.aligned;"
-      : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]), "=r"(x[6]), "=r"(x[7]), "=r"(x[8]), "=r"(x[9]),
-        "=r"(x[10]), "=r"(x[11]), "=r"(x[12]), "=r"(x[13]), "=r"(x[14]), "=r"(x[15]),
-        "=r"(y[0]), "=r"(y[1]), "=r"(y[2]), "=r"(y[3]), "=r"(y[4]), "=r"(y[5]), "=r"(y[6]), "=r"(y[7]), "=r"(y[8]), "=r"(y[9]),
-          "=r"(y[10]), "=r"(y[11]), "=r"(y[12]), "=r"(y[13]), "=r"(y[14]), "=r"(y[15])
-      : "r"(at0), "r"(at1) : "memory");
-}
-__device__ __forceinline__ void tm_ld2(uint32_t at0, uint32_t at1, uint32_t (&x)[8], uint32_t (&y)[8]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%16];\n\t"
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%8, %9, %10, %11, %12, %13, %14, %15}, [%17];\n\t"
-      "tcgen05.wait::ld.sync.aligned;"
-      : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]), "=r"(x[6]), "=r"(x[7]),
-        "=r"(y[0]), "=r"(y[1]), "=r"(y[2]), "=r"(y[3]), "=r"(y[4]), "=r"(y[5]), "=r"(y[6]), "=r"(y[7])
-      : "r"(at0), "r"(at1) : "memory");
-}
 __device__ __forceinline__ void tm_ld(uint32_t at, uint32_t (&x)[32]) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\ttcgen05.wait::ld.sync.aligned;"
                : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]), "=r"(x[6]), "=r"(x[7]), "=r"(x[8]), "=r"(x[9]),
@@ -111,6 +93,11 @@ __device__ __forceinline__ void tm_ld(uint32_t at, uint32_t (&x)[16]) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\ttcgen05.wait::ld.sync.aligned;"
                : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]), "=r"(x[6]), "=r"(x[7]), "=r"(x[8]), "=r"(x[9]),
                  "=r"(x[10]), "=r"(x[11]), "=r"(x[12]), "=r"(x[13]), "=r"(x[14]), "=r"(x[15])
+               : "r"(at) : "memory");
+}
+__device__ __forceinline__ void tm_ld(uint32_t at, uint32_t (&x)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n\ttcgen05.wait::ld.sync.aligned;"
+               : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]), "=r"(x[6]), "=r"(x[7])
                : "r"(at) : "memory");
 }
 __device__ __forceinline__ void tm_st(uint32_t at, const uint32_t (&r)[8]) {
@@ -332,8 +319,8 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv_attention_many_kernel(cons
         alive = __all_sync(0xffffffffu, ok);
         if (!alive) break;
         fence_after();
-        uint32_t hi[NC], lo[NC];
-        tm_ld2(s_tm + col0, s_tm + TM_SLO + col0, hi, lo);
+        uint32_t sc[NC];
+        tm_ld(s_tm + col0, sc);
 
         // which of this thread's tokens its row sees
         uint32_t seen = tok_there[slot][cg];
@@ -353,7 +340,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv_attention_many_kernel(cons
           seen >>= copy * NC;
         }
 
-        // x = (S_hi + S_lo) * scale_k, the score z = x * rs
+        // x = S * scale_k, the score z = x * rs
         float x[NC], u[NC], top = NEG_INF;
 #pragma unroll
         for (int i = 0; i < NC; i += 4) {
@@ -361,7 +348,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv_attention_many_kernel(cons
           const float kk[4] = {k.x, k.y, k.z, k.w}, vv[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
           for (int c = 0; c < 4; c++) {
-            x[i + c] = (__uint_as_float(hi[i + c]) + __uint_as_float(lo[i + c])) * kk[c];
+            x[i + c] = __uint_as_float(sc[i + c]) * kk[c];
             u[i + c] = fmaf(x[i + c], rs, vv[c]);
           }
         }
@@ -397,7 +384,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv_attention_many_kernel(cons
           split_f16(wt[2], wt[3], h[i / 2 + 1], l[i / 2 + 1]);
         }
         l_run = fmaf(l_run, fold_new, sum * P_UNIT);
-        // the sixteen tokens' weights, zero where another copy has them: 8 + 8 columns over their S_hi
+        // the sixteen tokens' weights, zero where another copy has them: 8 + 8 columns over their scores
         uint32_t ph[8], pl[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) {
@@ -584,9 +571,11 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv_attention_many_kernel(cons
       if (lane == 0) {
 #pragma unroll
         for (int s = 0; s < D / 16; s++) {                       // 16 dimensions = 32 bytes along K per instruction
-          mma_ss(s_tm, qh_desc + (s >> 2) * (C::Q_BLOCK >> 4) + 2 * (s & 3), kd + (s >> 2) * (C::K_BLOCK >> 4) + 2 * (s & 3), idesc, s != 0);
-          mma_ss(s_tm + TM_SLO, ql_desc + (s >> 2) * (C::Q_BLOCK >> 4) + 2 * (s & 3), kd + (s >> 2) * (C::K_BLOCK >> 4) + 2 * (s & 3), idesc, s != 0);
+          mma_ss(s_tm, ql_desc + (s >> 2) * (C::Q_BLOCK >> 4) + 2 * (s & 3), kd + (s >> 2) * (C::K_BLOCK >> 4) + 2 * (s & 3), idesc, s != 0);
         }
+#pragma unroll
+        for (int s = 0; s < D / 16; s++)
+          mma_ss(s_tm, qh_desc + (s >> 2) * (C::Q_BLOCK >> 4) + 2 * (s & 3), kd + (s >> 2) * (C::K_BLOCK >> 4) + 2 * (s & 3), idesc, 1);
         mma_commit(sh_base + S::SCORES + 8 * (t & 1));
       }
       __syncwarp();
