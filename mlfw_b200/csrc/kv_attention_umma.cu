@@ -10,7 +10,8 @@ namespace {
 // One block per SM walks a run of 64-token tiles; an item is up to 128 rows, the 128 lanes of tensor memory.  Roles:
 //   three staging warps: K and V of a tile from the cache into a ring in shared memory as binary16 tiles of the tensor cores'
 //     layout (V transposed), with the tokens' scales beside them, in units of sixteen tokens, which always share a page
-//     (three, so that the block has 20 warps and 96 registers per thread);
+//     (three, so that the block has 20 warps and 96 registers per thread: the first case below takes 108 us, with two
+//     staging warps 127, with four, which leave 80 registers, 126);
 //   one thread issues the products: S = Q_lo K^T + Q_hi K^T (tcgen05.mma kind::f16, 128 x 64) of tile j + 1, then
 //     O = P_lo V + P_hi V of tile j with the weights read from tensor memory;
 //   sixteen softmax warps, four threads per row with sixteen tokens of a tile each: scores from tensor memory, the row's c
