@@ -23,10 +23,10 @@ namespace {
 // that in binary16 products): 107 us with the join, whose 27 MB between L2 and the SMs take 9; eight drafted trees of 31 over
 // up to 5000 tokens, 32 heads on 8: 80 us.  Bound by the softmax warps: about 3150 cycles per tile of 64 tokens, of which
 // the products need 1200 (tensor pipe 25 % busy): 480 instructions per warp and tile, 0.56 issued per cycle, the rest their
-// latency (the scores' load from tensor memory, the row's meeting, the split and the store of the weights).  Tried and
-// slower, against 110 us on the same box: scores three tiles ahead 136 (the registers spill), Q in tensor memory with a
+// latency (the scores' load from tensor memory, the row's meeting, the split and the store of the weights).  Not kept
+// (against 110 us on the same box): scores three tiles ahead 136 (the registers spill), Q in tensor memory with a
 // single O 117; the two parts of the scores in columns of their own, added by the softmax warps, is 110 against 107.7; a
-// hardware barrier for the row's meeting 107.0, not worth a wait without a limit.
+// hardware barrier for the row's meeting 107.0 against 107.7, not worth a wait without a limit.
 //
 // With 64 or fewer rows (CS = 2) the lanes hold two copies of the rows, each copy takes half of a thread's tokens and has
 // weights of zero elsewhere, and the copies are joined at the end: the softmax work, which would leave lanes idle,
