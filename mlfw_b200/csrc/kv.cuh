@@ -32,6 +32,9 @@ int kv_workspace(b200q_ctx* ctx);
 // The calls on a cache follow one another within microseconds (append, attention, keep), so each kernel is launched as a
 // programmatic dependent of the one before it: its blocks come while that one drains, and kv_after_previous holds back
 // everything until it has completed.  With profiling on, an event sits between the two and the overlap is off.
+// A block may thus be resident while kernels two or three back still write what it is going to read (codes, scales, queries,
+// page tables, rows to keep): none of that is read-only for the lifetime of the kernel, so it is loaded with coherent loads
+// (plain or __ldcg; L2 is where the writers' stores are) and never through __ldg or a const __restrict__ pointer.
 #ifdef __CUDACC__
 __device__ __forceinline__ void kv_after_previous() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");

@@ -148,10 +148,10 @@ __global__ void __launch_bounds__(32 * Four<D>::WARPS, 1) kv_attention_four_kern
   auto look_up = [&](bool anew) {                               // the pages of the tile `ahead`
     const uint32_t pos = (uint32_t)ahead_tile * IT;
     if (wide) {
-      if (anew || (pos & in_page) == 0) page0 = pos < ahead_vis ? __ldg(ahead_table + (pos >> shift)) : -1;
+      if (anew || (pos & in_page) == 0) page0 = pos < ahead_vis ? __ldcg(ahead_table + (pos >> shift)) : -1;
     } else {
-      page0 = pos < ahead_vis ? __ldg(ahead_table + (pos >> 4)) : -1;
-      page1 = pos + 16 < ahead_vis ? __ldg(ahead_table + (pos >> 4) + 1) : -1;
+      page0 = pos < ahead_vis ? __ldcg(ahead_table + (pos >> 4)) : -1;
+      page1 = pos + 16 < ahead_vis ? __ldcg(ahead_table + (pos >> 4) + 1) : -1;
     }
   };
   auto fetch = [&](int s, int place) {
@@ -235,7 +235,7 @@ __global__ void __launch_bounds__(32 * Four<D>::WARPS, 1) kv_attention_four_kern
       uint32_t top = 0;
 #pragma unroll
       for (int s = 0; s < 2 * KS; s++) {
-        x[s] = used ? __ldg(reinterpret_cast<const float4*>(src + (s >> 2) * 64 + t4 * 16 + (s & 3) * 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        x[s] = used ? __ldcg(reinterpret_cast<const float4*>(src + (s >> 2) * 64 + t4 * 16 + (s & 3) * 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
         top = max(max(top, max(__float_as_uint(x[s].x) & 0x7fffffffu, __float_as_uint(x[s].y) & 0x7fffffffu)),
                   max(__float_as_uint(x[s].z) & 0x7fffffffu, __float_as_uint(x[s].w) & 0x7fffffffu));
       }

@@ -266,7 +266,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv_attention_many_kernel(cons
         uint32_t top = 0;
 #pragma unroll
         for (int i = 0; i < QD / 4; i++) {
-          x[i] = used ? __ldg(reinterpret_cast<const float4*>(src) + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+          x[i] = used ? __ldcg(reinterpret_cast<const float4*>(src) + i) : make_float4(0.f, 0.f, 0.f, 0.f);
           top = max(max(top, max(__float_as_uint(x[i].x) & 0x7fffffffu, __float_as_uint(x[i].y) & 0x7fffffffu)),
                     max(__float_as_uint(x[i].z) & 0x7fffffffu, __float_as_uint(x[i].w) & 0x7fffffffu));
         }
@@ -487,7 +487,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv_attention_many_kernel(cons
       const int64_t pos0 = (int64_t)w.tile0 * MT - (int64_t)first_unit * 16;
       auto page_of = [&](uint32_t u) -> int {                    // -1: nothing of the unit is visible
         const int64_t pos = pos0 + (int64_t)u * 16;
-        return (u < end_unit && pos < in_table) ? __ldg(table + (pos >> a.g.page_shift)) : -1;
+        return (u < end_unit && pos < in_table) ? __ldcg(table + (pos >> a.g.page_shift)) : -1;
       };
       uint4 rk[KN];
       uint32_t rv[VN * 8];
@@ -498,13 +498,13 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv_attention_many_kernel(cons
         const int64_t cell = ok ? (((int64_t)page * a.g.heads + w.head) << a.g.page_shift) + (pos & ((1 << a.g.page_shift) - 1)) : 0;
         const int8_t *kp = a.k + cell * D, *vp = a.v + cell * D;
 #pragma unroll
-        for (int i = 0; i < KN; i++) rk[i] = ok ? __ldg(reinterpret_cast<const uint4*>(kp) + i * 32 + lane) : make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < KN; i++) rk[i] = ok ? __ldcg(reinterpret_cast<const uint4*>(kp) + i * 32 + lane) : make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int o = 0; o < VN; o++)
 #pragma unroll
-          for (int i = 0; i < 8; i++) rv[o * 8 + i] = ok ? __ldg(reinterpret_cast<const uint32_t*>(vp + ((v_oct + o) * 8 + i) * D) + v_L) : 0u;
+          for (int i = 0; i < 8; i++) rv[o * 8 + i] = ok ? __ldcg(reinterpret_cast<const uint32_t*>(vp + ((v_oct + o) * 8 + i) * D) + v_L) : 0u;
         ks = vs = 0.0f;
-        if (ok && lane < 16 && pos + lane < w.vis) { ks = __ldg(a.ks + cell + lane); vs = __ldg(a.vs + cell + lane); }
+        if (ok && lane < 16 && pos + lane < w.vis) { ks = __ldcg(a.ks + cell + lane); vs = __ldcg(a.vs + cell + lane); }
       };
       int page = page_of(next), page_next = page_of(next + STAGE_WARPS);
       fetch(next, page);

@@ -82,7 +82,7 @@ __device__ __forceinline__ void append_row(const float4 (&x)[V4], bool live, int
 }
 
 template <int D>
-__global__ void __launch_bounds__(256, 4) kv_append_kernel(const KvArgs a, const float* __restrict__ k, const float* __restrict__ v, int64_t ld_k,
+__global__ void __launch_bounds__(256, 4) kv_append_kernel(const KvArgs a, const float* k, const float* v, int64_t ld_k,
                                                            int64_t ld_v, uint32_t units, uint32_t chunks) {
   constexpr int V4 = D / 32;
   kv_after_previous();
@@ -127,16 +127,23 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const KvArgs a, float* __r
   if ((int)t >= kv_rows_in_use(a.count, b, a.T) || head >= (uint32_t)a.g.heads) return;
   const int64_t row = kv_row(a.g, a.page_table, b, head, (int64_t)a.start[b] + t);
   if (row < 0 && sub == 0) atomicOr(a.status, STATUS_BAD_INDEX);
+  uint32_t w[2][V4];
+  float s[2];
 #pragma unroll
   for (int kv = 0; kv < 2; kv++) {
     const uint32_t* codes = reinterpret_cast<const uint32_t*>((kv ? a.v : a.k) + (row < 0 ? 0 : row) * D) + sub;
-    const float s = row < 0 ? 0.0f : __ldg((kv ? a.vs : a.ks) + row);
+    s[kv] = row < 0 ? 0.0f : __ldcg((kv ? a.vs : a.ks) + row);
+#pragma unroll
+    for (int i = 0; i < V4; i++) w[kv][i] = row < 0 ? 0u : __ldcg(codes + 8 * i);
+  }
+#pragma unroll
+  for (int kv = 0; kv < 2; kv++) {
     float4* y = reinterpret_cast<float4*>((kv ? v_out : k_out) + (int64_t)token * (kv ? ld_v : ld_k) + head * D) + sub;
 #pragma unroll
     for (int i = 0; i < V4; i++) {
-      const uint32_t w = row < 0 ? 0u : __ldg(codes + 8 * i);
-      __stcs(y + 8 * i, make_float4(__fmul_rn((float)(int8_t)w, s), __fmul_rn((float)(int8_t)(w >> 8), s),
-                                    __fmul_rn((float)(int8_t)(w >> 16), s), __fmul_rn((float)(int8_t)(w >> 24), s)));
+      const uint32_t x = w[kv][i];
+      __stcs(y + 8 * i, make_float4(__fmul_rn((float)(int8_t)x, s[kv]), __fmul_rn((float)(int8_t)(x >> 8), s[kv]),
+                                    __fmul_rn((float)(int8_t)(x >> 16), s[kv]), __fmul_rn((float)(int8_t)(x >> 24), s[kv])));
     }
   }
 }
@@ -148,7 +155,7 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const KvArgs a, float* __r
 // three dependent loads (count and keep, the page table, the rows): latency, 4.8 us for eight sequences of 8 heads.
 // ---------------------------------------------------------------------------
 template <int D>
-__global__ void __launch_bounds__(128) kv_keep_kernel(const KvArgs a, const int32_t* __restrict__ keep) {
+__global__ void __launch_bounds__(128) kv_keep_kernel(const KvArgs a, const int32_t* keep) {
   constexpr int Q = D / 16, PER = KV_MAX_TREE * Q / 128;   // 16-byte pieces of a row; pieces a thread holds of K (and of V)
   __shared__ int64_t from[KV_MAX_TREE], to[KV_MAX_TREE];
   kv_after_previous();

@@ -1,0 +1,90 @@
+"""GPU tests of the int8 key/value cache as a serving host calls it: steps one behind the other without a wait between
+them, and accuracy where the operands are uneven.
+
+The host model of the cache, the formula in binary64 and the guarded buffers are those of test_gpu_kv_cache.py.
+"""
+import numpy as np
+import pytest
+
+from gpu_util import Guarded
+from test_gpu_kv_cache import Setup, attention_rows, random_tree
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    import mlfw_b200
+    c = mlfw_b200.Context(0)
+    yield c
+    c.check_status()
+    c.close()
+
+
+# ------------------------------------------------------------------------------------------------ steps without a wait
+@pytest.mark.parametrize("heads,H,dim,T", [(2, 4, 128, 40), (3, 3, 64, 40), (2, 2, 64, 12)])
+def test_verification_steps_back_to_back(ctx, orc, heads, H, dim, T):
+    """Append, tree attention, keep, read, over and over on the same positions with other data, nothing between the launches:
+    every kernel reads what the one before it has just written.  Once call by call, twice as one recording."""
+    B, page, steps = 2, 16, 10
+    S = Setup(ctx, B, 100 + T, page, heads, dim)
+    start = np.array([100, 37])
+    S.fill(start)
+    ld = (H + 2 * heads) * dim
+    x = S.rng.standard_normal((steps, B * T, ld)).astype(np.float32)
+    trees = [random_tree(S.rng, B, T) for _ in range(steps)]
+    keep, kept = np.zeros((steps, B, T), np.int64), np.zeros((steps, B), np.int64)
+    for i in range(steps):
+        for b in range(B):
+            path = np.flatnonzero((trees[i][b, S.rng.integers(T // 2, T)] >> np.arange(T, dtype=np.uint64)) & np.uint64(1))
+            keep[i, b, : path.size], kept[i, b] = path, path.size
+    dx, dtree, dkeep, dkept = [ctx.to_device(a) for a in x], [S.dev(t, np.uint64) for t in trees], [S.dev(a) for a in keep], [S.dev(a) for a in kept]
+    dstart = S.dev(start)
+    outs = [[Guarded(ctx, (B * T, n * dim), np.float32, np.zeros((B * T, n * dim))) for n in (H, heads, heads)] for _ in range(steps)]
+
+    def run():
+        for i in range(steps):
+            p, (o, k, v) = dx[i].ptr, outs[i]
+            S.cache.append(p + 4 * H * dim, p + 4 * (H + heads) * dim, ld, ld, B, T, S.dtable, S.per, dstart)
+            S.cache.attention(p, ld, B, T, H, S.dtable, S.per, dstart, None, dtree[i], dim ** -0.5, o.ptr, H * dim)
+            S.cache.keep(B, T, S.dtable, S.per, dstart, dkeep[i], dkept[i])
+            S.cache.read(B, T, S.dtable, S.per, dstart, None, k.ptr, v.ptr, heads * dim, heads * dim)
+
+    want = []
+    for i in range(steps):
+        r = x[i].reshape(B, T, H + 2 * heads, dim)
+        S.append(orc, r[:, :, H:H + heads], r[:, :, H + heads:], start, [T] * B)
+        attn = attention_rows(S, np.ascontiguousarray(r[:, :, :H]), start, [T] * B, trees[i], dim ** -0.5)
+        for a in S.codes + S.scales:
+            for b in range(B):
+                src, dst = start[b] + keep[i, b, : kept[i, b]], start[b] + np.arange(kept[i, b])
+                a[S.table[b, dst // page], :, dst % page] = a[S.table[b, src // page], :, src % page]
+        back = []
+        for j in range(2):
+            pos = start[:, None] + np.arange(T)
+            p, at = np.take_along_axis(S.table, pos // page, 1), pos % page
+            back.append(S.codes[j][p, :, at].astype(np.float32) * S.scales[j][p, :, at][..., None])
+        want.append((attn, back))
+
+    def check():
+        for (o, k, v), ((value, bound), back) in zip(outs, want):
+            assert (np.abs(o.download().reshape(value.shape) - value).max(-1) <= bound).all()
+            for got, w in ((k, back[0]), (v, back[1])):
+                assert (got.download().view(np.uint32) == w.reshape(B * T, -1).view(np.uint32)).all()
+        S.check()
+
+    run()
+    check()
+    first = [o.download().view(np.uint32) for o, _, _ in outs]
+    ctx.graph_begin()
+    run()
+    graph = ctx.graph_end()
+    for _ in range(2):
+        for row in outs:
+            for buf in row:
+                buf.upload(np.zeros(buf.shape))
+        ctx.graph_launch(graph)
+        ctx.graph_launch(graph)
+        check()
+        assert all((o.download().view(np.uint32) == f).all() for (o, _, _), f in zip(outs, first))
+    ctx.graph_destroy(graph)
