@@ -372,7 +372,8 @@ int b200q_kv_keep(b200q_ctx* ctx, b200q_kv_cache* cache, int64_t B, int64_t T, c
  * Between begin and end every call on the context is recorded instead of executed; calls that synchronise or copy to
  * or from host memory are not allowed there, and every workspace must already have its size: run the same calls once,
  * not captured, before capturing them.  The recorded pointers and shapes are fixed; replay as often as wanted, also after
- * other calls have made a workspace grow: while a recording exists the memory it uses is kept. */
+ * other calls have made a workspace grow: while a recording exists the memory it uses is kept.  A recording belongs to the
+ * context it was made on; launching or destroying it through another one is refused. */
 typedef struct b200q_graph b200q_graph;
 int b200q_graph_begin(b200q_ctx* ctx);
 int b200q_graph_end(b200q_ctx* ctx, b200q_graph** out);

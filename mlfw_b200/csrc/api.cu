@@ -868,6 +868,7 @@ int b200q_linear_f32_host(b200q_ctx* ctx, const float* x_host, const int8_t* W_n
 
 // ---------------------------------------------------------------- captured steps
 struct b200q_graph {
+  b200q_ctx* ctx = nullptr;   // whose stream it was recorded on and whose workspaces it uses
   cudaGraph_t graph = nullptr;
   cudaGraphExec_t exec = nullptr;
   uint64_t kernels = 0;   // kernel launches recorded in it
@@ -913,6 +914,7 @@ int b200q_graph_end(b200q_ctx* ctx, b200q_graph** out) {
     set_error("b200q_graph_end: out of host memory");
     return 2;
   }
+  g->ctx = ctx;
   g->graph = graph;
   g->exec = exec;
   g->kernels = kernels;
@@ -924,6 +926,7 @@ int b200q_graph_end(b200q_ctx* ctx, b200q_graph** out) {
 int b200q_graph_launch(b200q_ctx* ctx, b200q_graph* graph) {
   if (use_device(ctx)) return 1;
   B200Q_REQUIRE(graph != nullptr && graph->exec != nullptr, "b200q_graph_launch: null graph");
+  B200Q_REQUIRE(graph->ctx == ctx, "b200q_graph_launch: the recording belongs to another context");
   B200Q_NOT_CAPTURING(ctx, "b200q_graph_launch");
   B200Q_CHECK_CUDA(cudaGraphLaunch(graph->exec, ctx->stream));
   ctx->launches += graph->kernels;
@@ -933,6 +936,7 @@ int b200q_graph_launch(b200q_ctx* ctx, b200q_graph* graph) {
 int b200q_graph_destroy(b200q_ctx* ctx, b200q_graph* graph) {
   if (use_device(ctx)) return 1;
   if (!graph) return 0;
+  B200Q_REQUIRE(graph->ctx == ctx, "b200q_graph_destroy: the recording belongs to another context");
   B200Q_CHECK_CUDA(cudaStreamSynchronize(ctx->stream));
   if (graph->exec) cudaGraphExecDestroy(graph->exec);
   if (graph->graph) cudaGraphDestroy(graph->graph);

@@ -88,3 +88,25 @@ def test_verification_steps_back_to_back(ctx, orc, heads, H, dim, T):
         check()
         assert all((o.download().view(np.uint32) == f).all() for (o, _, _), f in zip(outs, first))
     ctx.graph_destroy(graph)
+
+
+def test_a_recording_belongs_to_its_context(ctx):
+    """Launching or destroying it through another context is refused: the workspaces it uses are its own context's."""
+    import mlfw_b200
+    S = Setup(ctx, 1, 40, 16, 2, 64)
+    S.fill([40])
+    start, q = S.dev([39]), ctx.to_device(S.rng.standard_normal((1, 128)).astype(np.float32))
+    out = Guarded(ctx, (1, 128), np.float32, np.zeros((1, 128)))
+    ctx.graph_begin()
+    S.cache.attention(q, 128, 1, 1, 2, S.dtable, S.per, start, None, None, 0.125, out.ptr, 128)
+    graph = ctx.graph_end()
+    with mlfw_b200.Context(0) as other:
+        with pytest.raises(mlfw_b200.B200QError, match="another context"):
+            other.graph_launch(graph)
+        with pytest.raises(mlfw_b200.B200QError, match="another context"):
+            other.graph_destroy(graph)
+    assert (out.download() == 0).all()
+    ctx.graph_launch(graph)
+    value, bound = attention_rows(S, q.download().reshape(1, 1, 2, 64), [39], [1], None, 0.125)
+    assert (np.abs(out.download().reshape(value.shape) - value).max(-1) <= bound).all()
+    ctx.graph_destroy(graph)
