@@ -20,10 +20,11 @@ Weights are quantized per output channel on the device when the block is built a
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Dict, Optional
+from typing import Dict, List, Optional
 
 import numpy as np
 
+from ._lib import B200QError
 from .device import Context, DeviceBuffer, W_NK
 from .kv_cache import KVCache
 
@@ -65,6 +66,14 @@ class QuantLinear:
                            ctx.to_device(np.ascontiguousarray(bias.data, np.float32)) if bias is not None else None)
 
 
+@dataclass
+class _Rows:
+    """Intermediate buffers of a block for up to ``rows`` rows, and whether a recorded call used them."""
+    rows: int
+    bufs: Dict[str, DeviceBuffer]
+    recorded: bool = False
+
+
 class GPTBlock:
     """One block for activations [B*S, D]; ``forward`` enqueues everything on the context's stream."""
 
@@ -82,7 +91,8 @@ class GPTBlock:
         self.fc2 = QuantLinear.from_float(ctx, params["w2"], params["b2"])
         self._bufs: Dict[str, DeviceBuffer] = {}
         self._M = -1
-        self._cached_bufs: Dict[int, Dict[str, DeviceBuffer]] = {}
+        self._cached = _Rows(0, {})                # buffers of forward_cached
+        self._recorded: List[_Rows] = []           # smaller ones that recordings go on using
 
     def _reserve(self, M: int) -> Dict[str, DeviceBuffer]:
         if M != self._M:
@@ -98,6 +108,25 @@ class GPTBlock:
             "n2_q": c.empty((M, D), np.int8), "n2_s": c.empty((M,), np.float32), "f1": c.empty((M, FF), np.float32),
             "f1_q": c.empty((M, FF), np.int8), "f1_s": c.empty((M,), np.float32), "f2": c.empty((M, D), np.float32),
         }
+
+    def _reserve_cached(self, M: int) -> Dict[str, DeviceBuffer]:
+        """Buffers of M rows: the first rows of one set that grows.  A recording holds the addresses of the set it was made with,
+        so a set that a recorded call used is kept beside the larger one until the context has no recording left."""
+        c = self.ctx
+        if not c.recording and c.recordings == 0:
+            self._recorded.clear()
+            self._cached.recorded = False
+        if M > self._cached.rows or not self._cached.bufs:
+            if c.recording:
+                raise B200QError(f"forward_cached: {M} rows are more than the block has buffers for; make the same call once before b200q_graph_begin")
+            rows = M + M // 8
+            if self._cached.recorded:
+                self._recorded.append(self._cached)
+            self._cached = _Rows(0, {})            # the old set goes before the new one comes
+            self._cached = _Rows(rows, self._buffers(rows))
+        if c.recording:
+            self._cached.recorded = True
+        return {name: b.head(M) for name, b in self._cached.bufs.items()}
 
     def forward(self, h: DeviceBuffer, B: int, S: int, out: DeviceBuffer, causal: bool = True) -> Dict[str, DeviceBuffer]:
         """h, out: f32 [B*S, D].  Returns the intermediate buffers (reused by the next call with the same size)."""
@@ -127,14 +156,12 @@ class GPTBlock:
         the new tokens are appended, attention reads the cache.  h, out: f32 [B*T, D], row b*T + t.  A prompt's chunk (T tokens),
         a decoding step (T = 1) or, with ``tree`` (uint64 [B*T]), drafted tokens; after a verification
         :meth:`KVCache.keep` drops the refused ones.  Every row is computed, rows from count[b] on without attention.
-        Returns the intermediate buffers; those of every B*T it was called with stay with the block, so that a recorded step
-        remains valid while prompts of other lengths pass in between."""
+        Returns the intermediate buffers, valid until the next call: one set serves every B*T and grows with the largest, and a
+        recorded step remains valid while larger prompts pass in between."""
         c, D, H = self.ctx, self.D, self.H
         assert cache.heads == H and cache.head_dim == 64, "the cache has another shape than the block's heads"
         M = B * T
-        if M not in self._cached_bufs:
-            self._cached_bufs[M] = self._buffers(M)
-        t = self._cached_bufs[M]
+        t = self._reserve_cached(M)
         c.layernorm_quantize(h, None, self.g1, self.b1, self.eps, M, D, None, None, t["n1_q"], t["n1_s"])
         c.int8_linear(t["n1_q"], t["n1_s"], self.qkv.w, self.qkv.scales, self.qkv.bias, "none", M, 3 * D, D, t["qkv"])
         base = t["qkv"].ptr

@@ -51,6 +51,14 @@ class DeviceBuffer:
         check(self.ctx.lib.b200q_memset(self.ctx.handle, self.ptr, value, self.nbytes), "b200q_memset")
         return self
 
+    def head(self, rows: int) -> "DeviceBuffer":
+        """The first ``rows`` rows as a buffer of that shape; the memory stays this buffer's, which lives as long as the view does."""
+        v = object.__new__(DeviceBuffer)
+        v.ctx, v.shape, v.dtype, v.ptr, v.owner = self.ctx, (int(rows),) + self.shape[1:], self.dtype, self.ptr, self
+        v.nbytes = int(np.prod(v.shape, dtype=np.int64)) * v.dtype.itemsize
+        v._free = False
+        return v
+
     def free(self) -> None:
         if self._free and self.ptr is not None and self.ctx.handle:
             self.ctx.lib.b200q_free(self.ctx.handle, self.ptr)
@@ -96,7 +104,12 @@ def _ptr(b):
 
 
 class Context:
-    """One GPU.  Raises if no CUDA device (or the library) is available."""
+    """One GPU.  Raises if no CUDA device (or the library) is available.
+
+    ``recording`` is true between :meth:`graph_begin` and :meth:`graph_end`; ``recordings`` counts those that exist."""
+
+    recording = False
+    recordings = 0
 
     def __init__(self, device: int = 0, _borrowed_handle=None):
         self.lib = _lib.lib()
@@ -189,10 +202,13 @@ class Context:
     # ---- captured steps
     def graph_begin(self):
         check(self.lib.b200q_graph_begin(self.handle), "b200q_graph_begin")
+        self.recording = True
 
     def graph_end(self) -> int:
         g = C.c_void_p()
+        self.recording = False          # also when it fails
         check(self.lib.b200q_graph_end(self.handle, C.byref(g)), "b200q_graph_end")
+        self.recordings += 1
         return g.value
 
     def graph_launch(self, graph: int):
@@ -200,6 +216,8 @@ class Context:
 
     def graph_destroy(self, graph: int):
         check(self.lib.b200q_graph_destroy(self.handle, graph), "b200q_graph_destroy")
+        if graph:
+            self.recordings -= 1
 
     def set_quant_variant(self, variant: int):
         check(self.lib.b200q_set_quant_variant(self.handle, variant), "b200q_set_quant_variant")

@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 
 from gpu_util import Guarded
-from test_gpu_kv_cache import Setup, attention_rows, random_tree
+from test_gpu_kv_cache import Setup, attention_bound, attention_rows, random_tree
 
 pytestmark = pytest.mark.gpu
 
@@ -110,3 +110,80 @@ def test_a_recording_belongs_to_its_context(ctx):
     value, bound = attention_rows(S, q.download().reshape(1, 1, 2, 64), [39], [1], None, 0.125)
     assert (np.abs(out.download().reshape(value.shape) - value).max(-1) <= bound).all()
     ctx.graph_destroy(graph)
+
+
+# ------------------------------------------------------------------------------------------------ the block over a cache
+def block_attention(k, v, qkv, start, count, tree):
+    """The formula in binary64 over rows read back (k, v [B, n, H, 64]) and its bound, for the rows in use."""
+    for b in range(len(start)):
+        n = int(start[b]) + int(count[b])
+        j = np.arange(n) - int(start[b])
+        for r in range(int(count[b])):
+            see = (j < 0) | ((j <= r) if tree is None else ((tree[b, r] >> np.clip(j, 0, 63).astype(np.uint64)) & np.uint64(1)).astype(bool))
+            for h in range(k.shape[2]):
+                x = qkv[b, r, 0, h].astype(np.float64)
+                z = 0.125 * (k[b, :n][see, h] @ x)
+                w = np.exp(z - z.max())
+                one = np.ones(n)
+                yield b, r, h, w @ v[b, :n][see, h] / w.sum(), attention_bound(x, k[b, :n, h], one, v[b, :n, h], one, 0.125, see)
+
+
+@pytest.mark.parametrize("tree", [False, True])
+def test_block_with_a_padded_batch(ctx, tree):
+    """forward_cached with uneven counts, none among them, call by call and recorded: rows in use follow the formula, rows behind
+    them have no attention and change nothing."""
+    import mlfw_b200
+    from mlfw_b200.block import GPTBlock, random_block_params
+    D, H, FF, B, T, page = 128, 2, 512, 4, 9, 16
+    blk = GPTBlock(ctx, D, H, FF, random_block_params(D, FF, seed=12, std=0.3))
+    rng = np.random.default_rng(13)
+    table, cache = rng.permutation(16).reshape(B, 4).astype(np.int32), mlfw_b200.KVCache(ctx, 16, page, H, 64)
+    for b in (cache.k_codes, cache.v_codes):
+        b.fill_bytes(0x80)
+    for b in (cache.k_scales, cache.v_scales):
+        b.fill_bytes(0xff)                                        # NaN: what no call has written must not show
+    dt, length, zero = ctx.to_device(table), np.array([0, 20, 7, 30], np.int32), ctx.to_device(np.zeros(B, np.int32))
+    fill = rng.standard_normal((B * 30, D)).astype(np.float32)
+    blk.forward_cached(ctx.to_device(fill), B, 30, cache, dt, 4, zero, ctx.empty((B * 30, D), np.float32), count=ctx.to_device(length))
+    start, counts = ctx.to_device(length), [np.array(c, np.int32) for c in ([9, 0, 4, 1], [0, 0, 0, 0], [3, 9, 0, 8])]
+    trees = random_tree(rng, B, T) if tree else None
+    h, out = Guarded(ctx, (B * T, D), np.float32), Guarded(ctx, (B * T, D), np.float32)
+    dcount, dtree = Guarded(ctx, (B,), np.int32), ctx.to_device(trees) if tree else None
+
+    def step():
+        return blk.forward_cached(h.ptr, B, T, cache, dt, 4, start, out.ptr, count=dcount.ptr, tree=dtree)
+
+    def rows(count):
+        h.upload(x)
+        dcount.upload(count)
+
+    graph = None
+    for count in counts + counts:
+        x = rng.standard_normal((B * T, D)).astype(np.float32)
+        rows(count)
+        if graph is None:
+            t = step()
+        else:
+            ctx.graph_launch(graph)
+        ctx.sync()
+        attn, got = t["attn"].download().reshape(B, T, H, 64), out.download().reshape(B, T, D)
+        back = [ctx.empty((B, 40, H, 64), np.float32).fill_bytes(0) for _ in range(2)]
+        cache.read(B, 40, dt, 4, zero, ctx.to_device(length + count), back[0], back[1], D, D)
+        k, v = (o.download().astype(np.float64) for o in back)
+        qkv = t["qkv"].download().reshape(B, T, 3, H, 64)
+        for b, r, hd, want, bound in block_attention(k, v, qkv, length, count, trees):
+            assert np.abs(attn[b, r, hd] - want).max() <= bound
+        used = np.arange(T)[None, :] < count[:, None]
+        assert (attn[~used] == 0).all() and np.isfinite(got).all()
+        x[~used.reshape(-1)] = rng.standard_normal((int((~used).sum()), D)) * 50      # other padding, the same rows in use
+        rows(count)
+        step()
+        ctx.sync()
+        again = out.download().reshape(B, T, D)
+        assert (again[used].view(np.uint32) == got[used].view(np.uint32)).all()
+        if graph is None and count is counts[-1]:
+            ctx.graph_begin()
+            t = step()
+            graph = ctx.graph_end()
+    ctx.graph_destroy(graph)
+    cache.close()
