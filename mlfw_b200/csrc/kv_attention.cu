@@ -29,7 +29,8 @@ __device__ __forceinline__ uint32_t v_at(int t, int c) {
 // columns after one exchange, so no score is computed twice.  Sums are 32-bit integers and exact: scores carry the rounding of
 // adding the digits, and the outputs are added up without rounding until a row's c changes (or 2^15 tokens have passed), when
 // they are converted, scaled and moved to binary32.  c = top - 26 leaves 5.5 bits before a larger weight (below 2^32) moves it.
-// Scales of V are taken relative to the power of two of the first tile's largest (kappa), so that tiny values keep their digits.
+// Scales of V are taken relative to a power of two 2^kappa, that of the first tile's largest until one 2^60 times as large comes, so
+// that neither tiny nor huge values leave binary32 anywhere on the way: 2^kappa meets the quotient of the two sums at the end.
 //
 // About 550 instructions per warp and 32 tokens of 128 dimensions, 500 of 64 (conversion of the codes to binary16 for
 // m16n8k16, tried first, took 1300).  Bound by reading the cache: 5.4 TB/s of the 6.5 measured at 48 sequences of up to 6000
@@ -44,7 +45,7 @@ template <int D>
 struct Four {
   static constexpr int WARPS = D == 128 ? 8 : 12, STAGES = D == 128 ? 2 : 3;
   static constexpr int GRAN = 2 * KV_TILE * D + 2 * KV_TILE * 4, TILE = 2 * GRAN;   // sixteen tokens: K and V codes, K and V scales
-  static constexpr int RING = WARPS * STAGES * TILE, SLOT = 4 * (D + 2) * 4, SMEM = RING + WARPS * SLOT;
+  static constexpr int RING = WARPS * STAGES * TILE, SLOT = 4 * (D + 3) * 4, SMEM = RING + WARPS * SLOT;
 };
 __device__ __forceinline__ void imma(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {   // s8 x s8
   asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -314,25 +315,43 @@ __global__ void __launch_bounds__(32 * Four<D>::WARPS, 1) kv_attention_four_kern
           if (!(held && (q < 0 || (a.tree ? (row_seen >> q) & 1 : q <= row_t)))) z[j] = NEG_INF;
         }
       }
-      if (kf == 0.0f) {                                         // kappa: the power of two of the first scales
-        float big = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
+      auto kappa_of = [](float big) {                           // 2^-kappa of a tile's scales, 0 where none is above zero
 #pragma unroll
         for (int x = 1; x < 32; x <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, x));
-        if (big > 0.0f) kf = pow2(127 - min(max(__float_as_int(big) >> 23, 1), 253));
-      }
-      float top = NEG_INF;
+        return big > 0.0f ? pow2(127 - min(max(__float_as_int(big) >> 23, 1), 253)) : 0.0f;
+      };
+      if (kf == 0.0f) kf = kappa_of(fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3])));
+      auto top_of = [&] {                                       // scales relative to kappa, and the row's largest weight in units of log2
+        float top = NEG_INF;
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
-        vs[j] *= kf;
-        top = fmaxf(top, z[j] + fmaxf(log2_raw(vs[j]), -88.0f));
-      }
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-      const bool grow = top > c_run + C_SLACK;
-      if (__any_sync(0xffffffffu, grow) || since == 1024) {
-        const float c_new = grow ? top - C_BELOW : c_run, f = ex2(c_run - c_new);
-        if (since != 0) move_sums(f);
+        for (int j = 0; j < 4; j++) {
+          vs[j] *= kf;
+          top = fmaxf(top, z[j] + fmaxf(log2_raw(vs[j]), -88.0f));
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        return fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+      };
+      float top = top_of();
+      if (__any_sync(0xffffffffu, top > c_run + C_SLACK) || since == 1024) {
+        float c_old = c_run, g = 1.0f;
+        if (__any_sync(0xffffffffu, fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3])) > 0x1p60f)) {   // another kappa; vs may be infinite
+          float big = 0.0f;
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            vs[j] = vs[j] == 0.0f ? 0.0f : lds_f(s_src + here + (j >> 1) * C::GRAN + (j & 1) * 32 + 64);
+            big = fmaxf(big, vs[j]);
+          }
+          const float kf_old = kf;
+          kf = kappa_of(big);
+          top = top_of();
+          // the integer sums are in units of 2^(c + kappa).  c goes down by what kappa goes up, so that a row that does not see the
+          // large values keeps its digits; by 2^80 at most, which the sums of p have room for
+          g = kf / kf_old;
+          c_old = fmaxf(c_run - fminf((float)((__float_as_int(kf_old) - __float_as_int(kf)) >> 23), 80.0f), C_NONE);
+        }
+        const float c_new = top > c_old + C_SLACK ? top - C_BELOW : c_old, f = ex2(c_run - c_new);
+        if (since != 0 || g != 1.0f) move_sums(f * g);
         l *= f;
         c_run = c_new;
       }
@@ -376,20 +395,18 @@ __global__ void __launch_bounds__(32 * Four<D>::WARPS, 1) kv_attention_four_kern
     }
     move_sums(1.0f);
 
-    // ---- the piece: outputs (2 t4 + odd) * CH .. + CH - 1 of row r, relative to c_run; 2^-40 as the sums of p, before 2^kappa:
-    // huge values of V times weights of 2^31 would leave binary32
+    // ---- the piece: outputs (2 t4 + odd) * CH .. + CH - 1 of row r in units of 2^(c_run + kappa), the sum of p in units of 2^c_run
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
     l += __shfl_xor_sync(0xffffffffu, l, 4);
-    l *= 0x1p-40f;
-    const float kappa = kf == 0.0f ? 1.0f : pow2(127 - (__float_as_int(kf) >> 23));
+    float kappa = kf == 0.0f ? -200.0f : (float)(127 - (__float_as_int(kf) >> 23));   // -200: no scale was seen, any other counts instead
     float val[CH];
 #pragma unroll
     for (int i = 0; i < CH; i++) {
       const float got = __shfl_xor_sync(0xffffffffu, odd ? o[i][0] : o[i][1], 4);
-      val[i] = ((odd ? o[i][1] : o[i][0]) + got) * 0x1p-40f * kappa;
+      val[i] = (odd ? o[i][1] : o[i][0]) + got;
     }
-    const int mine = r * D + (2 * t4 + odd) * CH;               // this thread's place in a slot: [row][D], then c and l of the rows
+    const int mine = r * D + (2 * t4 + odd) * CH;               // this thread's place in a slot: [row][D], then c, l and kappa of the rows
     bool last = true;
     if (tile0 != 0 || tile1 != it.tiles) {
       // other warps of the block that have pieces of the item
@@ -406,7 +423,7 @@ __global__ void __launch_bounds__(32 * Four<D>::WARPS, 1) kv_attention_four_kern
         if (tile0 == 0) { cp_wait<0>(); __syncwarp(); }
 #pragma unroll
         for (int i = 0; i < CH; i += 4) *reinterpret_cast<float4*>(s + mine + i) = make_float4(val[i], val[i + 1], val[i + 2], val[i + 3]);
-        if (t4 == 0 && !odd) { s[ROWS * D + r] = c_run; s[ROWS * D + ROWS + r] = l; }
+        if (t4 == 0 && !odd) { s[ROWS * D + r] = c_run; s[ROWS * D + ROWS + r] = l; s[ROWS * D + 2 * ROWS + r] = kappa; }
         __threadfence_block();
         __syncwarp();
         int before = 0;
@@ -415,17 +432,20 @@ __global__ void __launch_bounds__(32 * Four<D>::WARPS, 1) kv_attention_four_kern
         if (last) {
           __threadfence_block();
           float top = C_NONE, sum = 0.0f;
-          for (int w = warp0; w <= warp1; w++) top = fmaxf(top, slot_of(w)[ROWS * D + r]);
+          for (int w = warp0; w <= warp1; w++) {
+            top = fmaxf(top, slot_of(w)[ROWS * D + r]);
+            kappa = fmaxf(kappa, slot_of(w)[ROWS * D + 2 * ROWS + r]);
+          }
 #pragma unroll
           for (int i = 0; i < CH; i++) val[i] = 0.0f;
           for (int w = warp0; w <= warp1; w++) {
             const float* x = slot_of(w);
-            const float f = ex2(x[ROWS * D + r] - top);
+            const float f = ex2(x[ROWS * D + r] - top), h = f * ex2(x[ROWS * D + 2 * ROWS + r] - kappa);
             sum = fmaf(x[ROWS * D + ROWS + r], f, sum);
 #pragma unroll
             for (int i = 0; i < CH; i += 4) {
               const float4 y = *reinterpret_cast<const float4*>(x + mine + i);
-              val[i] = fmaf(y.x, f, val[i]); val[i + 1] = fmaf(y.y, f, val[i + 1]); val[i + 2] = fmaf(y.z, f, val[i + 2]); val[i + 3] = fmaf(y.w, f, val[i + 3]);
+              val[i] = fmaf(y.x, h, val[i]); val[i + 1] = fmaf(y.y, h, val[i + 1]); val[i + 2] = fmaf(y.z, h, val[i + 2]); val[i + 3] = fmaf(y.w, h, val[i + 3]);
             }
           }
           c_run = top; l = sum;
@@ -439,7 +459,7 @@ __global__ void __launch_bounds__(32 * Four<D>::WARPS, 1) kv_attention_four_kern
         float* s = piece((int)blockIdx.x);
 #pragma unroll
         for (int i = 0; i < CH; i += 4) __stcg(reinterpret_cast<float4*>(s + mine + i), make_float4(val[i], val[i + 1], val[i + 2], val[i + 3]));
-        if (t4 == 0 && !odd) { __stcg(s + ROWS * D + r, c_run); __stcg(s + ROWS * D + ROWS + r, l); }
+        if (t4 == 0 && !odd) { __stcg(s + ROWS * D + r, c_run); __stcg(s + ROWS * D + ROWS + r, l); __stcg(s + ROWS * D + 2 * ROWS + r, kappa); }
         __threadfence();
         __syncwarp();
         uint32_t before = 0;
@@ -449,18 +469,21 @@ __global__ void __launch_bounds__(32 * Four<D>::WARPS, 1) kv_attention_four_kern
           __threadfence();
           if (lane == 0) a.counters[run0] = 0;
           float top = C_NONE, sum = 0.0f;
-          for (int c = run0; c <= run1; c++) top = fmaxf(top, __ldcg(piece(c) + ROWS * D + r));
+          for (int c = run0; c <= run1; c++) {
+            top = fmaxf(top, __ldcg(piece(c) + ROWS * D + r));
+            kappa = fmaxf(kappa, __ldcg(piece(c) + ROWS * D + 2 * ROWS + r));
+          }
 #pragma unroll
           for (int i = 0; i < CH; i++) val[i] = 0.0f;
 #pragma unroll 2
           for (int c = run0; c <= run1; c++) {
             const float* x = piece(c);
-            const float f = ex2(__ldcg(x + ROWS * D + r) - top);
+            const float f = ex2(__ldcg(x + ROWS * D + r) - top), h = f * ex2(__ldcg(x + ROWS * D + 2 * ROWS + r) - kappa);
             sum = fmaf(__ldcg(x + ROWS * D + ROWS + r), f, sum);
 #pragma unroll
             for (int i = 0; i < CH; i += 4) {
               const float4 y = __ldcg(reinterpret_cast<const float4*>(x + mine + i));
-              val[i] = fmaf(y.x, f, val[i]); val[i + 1] = fmaf(y.y, f, val[i + 1]); val[i + 2] = fmaf(y.z, f, val[i + 2]); val[i + 3] = fmaf(y.w, f, val[i + 3]);
+              val[i] = fmaf(y.x, h, val[i]); val[i + 1] = fmaf(y.y, h, val[i + 1]); val[i + 2] = fmaf(y.z, h, val[i + 2]); val[i + 3] = fmaf(y.w, h, val[i + 3]);
             }
           }
           l = sum;
@@ -468,14 +491,13 @@ __global__ void __launch_bounds__(32 * Four<D>::WARPS, 1) kv_attention_four_kern
       }
     }
     if (last && r < rows_here) {
-      const float inv = l == 0.0f ? 0.0f : P_UNIT;
+      const float up = pow2((int)fmaxf(kappa, -126.0f)), d = l == 0.0f ? 1.0f : l;
       int t;
       float* dst = a.out + row_offset(a, it.b, it.head, it.rb * ROWS + r, a.ld_o, D, t) + (2 * t4 + odd) * CH;
 #pragma unroll
-      for (int i = 0; i < CH; i += 4) {
-        const float d = l == 0.0f ? 1.0f : l;
-        *reinterpret_cast<float4*>(dst + i) = make_float4(val[i] / d * inv, val[i + 1] / d * inv, val[i + 2] / d * inv, val[i + 3] / d * inv);
-      }
+      for (int i = 0; i < CH; i++) val[i] = l == 0.0f ? 0.0f : val[i] * P_UNIT / d * up;
+#pragma unroll
+      for (int i = 0; i < CH; i += 4) *reinterpret_cast<float4*>(dst + i) = make_float4(val[i], val[i + 1], val[i + 2], val[i + 3]);
     }
     at += tile1 - tile0;
     left -= tile1 - tile0;

@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 
 from gpu_util import Guarded
-from test_gpu_kv_cache import Setup, attention_bound, attention_rows, random_tree
+from test_gpu_kv_cache import Setup, attention_bound, attention_rows, check_attention, random_tree
 
 pytestmark = pytest.mark.gpu
 
@@ -187,3 +187,32 @@ def test_block_with_a_padded_batch(ctx, tree):
             graph = ctx.graph_end()
     ctx.graph_destroy(graph)
     cache.close()
+
+
+# ------------------------------------------------------------------------------------------------ operands of any magnitude
+MAGNITUDES = [(1e37, 1e37), (1e-35, 1e-35), (1e-36, 1e3), (1e-30, 1e12), (1e-20, 1e20), (1, 1e37), (1e37, 1), (1e3, 1e-36)]
+
+
+@pytest.mark.parametrize("T,dim", [(1, 64), (1, 128), (9, 64), (9, 128)])
+def test_attention_over_values_of_any_magnitude(ctx, T, dim):
+    """V near both ends of binary32, changing from the first tokens to the later ones and from token to token."""
+    n = 300
+    S = Setup(ctx, 1, n + T, 32, 2, dim)
+    S.fill([n + T])
+    q = S.rng.standard_normal((1, T, 4, dim)).astype(np.float32)
+    plain = [a.copy() for a in S.scales]
+    pos = np.arange(n + T)
+    page, row = S.table[0, pos // S.page], pos % S.page
+    for a, b in MAGNITUDES:
+        for which in (pos < 32, pos % 2 == 0, pos < 200):
+            S.scales[1][:] = plain[1]
+            S.scales[1][page, :, row] *= np.where(which, a, b).astype(np.float32)[:, None]
+            S.upload()
+            check_attention(S, q, [n], None, None, dim ** -0.5)
+    # the largest values there are, in one sequence that the whole GPU shares
+    S = Setup(ctx, 1, 6000 + T, 64, 2, dim)
+    S.codes[1][:], S.scales[1][:] = 127, np.float32(2.6e36)
+    S.codes[0][:] = np.clip(np.round(S.rng.standard_normal(S.codes[0].shape) * 42), -127, 127)
+    S.scales[0][:] = 0.02
+    S.upload()
+    check_attention(S, q, [6000], None, None, dim ** -0.5)
