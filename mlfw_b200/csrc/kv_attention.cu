@@ -31,6 +31,9 @@ __device__ __forceinline__ uint32_t v_at(int t, int c) {
 // they are converted, scaled and moved to binary32.  c = top - 26 leaves 5.5 bits before a larger weight (below 2^32) moves it.
 // Scales of V are taken relative to a power of two 2^kappa, that of the first tile's largest until one 2^60 times as large comes, so
 // that neither tiny nor huge values leave binary32 anywhere on the way: 2^kappa meets the quotient of the two sums at the end.
+// Scores more than 2^20 from zero, where binary32 has no room for a difference of a few units, are taken relative to m, a score of
+// the row that is, so c stays small.  m, kappa and c change in a branch that is entered when a row's largest weight
+// leaves its window (`limit`), on every tile once m is not zero.
 //
 // About 550 instructions per warp and 32 tokens of 128 dimensions, 500 of 64 (conversion of the codes to binary16 for
 // m16n8k16, tried first, took 1300).  Bound by reading the cache: 5.4 TB/s of the 6.5 measured at 48 sequences of up to 6000
@@ -45,7 +48,7 @@ template <int D>
 struct Four {
   static constexpr int WARPS = D == 128 ? 8 : 12, STAGES = D == 128 ? 2 : 3;
   static constexpr int GRAN = 2 * KV_TILE * D + 2 * KV_TILE * 4, TILE = 2 * GRAN;   // sixteen tokens: K and V codes, K and V scales
-  static constexpr int RING = WARPS * STAGES * TILE, SLOT = 4 * (D + 3) * 4, SMEM = RING + WARPS * SLOT;
+  static constexpr int RING = WARPS * STAGES * TILE, SLOT = 4 * (D + 4) * 4, SMEM = RING + WARPS * SLOT;
 };
 __device__ __forceinline__ void imma(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {   // s8 x s8
   asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -82,6 +85,44 @@ struct Item {
     vis = kv_visible(a.g, first, n, a.group, ROWS, rb, a.tree != nullptr);
   }
 };
+
+// Pieces first .. last of an item, at(i) each, added up in that order: outputs `mine` of row r in units of 2^(m + c + kappa), l in units of
+// 2^(m + c); behind the outputs of a piece stand c, l, kappa and m of its rows.  `ld` loads four floats.  A chain of latencies: four pieces
+// at a time (one sequence of 2000 tokens, 12 heads of 64, joined between blocks: 11.3 us, two at a time in the second loop 11.7).
+template <int D, typename At, typename Ld>
+__device__ __forceinline__ void join_pieces(int first, int last, At at, Ld ld, int r, int mine, float (&val)[D / 8], float4& row) {
+  float top = C_NONE, kappa = -200.0f, far = C_NONE, sum = 0.0f;   // far: the largest m of a piece that has seen something
+  bool some = false;
+#pragma unroll 4
+  for (int i = first; i <= last; i++) {
+    const float4 x = ld(at(i) + 4 * D + 4 * r);
+    top = fmaxf(top, x.x);
+    kappa = fmaxf(kappa, x.z);
+    far = fmaxf(far, x.x > C_SEEN ? x.w : C_NONE);
+    some |= x.w != 0.0f;
+  }
+  if (__builtin_expect(some, 0)) {
+    top = C_NONE;
+    for (int i = first; i <= last; i++) {
+      const float4 x = ld(at(i) + 4 * D + 4 * r);
+      top = fmaxf(top, x.x + (x.w - far));
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < D / 8; i++) val[i] = 0.0f;
+#pragma unroll 4
+  for (int i = first; i <= last; i++) {
+    const float4 x = ld(at(i) + 4 * D + 4 * r);
+    const float e = (some ? x.x + (x.w - far) : x.x) - top, f = ex2(e + (x.z - kappa));
+    sum = fmaf(x.y, ex2(e), sum);
+#pragma unroll
+    for (int k = 0; k < D / 8; k += 4) {
+      const float4 v = ld(at(i) + mine + k);
+      val[k] = fmaf(v.x, f, val[k]); val[k + 1] = fmaf(v.y, f, val[k + 1]); val[k + 2] = fmaf(v.z, f, val[k + 2]); val[k + 3] = fmaf(v.w, f, val[k + 3]);
+    }
+  }
+  row = make_float4(top, sum, kappa, some && far > C_SEEN ? far : 0.0f);
+}
 
 // Every warp has a run of its own, a part of the block's, and a ring that it keeps full across the items of its run; the warps
 // never wait for one another.  Results of an item that several warps of the block worked on are joined by the last of them
@@ -260,7 +301,7 @@ __global__ void __launch_bounds__(32 * Four<D>::WARPS, 1) kv_attention_four_kern
     }
 
     int acc[CH][4];
-    float o[CH][2], c_run = C_NONE, l = 0.0f, kf = 0.0f;        // kf: 2^-kappa, 0 until a tile has a scale
+    float o[CH][2], c_run = C_NONE, limit = NEG_INF, m = 0.0f, l = 0.0f, kf = 0.0f;   // kf: 2^-kappa, 0 until a tile has a scale
 #pragma unroll
     for (int i = 0; i < CH; i++) { acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0; o[i][0] = o[i][1] = 0.0f; }
     int since = 0;                                              // tiles in the integer sums
@@ -321,21 +362,20 @@ __global__ void __launch_bounds__(32 * Four<D>::WARPS, 1) kv_attention_four_kern
         return big > 0.0f ? pow2(127 - min(max(__float_as_int(big) >> 23, 1), 253)) : 0.0f;
       };
       if (kf == 0.0f) kf = kappa_of(fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3])));
-      auto top_of = [&] {                                       // scales relative to kappa, and the row's largest weight in units of log2
+      auto top_of = [&] {                                       // the row's largest weight in units of log2
         float top = NEG_INF;
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-          vs[j] *= kf;
-          top = fmaxf(top, z[j] + fmaxf(log2_raw(vs[j]), -88.0f));
-        }
+        for (int j = 0; j < 4; j++) top = fmaxf(top, z[j] + fmaxf(log2_raw(vs[j]), -88.0f));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         return fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
       };
+#pragma unroll
+      for (int j = 0; j < 4; j++) vs[j] *= kf;
       float top = top_of();
-      if (__any_sync(0xffffffffu, top > c_run + C_SLACK) || since == 1024) {
-        float c_old = c_run, g = 1.0f;
-        if (__any_sync(0xffffffffu, fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3])) > 0x1p60f)) {   // another kappa; vs may be infinite
+      if (__any_sync(0xffffffffu, top > limit) || since == 1024) {
+        float c_old = c_run, lower = 0.0f, g = 1.0f;
+        if (__builtin_expect(__any_sync(0xffffffffu, fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3])) > 0x1p60f), 0)) {   // another kappa; vs may be infinite
           float big = 0.0f;
 #pragma unroll
           for (int j = 0; j < 4; j++) {
@@ -344,16 +384,36 @@ __global__ void __launch_bounds__(32 * Four<D>::WARPS, 1) kv_attention_four_kern
           }
           const float kf_old = kf;
           kf = kappa_of(big);
+#pragma unroll
+          for (int j = 0; j < 4; j++) vs[j] *= kf;
           top = top_of();
           // the integer sums are in units of 2^(c + kappa).  c goes down by what kappa goes up, so that a row that does not see the
           // large values keeps its digits; by 2^80 at most, which the sums of p have room for
-          g = kf / kf_old;
-          c_old = fmaxf(c_run - fminf((float)((__float_as_int(kf_old) - __float_as_int(kf)) >> 23), 80.0f), C_NONE);
+          const int up = (__float_as_int(kf_old) - __float_as_int(kf)) >> 23;
+          g = up > 126 ? 0.0f : pow2(-up);
+          lower = fminf((float)up, 80.0f);
         }
-        const float c_new = top > c_old + C_SLACK ? top - C_BELOW : c_old, f = ex2(c_run - c_new);
+        if (__builtin_expect(__any_sync(0xffffffffu, m != 0.0f || (fabsf(top) > FAR && top > NEG_INF)), 0)) {
+#pragma unroll
+          for (int j = 0; j < 4; j++) z[j] -= m;
+          top = top_of();
+          for (int k = 0; k < 8; k++) {                         // each round leaves a rounding of the one before: 2^-23 of it
+            const bool far = top > FAR || (top < -FAR && top > NEG_INF && c_old < C_SEEN);
+            if (!__any_sync(0xffffffffu, far)) break;
+            const float d = far ? top : 0.0f;
+#pragma unroll
+            for (int j = 0; j < 4; j++) z[j] -= d;
+            m += d;
+            c_old = fmaxf(c_old - d, C_NONE);
+            top = top_of();
+          }
+        }
+        const float c_low = fmaxf(c_old - lower, C_NONE);
+        const float c_new = top > c_low + C_SLACK ? top - C_BELOW : c_low, f = ex2(c_old - c_new);
         if (since != 0 || g != 1.0f) move_sums(f * g);
         l *= f;
         c_run = c_new;
+        limit = m != 0.0f || c_new < C_SEEN ? NEG_INF : c_new + C_SLACK;
       }
       since++;
       float sum = 0.0f;
@@ -395,18 +455,18 @@ __global__ void __launch_bounds__(32 * Four<D>::WARPS, 1) kv_attention_four_kern
     }
     move_sums(1.0f);
 
-    // ---- the piece: outputs (2 t4 + odd) * CH .. + CH - 1 of row r in units of 2^(c_run + kappa), the sum of p in units of 2^c_run
+    // ---- the piece: outputs (2 t4 + odd) * CH .. + CH - 1 of row r in units of 2^(m + c_run + kappa), the sum of p in units of 2^(m + c_run)
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
     l += __shfl_xor_sync(0xffffffffu, l, 4);
-    float kappa = kf == 0.0f ? -200.0f : (float)(127 - (__float_as_int(kf) >> 23));   // -200: no scale was seen, any other counts instead
+    float4 row = make_float4(c_run, l, kf == 0.0f ? -200.0f : (float)(127 - (__float_as_int(kf) >> 23)), m);   // kappa -200: no scale was seen
     float val[CH];
 #pragma unroll
     for (int i = 0; i < CH; i++) {
       const float got = __shfl_xor_sync(0xffffffffu, odd ? o[i][0] : o[i][1], 4);
       val[i] = (odd ? o[i][1] : o[i][0]) + got;
     }
-    const int mine = r * D + (2 * t4 + odd) * CH;               // this thread's place in a slot: [row][D], then c, l and kappa of the rows
+    const int mine = r * D + (2 * t4 + odd) * CH;               // this thread's place in a slot: [row][D], then (c, l, kappa, m) of the rows
     bool last = true;
     if (tile0 != 0 || tile1 != it.tiles) {
       // other warps of the block that have pieces of the item
@@ -423,7 +483,7 @@ __global__ void __launch_bounds__(32 * Four<D>::WARPS, 1) kv_attention_four_kern
         if (tile0 == 0) { cp_wait<0>(); __syncwarp(); }
 #pragma unroll
         for (int i = 0; i < CH; i += 4) *reinterpret_cast<float4*>(s + mine + i) = make_float4(val[i], val[i + 1], val[i + 2], val[i + 3]);
-        if (t4 == 0 && !odd) { s[ROWS * D + r] = c_run; s[ROWS * D + ROWS + r] = l; s[ROWS * D + 2 * ROWS + r] = kappa; }
+        if (t4 == 0 && !odd) *reinterpret_cast<float4*>(s + ROWS * D + 4 * r) = row;
         __threadfence_block();
         __syncwarp();
         int before = 0;
@@ -431,24 +491,7 @@ __global__ void __launch_bounds__(32 * Four<D>::WARPS, 1) kv_attention_four_kern
         last = __shfl_sync(0xffffffffu, before, 0) == warp1 - warp0;
         if (last) {
           __threadfence_block();
-          float top = C_NONE, sum = 0.0f;
-          for (int w = warp0; w <= warp1; w++) {
-            top = fmaxf(top, slot_of(w)[ROWS * D + r]);
-            kappa = fmaxf(kappa, slot_of(w)[ROWS * D + 2 * ROWS + r]);
-          }
-#pragma unroll
-          for (int i = 0; i < CH; i++) val[i] = 0.0f;
-          for (int w = warp0; w <= warp1; w++) {
-            const float* x = slot_of(w);
-            const float f = ex2(x[ROWS * D + r] - top), h = f * ex2(x[ROWS * D + 2 * ROWS + r] - kappa);
-            sum = fmaf(x[ROWS * D + ROWS + r], f, sum);
-#pragma unroll
-            for (int i = 0; i < CH; i += 4) {
-              const float4 y = *reinterpret_cast<const float4*>(x + mine + i);
-              val[i] = fmaf(y.x, h, val[i]); val[i + 1] = fmaf(y.y, h, val[i + 1]); val[i + 2] = fmaf(y.z, h, val[i + 2]); val[i + 3] = fmaf(y.w, h, val[i + 3]);
-            }
-          }
-          c_run = top; l = sum;
+          join_pieces<D>(warp0, warp1, slot_of, [](const float* x) { return *reinterpret_cast<const float4*>(x); }, r, mine, val, row);
         }
       }
       // the same between blocks, through memory
@@ -459,7 +502,7 @@ __global__ void __launch_bounds__(32 * Four<D>::WARPS, 1) kv_attention_four_kern
         float* s = piece((int)blockIdx.x);
 #pragma unroll
         for (int i = 0; i < CH; i += 4) __stcg(reinterpret_cast<float4*>(s + mine + i), make_float4(val[i], val[i + 1], val[i + 2], val[i + 3]));
-        if (t4 == 0 && !odd) { __stcg(s + ROWS * D + r, c_run); __stcg(s + ROWS * D + ROWS + r, l); __stcg(s + ROWS * D + 2 * ROWS + r, kappa); }
+        if (t4 == 0 && !odd) __stcg(reinterpret_cast<float4*>(s + ROWS * D + 4 * r), row);
         __threadfence();
         __syncwarp();
         uint32_t before = 0;
@@ -468,34 +511,16 @@ __global__ void __launch_bounds__(32 * Four<D>::WARPS, 1) kv_attention_four_kern
         if (last) {
           __threadfence();
           if (lane == 0) a.counters[run0] = 0;
-          float top = C_NONE, sum = 0.0f;
-          for (int c = run0; c <= run1; c++) {
-            top = fmaxf(top, __ldcg(piece(c) + ROWS * D + r));
-            kappa = fmaxf(kappa, __ldcg(piece(c) + ROWS * D + 2 * ROWS + r));
-          }
-#pragma unroll
-          for (int i = 0; i < CH; i++) val[i] = 0.0f;
-#pragma unroll 2
-          for (int c = run0; c <= run1; c++) {
-            const float* x = piece(c);
-            const float f = ex2(__ldcg(x + ROWS * D + r) - top), h = f * ex2(__ldcg(x + ROWS * D + 2 * ROWS + r) - kappa);
-            sum = fmaf(__ldcg(x + ROWS * D + ROWS + r), f, sum);
-#pragma unroll
-            for (int i = 0; i < CH; i += 4) {
-              const float4 y = __ldcg(reinterpret_cast<const float4*>(x + mine + i));
-              val[i] = fmaf(y.x, h, val[i]); val[i + 1] = fmaf(y.y, h, val[i + 1]); val[i + 2] = fmaf(y.z, h, val[i + 2]); val[i + 3] = fmaf(y.w, h, val[i + 3]);
-            }
-          }
-          l = sum;
+          join_pieces<D>(run0, run1, piece, [](const float* x) { return __ldcg(reinterpret_cast<const float4*>(x)); }, r, mine, val, row);
         }
       }
     }
     if (last && r < rows_here) {
-      const float up = pow2((int)fmaxf(kappa, -126.0f)), d = l == 0.0f ? 1.0f : l;
+      const float up = pow2((int)fmaxf(row.z, -126.0f)), inv = row.y == 0.0f ? 0.0f : 1.0f / row.y;
       int t;
       float* dst = a.out + row_offset(a, it.b, it.head, it.rb * ROWS + r, a.ld_o, D, t) + (2 * t4 + odd) * CH;
 #pragma unroll
-      for (int i = 0; i < CH; i++) val[i] = l == 0.0f ? 0.0f : val[i] * P_UNIT / d * up;
+      for (int i = 0; i < CH; i++) val[i] = val[i] * P_UNIT * inv * up;
 #pragma unroll
       for (int i = 0; i < CH; i += 4) *reinterpret_cast<float4*>(dst + i) = make_float4(val[i], val[i + 1], val[i + 2], val[i + 3]);
     }

@@ -49,6 +49,8 @@ namespace {
 constexpr float NEG_INF = -__builtin_huge_valf();
 constexpr float P_UNIT = 0x1p-22f;       // sums of p are held times this: up to 2^24 keys of weight 2^120 stay finite
 constexpr float C_NONE = -3.0e38f;       // c of a row that has seen nothing: finite, so that differences with it are numbers
+constexpr float C_SEEN = -1.0e38f;       // ... and of a row that has seen something it is above this
+constexpr float FAR = 0x1p20f;           // scores are taken relative to a score of the row when they are further from zero
 
 __device__ __forceinline__ float ex2(float x) {
   float r;

@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 
 from gpu_util import Guarded
-from test_gpu_kv_cache import Setup, attention_bound, attention_rows, check_attention, random_tree
+from test_gpu_kv_cache import Setup, attention_bound, attention_rows, check_attention, random_tree, run_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -216,3 +216,29 @@ def test_attention_over_values_of_any_magnitude(ctx, T, dim):
     S.scales[0][:] = 0.02
     S.upload()
     check_attention(S, q, [6000], None, None, dim ** -0.5)
+
+
+@pytest.mark.parametrize("T,dim,n", [(1, 64, 200), (1, 128, 5000), (9, 64, 3000), (9, 128, 150)])
+def test_attention_scores_of_any_magnitude(ctx, T, dim, n):
+    """Two equal keys lead all others by more than any weight survives, at opposite ends of the sequence: their values' mean, however
+    large the scores are and whichever sign they have.  One exact addition and one division: off by a few roundings."""
+    S = Setup(ctx, 1, n + T, 32, 1, dim)
+    S.fill([n + T])
+    plain = [a.copy() for a in S.codes + S.scales]
+    sign = S.rng.choice([-1, 1], dim)
+    q = np.broadcast_to(sign * S.rng.uniform(0.5, 2, dim), (1, T, 2, dim)).astype(np.float32)
+    lead = [5, n - 9]
+    page, row = S.table[0, lead[0] // 32], lead[0] % 32
+    page2, row2 = S.table[0, lead[1] // 32], lead[1] % 32
+    want = np.mean([S.codes[1][p, 0, r].astype(np.float64) * S.scales[1][p, 0, r] for p, r in ((page, row), (page2, row2))], axis=0)
+    vmax = np.max(np.abs(want)) * 2
+    for negative in (False, True):
+        for f_q, f_k in ((1e5, 1), (1e7, 1), (1e9, 1), (1e13, 1), (1e20, 1e10), (1e36, 1), (1, 1e7), (1, 1e25), (1, 1e34)):
+            S.codes[0][:], S.scales[0][:] = plain[0], np.float32(0.02 * f_k)
+            if negative:                                          # every score far below zero
+                S.codes[0][:] = -sign * (100 + S.rng.integers(0, 28, S.codes[0].shape[:-1])[..., None])
+            for p, r in ((page, row), (page2, row2)):
+                S.codes[0][p, 0, r] = sign * (-60 if negative else 127)
+            S.upload()
+            got = run_attention(S, (q * np.float32(f_q)).astype(np.float32), [n], None, None, dim ** -0.5)
+            assert np.abs(got - want).max() <= 8 * 2.0**-24 * vmax, (negative, f_q, f_k, np.abs(got - want).max() / vmax)
