@@ -28,7 +28,11 @@ __device__ __forceinline__ uint32_t v_at(int t, int c) {
 // row therefore finds sum d3 code and sum d1 code, its neighbour in the odd row those of d2 and d0; each takes one of their two
 // columns after one exchange, so no score is computed twice.  Sums are 32-bit integers and exact: scores carry the rounding of
 // adding the digits, and the outputs are added up without rounding until a row's c changes (or 2^15 tokens have passed), when
-// they are converted, scaled and moved to binary32.  c = top - 26 leaves 5.5 bits before a larger weight (below 2^32) moves it.
+// they are converted, scaled and moved to binary32.  c = floor(top) - 28, an integer, so that moving is exact; 3.75 bits are left
+// before a larger weight (below 2^32) moves it.  The unit is thus 2^-28 of the row's largest weight or less.  Many weights below it
+// must neither vanish nor count double, so a weight is rounded down after adding `dither` in (0, 1), which goes round by the golden
+// ratio from tile to tile: over many tokens a unit's share of all weights is kept, and what is left of a token's rounding is noise.
+// The sum of p carries the rounding of each addition into the next one for the same reason.
 // Scales of V are taken relative to a power of two 2^kappa, that of the first tile's largest until one 2^60 times as large comes, so
 // that neither tiny nor huge values leave binary32 anywhere on the way: 2^kappa meets the quotient of the two sums at the end.
 // Scores more than 2^20 from zero, where binary32 has no room for a difference of a few units, are taken relative to m, a score of
@@ -131,7 +135,7 @@ template <int D>
 __global__ void __launch_bounds__(32 * Four<D>::WARPS, 1) kv_attention_four_kernel(const AttnArgs a, int row_blocks) {
   using C = Four<D>;
   constexpr int ROWS = 4, WARPS = C::WARPS, ST = C::STAGES, KS = D / 32, CH = D / 8, W = D / 32;
-  constexpr float C_BELOW = 26.0f, C_SLACK = 31.5f;
+  constexpr float C_BELOW = 28.0f, C_SLACK = 31.75f, GOLDEN = 0.61803399f;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int arrived[WARPS];                                // pieces of an item within the block, by the first warp that has it
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, t4 = lane & 3, r = g8 >> 1, odd = g8 & 1;
@@ -301,7 +305,8 @@ __global__ void __launch_bounds__(32 * Four<D>::WARPS, 1) kv_attention_four_kern
     }
 
     int acc[CH][4];
-    float o[CH][2], c_run = C_NONE, limit = NEG_INF, m = 0.0f, l = 0.0f, kf = 0.0f;   // kf: 2^-kappa, 0 until a tile has a scale
+    float o[CH][2], c_run = C_NONE, limit = NEG_INF, m = 0.0f, l = 0.0f, l_over = 0.0f, kf = 0.0f;   // kf: 2^-kappa, 0 until a tile has a scale
+    float dither = (2 * t4 + odd) * 0.125f + 0.0625f;
 #pragma unroll
     for (int i = 0; i < CH; i++) { acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0; o[i][0] = o[i][1] = 0.0f; }
     int since = 0;                                              // tiles in the integer sums
@@ -409,9 +414,10 @@ __global__ void __launch_bounds__(32 * Four<D>::WARPS, 1) kv_attention_four_kern
           }
         }
         const float c_low = fmaxf(c_old - lower, C_NONE);
-        const float c_new = top > c_low + C_SLACK ? top - C_BELOW : c_low, f = ex2(c_old - c_new);
+        const float c_new = top > c_low + C_SLACK ? floorf(top) - C_BELOW : c_low, f = ex2(c_old - c_new);
         if (since != 0 || g != 1.0f) move_sums(f * g);
         l *= f;
+        l_over *= f;
         c_run = c_new;
         limit = m != 0.0f || c_new < C_SEEN ? NEG_INF : c_new + C_SLACK;
       }
@@ -422,10 +428,13 @@ __global__ void __launch_bounds__(32 * Four<D>::WARPS, 1) kv_attention_four_kern
       for (int j = 0; j < 4; j++) {
         const float p = ex2(z[j] - c_run);
         sum += p;
-        const uint32_t w = __float2uint_rn(p * vs[j]);
+        const uint32_t w = __float2uint_rz(fmaf(p, vs[j], (j & 1) ? 0.99999994f - dither : dither));
         t[j] = __byte_perm(w, __shfl_xor_sync(0xffffffffu, w, 4), sel);   // digits (3, 3, 1, 1) or (2, 2, 0, 0) of two neighbouring tokens
       }
-      l = fmaf(sum, P_UNIT, l);
+      dither += dither < 1.0f - GOLDEN ? GOLDEN : GOLDEN - 1.0f;
+      const float add = fmaf(sum, P_UNIT, -l_over), l_new = l + add;
+      l_over = (l_new - l) - add;                               // what the sum is above the true one
+      l = l_new;
       const uint32_t p0 = __byte_perm(t[0], t[1], 0x5410), p1 = __byte_perm(t[0], t[1], 0x7632);
       const uint32_t p2 = __byte_perm(t[2], t[3], 0x5410), p3 = __byte_perm(t[2], t[3], 0x7632);
 
@@ -456,6 +465,7 @@ __global__ void __launch_bounds__(32 * Four<D>::WARPS, 1) kv_attention_four_kern
     move_sums(1.0f);
 
     // ---- the piece: outputs (2 t4 + odd) * CH .. + CH - 1 of row r in units of 2^(m + c_run + kappa), the sum of p in units of 2^(m + c_run)
+    l -= l_over;
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
     l += __shfl_xor_sync(0xffffffffu, l, 4);

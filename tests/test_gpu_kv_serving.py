@@ -242,3 +242,44 @@ def test_attention_scores_of_any_magnitude(ctx, T, dim, n):
             S.upload()
             got = run_attention(S, (q * np.float32(f_q)).astype(np.float32), [n], None, None, dim ** -0.5)
             assert np.abs(got - want).max() <= 8 * 2.0**-24 * vmax, (negative, f_q, f_k, np.abs(got - want).max() / vmax)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("spread", [0.0, 0.3])
+def test_attention_one_key_above_many(ctx, dim, spread):
+    """One key 2^9 to 2^35 times as heavy as each of 20000 others, which one warp walks: none of the others' weight may get lost.
+
+    Many sequences over the same pages, so that a piece is nearly a whole context.  With w the weights, v the values, r the result
+    and u = 2^-24: a weight is off by its score's rounding, ten u of |z| (two terms and what combines them), ex2 (2^-21) and the
+    rounding of z - c (u times its 40 or fewer bits), which moves r by w |v - r| / sum w; its rounding to units, 2^-28 of the largest weight,
+    is noise of at most half a unit each, six deviations of which are 3 sqrt(sum v^2) units; 24 u of sum w |v| for the sums and joins.
+    """
+    B, n, page = 1300, 20000, 256
+    S = Setup(ctx, 1, n, page, 1, dim)
+    S.codes[0][:], S.scales[0][:] = 0, np.float32(0.01)
+    S.codes[0][..., 1] = S.rng.integers(-127, 128, S.codes[0].shape[:-1])
+    S.codes[1][:] = np.clip(np.round(S.rng.standard_normal(S.codes[1].shape) * 42), -127, 127)
+    S.codes[1][..., 0] = 100
+    S.scales[1][:] = np.float32(0.02)
+    at = 777
+    S.codes[0][S.table[0, at // page], 0, at % page, :2] = 127, 0
+    S.codes[1][S.table[0, at // page], 0, at % page] = S.rng.integers(-127, 128, dim)
+    S.upload()
+    bits = np.linspace(9, 35, B)
+    q = np.zeros((B, 1, 1, dim), np.float32)
+    q[:, 0, 0, 0], q[:, 0, 0, 1] = bits * np.log(2) / 1.27, spread * np.log(2) / 1.27
+    out = Guarded(ctx, (B, dim), np.float32, np.zeros((B, dim)))
+    table = ctx.to_device(np.ascontiguousarray(np.broadcast_to(S.table, (B, S.per))))
+    S.cache.attention(ctx.to_device(q), dim, B, 1, 1, table, S.per, S.dev([n - 1] * B), None, None, 1.0, out.ptr, dim)
+    got = out.download()
+    kc, vc, ks, vs = S.tokens(0, n)
+    v = vc[:, 0].astype(np.float64) * vs[:, 0, None]
+    u = 2.0**-24
+    for b in range(0, B, 13):
+        z = ks[:, 0].astype(np.float64) * (kc[:, 0].astype(np.float64) @ q[b, 0, 0].astype(np.float64))
+        w = np.exp(z - z.max())
+        total = w.sum()
+        want = w @ v / total
+        delta = 10 * u * np.abs(z) + 2.0**-21 + 40 * u
+        bound = (w * delta) @ np.abs(v - want) / total + 3 * np.sqrt((v * v).sum(0)) * 2.0**-28 / total + 24 * u * (w @ np.abs(v)) / total
+        assert (np.abs(got[b] - want) <= bound).all(), (bits[b], np.max(np.abs(got[b] - want) / bound))
