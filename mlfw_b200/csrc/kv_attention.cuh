@@ -6,11 +6,11 @@
 // The arithmetic.  A cached value is code * scale with an integer |code| <= 128.  The codes go into the tensor cores as they
 // are; queries and weights, which are binary32, are split into parts that the tensor cores take, so the result has binary32
 // accuracy and the cache is never dequantized.  Two forms:
-//   Many rows (kv_attention_umma.cu), binary16 products, two per contraction.  A query row is written in fixed point against
-//   its largest element, x = q * 2^(10 - e) with 2^e <= max|q| < 2^(e+1), and split x = hi + lo, |hi| <= 2^11 an integer,
-//   |lo| <= 1/2: 23 bits.  sum_d q_d code_d = 2^(e-10) * (sum lo code + sum hi code), in one binary32 sum with the small parts
-//   first: D / 16 steps of integers, whose roundings of the running sum stay below the D that an ordinary binary32 sum has.
-//   A weight is its rounding to binary16 and the rounding of what is left: 22 bits.
+//   Many rows (kv_attention_umma.cu), binary16 products, two per contraction.  A query row is scaled by a power of two to
+//   x = q * 2^(14 - e) with 2^e <= max|q| < 2^(e+1), and an element is its rounding to binary16 and the rounding of what is left: 22
+//   bits of its own down to 2^-17 of the row's largest, 2^-40 of the largest below that (a fixed point against the largest, tried
+//   first, left an element beside one 2000 times as large 11 bits).  sum_d q_d code_d = 2^(e-14) * (sum lo code + sum hi code), in one
+//   binary32 sum with the small parts first.  A weight is split the same way, the largest of a tile's at 2^10.
 //   Few rows (kv_attention.cu), integer products: queries and weights as 32-bit fixed-point numbers in four 8-bit digits, sums
 //   in 32-bit integers, exact.
 // Either way a score carries the rounding of q (2^-23 of the row's largest element or better) and the one of adding the
@@ -94,12 +94,7 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {   // lo in th
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-// x = hi + lo for |x| <= 2^11: hi an integer (1.5 * 2^23 trick), lo exact.
-__device__ __forceinline__ void split_whole(float x, float& hi, float& lo) {
-  hi = __fsub_rn(__fadd_rn(x, 12582912.0f), 12582912.0f);
-  lo = __fsub_rn(x, hi);
-}
-// Two weights as binary16 halves: the rounded values and what is left of them (exact before its own rounding).
+// Two numbers as binary16 halves: the rounded values and what is left of them (exact before its own rounding).
 __device__ __forceinline__ void split_f16(float x0, float x1, uint32_t& hi, uint32_t& lo) {
   hi = pack_f16(x0, x1);
   float y0, y1;

@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv_attention_many_kernel(cons
     };
     while (alive && w.open(a, mp.row_blocks)) {
       if (tid == 0 && (w.first < 0 || w.first + w.n > (a.g.max_pages << a.g.page_shift))) atomicOr(a.status, STATUS_BAD_INDEX);
-      // ---- the query row: this thread's quarter of it, in fixed point
+      // ---- the query row: this thread's quarter of it, below 2^15, in two binary16 parts
       float rs;
       int row_t;
       uint64_t row_seen;
@@ -278,18 +278,21 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv_attention_many_kernel(cons
         const bool finite = top < 0x7f800000u;
         const int ex = max((int)(top >> 23), 24) - 127;
         // rs is kept positive, so that a masked x = -Inf stays -Inf: a negative scale turns the query's sign, a zero one zeroes it
-        const float up = a.scale_log2e == 0.0f ? 0.0f : copysignf(pow2(10 - ex), a.scale_log2e);
-        rs = finite ? fmaxf(fabsf(a.scale_log2e) * pow2(ex - 10), 1e-37f) : __int_as_float(0x7fc00000);
+        const float up = a.scale_log2e == 0.0f ? 0.0f : copysignf(pow2(14 - ex), a.scale_log2e);
+        rs = finite ? fmaxf(fabsf(a.scale_log2e) * pow2(ex - 14), 1e-37f) : __int_as_float(0x7fc00000);
 #pragma unroll
         for (int i = 0; i < QD / 4; i += 2) {                    // eight dimensions: 16 bytes of either half, in the order of staged K
-          float h[8], l[8];
+          uint32_t h[4], l[4];
           const float y[8] = {x[i].x, x[i].y, x[i].z, x[i].w, x[i + 1].x, x[i + 1].y, x[i + 1].z, x[i + 1].w};
 #pragma unroll
-          for (int c = 0; c < 8; c++) split_whole(finite ? y[c] * up : 0.0f, h[c], l[c]);
+          for (int c = 0; c < 4; c++) {
+            const int e = (c & 1) + 4 * (c >> 1);
+            split_f16(finite ? y[e] * up : 0.0f, finite ? y[e + 2] * up : 0.0f, h[c], l[c]);
+          }
           const int dim = cg * QD + i * 4;
           const uint32_t to = sm_base + (dim >> 6) * C::Q_BLOCK + sw128(row, (dim & 63) * 2);
-          sts128(to + C::QHI, pack_f16(h[0], h[2]), pack_f16(h[1], h[3]), pack_f16(h[4], h[6]), pack_f16(h[5], h[7]));
-          sts128(to + C::QLO, pack_f16(l[0], l[2]), pack_f16(l[1], l[3]), pack_f16(l[4], l[6]), pack_f16(l[5], l[7]));
+          sts128(to + C::QHI, h[0], h[1], h[2], h[3]);
+          sts128(to + C::QLO, l[0], l[1], l[2], l[3]);
         }
         fence_proxy();                                           // the tensor cores read what the threads wrote
         __syncwarp();

@@ -283,3 +283,38 @@ def test_attention_one_key_above_many(ctx, dim, spread):
         delta = 10 * u * np.abs(z) + 2.0**-21 + 40 * u
         bound = (w * delta) @ np.abs(v - want) / total + 3 * np.sqrt((v * v).sum(0)) * 2.0**-28 / total + 24 * u * (w @ np.abs(v)) / total
         assert (np.abs(got[b] - want) <= bound).all(), (bits[b], np.max(np.abs(got[b] - want) / bound))
+
+
+@pytest.mark.parametrize("T,dim", [(1, 64), (1, 128), (40, 64), (40, 128), (130, 128)])
+def test_attention_beside_a_strong_channel(ctx, T, dim):
+    """One channel of the queries far above the others, on which K is zero: the others keep their digits.
+
+    K has four channels that are not zero.  With u = 2^-24, a score is off by 16 u of sum |q k|: four products and their sum, eight
+    roundings that combine and scale it, four u for a query element in two binary16 parts; in the kernel for few rows an element is
+    held to 2^-31 of the row's largest as well.  That moves the result by sum w |v - r| delta / sum w, with 2^-21 for ex2 and u times the
+    bits between a score and the largest; 22 bits of a weight and (n / 64 + 24) u of sum w |v| for the sums.
+    """
+    n = 260
+    S = Setup(ctx, 1, n + T, 32, 2, dim)
+    S.fill([n + T])
+    S.codes[0][..., 4:] = 0
+    S.upload()
+    kc, vc, ks, vs = S.tokens(0, n + T)
+    u = 2.0**-24
+    few = T * 2 <= 36
+    for strong in (1.0, 200.0, 2000.0, 1e4) + (() if few else (1e5, 1e7)):
+        q = (S.rng.standard_normal((1, T, 4, dim)) * 6).astype(np.float32)
+        q[..., dim - 1] = strong
+        got = run_attention(S, q, [n], None, None, 0.125)
+        for t in range(T):
+            for h in range(4):
+                g, m = h // 2, n + t + 1
+                x, k = q[0, t, h].astype(np.float64), kc[:m, g].astype(np.float64) * ks[:m, g, None]
+                v = vc[:m, g].astype(np.float64) * vs[:m, g, None]
+                z = 0.125 * (k @ x)
+                w = np.exp(z - z.max())
+                r = w @ v / w.sum()
+                held = np.abs(k).sum(1) * strong * 2.0**-31 if few else 0
+                delta = 0.125 * (16 * u * (np.abs(k) @ np.abs(x)) + held) + 2.0**-21 + u * (z.max() - z + 16)
+                bound = (w * delta) @ np.abs(v - r) / w.sum() + (4 * u + (m / 64 + 24) * u) * (w @ np.abs(v)) / w.sum()
+                assert (np.abs(got[0, t, h] - r) <= bound).all(), (strong, t, h, np.max(np.abs(got[0, t, h] - r) / bound))
