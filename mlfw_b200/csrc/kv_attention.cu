@@ -135,6 +135,7 @@ template <int D>
 __global__ void __launch_bounds__(32 * Four<D>::WARPS, 1) kv_attention_four_kernel(const AttnArgs a, int row_blocks) {
   using C = Four<D>;
   constexpr int ROWS = 4, WARPS = C::WARPS, ST = C::STAGES, KS = D / 32, CH = D / 8, W = D / 32;
+  constexpr float P_UNIT = 0x1p-22f;                            // sums of p are held times this: 2^24 keys of weight 2^120 stay finite
   constexpr float C_BELOW = 28.0f, C_SLACK = 31.75f, GOLDEN = 0.61803399f;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int arrived[WARPS];                                // pieces of an item within the block, by the first warp that has it

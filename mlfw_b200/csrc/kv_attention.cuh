@@ -10,7 +10,7 @@
 //   x = q * 2^(14 - e) with 2^e <= max|q| < 2^(e+1), and an element is its rounding to binary16 and the rounding of what is left: 22
 //   bits of its own down to 2^-17 of the row's largest, 2^-40 of the largest below that (a fixed point against the largest, tried
 //   first, left an element beside one 2000 times as large 11 bits).  sum_d q_d code_d = 2^(e-14) * (sum lo code + sum hi code), in one
-//   binary32 sum with the small parts first.  A weight is split the same way, the largest of a tile's at 2^10.
+//   binary32 sum with the small parts first.  A weight is split the same way, the largest below 2^15.
 //   Few rows (kv_attention.cu), integer products: queries and weights as 32-bit fixed-point numbers in four 8-bit digits, sums
 //   in 32-bit integers, exact.
 // Either way a score carries the rounding of q (2^-23 of the row's largest element or better) and the one of adding the
@@ -18,8 +18,7 @@
 //     c = max over the keys of (z + log2 scale_v) - a constant,      p = 2^(z - c),      w = p * scale_v,
 // the row's result is sum w code / sum p, so one running number per row replaces the softmax's maximum and the weights'
 // exponent, and a key whose score is high but whose scale is small (or the other way round) costs no precision.  log2 of
-// the scale only steers c, so the approximate one does; it is held from below (a scale of 1e-33 of the unit), which keeps p
-// below 2^121; sums of p are kept in units of 2^22.
+// the scale only steers c, so the approximate one does; it is held from below, which keeps p inside binary32.
 #pragma once
 #include "kernels.cuh"
 #include "kv.cuh"
@@ -47,7 +46,6 @@ int launch_kv_attention_many(b200q_ctx* ctx, const AttnArgs& a, int D);   // kv_
 namespace {
 
 constexpr float NEG_INF = -__builtin_huge_valf();
-constexpr float P_UNIT = 0x1p-22f;       // sums of p are held times this: up to 2^24 keys of weight 2^120 stay finite
 constexpr float C_NONE = -3.0e38f;       // c of a row that has seen nothing: finite, so that differences with it are numbers
 constexpr float C_SEEN = -1.0e38f;       // ... and of a row that has seen something it is above this
 constexpr float FAR = 0x1p20f;           // scores are taken relative to a score of the row when they are further from zero
@@ -62,7 +60,7 @@ __device__ __forceinline__ float log2_raw(float s) {
   asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
   return r;
 }
-__device__ __forceinline__ float log2_scale(float s) { return fmaxf(log2_raw(s), -110.0f); }
+__device__ __forceinline__ float log2_scale(float s) { return fmaxf(log2_raw(s), -103.0f); }
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");

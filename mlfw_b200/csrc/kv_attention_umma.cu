@@ -45,6 +45,9 @@ struct Many {
   static constexpr int QHI = 0, QLO = Q_BYTES, RING = 2 * Q_BYTES, END = RING + STAGES * STAGE;
   static constexpr int SMEM = END + 1024;
 };
+// Weights stay below 2^15 for any scale of V: p is up to 2^118 where the scale is 2^-103 or less, 2^-106 where it is the
+// largest there is.  Sums of p times this stay inside binary32 at both ends: 2^24 keys of the one, a single key of the other.
+constexpr float L_UNIT = 0x1p-14f;
 // columns: scores of even and odd tiles, the weights over them; O of even and odd tiles
 constexpr int TM_S = 0, TM_S_STEP = 64, TM_O = 128, TM_O_STEP = 128, TM_COLS = 512;
 
@@ -369,7 +372,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv_attention_many_kernel(cons
         if (!alive) break;
 #pragma unroll
         for (int k = 0; k < 4; k++) top = fmaxf(top, top_x[buf][k][row]);
-        const float c_new = fmaxf(c_run, top - 10.0f), fold_new = ex2(c_run - c_new);
+        const float c_new = fmaxf(c_run, top - 15.0f), fold_new = ex2(c_run - c_new);
         c_run = c_new;
         float sum = 0.0f;
         uint32_t h[NC / 2], l[NC / 2];
@@ -387,7 +390,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv_attention_many_kernel(cons
           split_f16(wt[0], wt[1], h[i / 2], l[i / 2]);
           split_f16(wt[2], wt[3], h[i / 2 + 1], l[i / 2 + 1]);
         }
-        l_run = fmaf(l_run, fold_new, sum * P_UNIT);
+        l_run = fmaf(l_run, fold_new, sum * L_UNIT);
         // the sixteen tokens' weights, zero where another copy has them: 8 + 8 columns over their scores
         uint32_t ph[8], pl[8];
 #pragma unroll
@@ -456,9 +459,9 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv_attention_many_kernel(cons
           v.x += y.x; v.y += y.y; v.z += y.z; v.w += y.w;
         }
         if (whole) {
-          const float inv = sum == 0.0f ? 0.0f : P_UNIT / sum;
+          const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
           int t;
-          *reinterpret_cast<float4*>(a.out + row_offset(a, w.b, w.head, w.rb * ROWS + r, a.ld_o, D, t) + p * 4) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+          *reinterpret_cast<float4*>(a.out + row_offset(a, w.b, w.head, w.rb * ROWS + r, a.ld_o, D, t) + p * 4) = make_float4(v.x * L_UNIT * inv, v.y * L_UNIT * inv, v.z * L_UNIT * inv, v.w * L_UNIT * inv);
         } else {
           __stcg(reinterpret_cast<float4*>(slot + r * D) + p, v);
           if (p == 0) { __stcg(slot + ROWS * D + r, c_max); __stcg(slot + ROWS * D + ROWS + r, sum); }
@@ -648,9 +651,9 @@ __global__ void __launch_bounds__(256) kv_attention_join_kernel(const AttnArgs a
       sum = fmaf(__ldcg(s + ROWS * D + ROWS + r), f, sum);
       v.x = fmaf(y.x, f, v.x); v.y = fmaf(y.y, f, v.y); v.z = fmaf(y.z, f, v.z); v.w = fmaf(y.w, f, v.w);
     }
-    const float inv = sum == 0.0f ? 0.0f : P_UNIT / sum;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     int t;
-    *reinterpret_cast<float4*>(a.out + row_offset(a, b, item.y, rb * ROWS + r, a.ld_o, D, t) + p * 4) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+    *reinterpret_cast<float4*>(a.out + row_offset(a, b, item.y, rb * ROWS + r, a.ld_o, D, t) + p * 4) = make_float4(v.x * L_UNIT * inv, v.y * L_UNIT * inv, v.z * L_UNIT * inv, v.w * L_UNIT * inv);
   }
 }
 

@@ -318,3 +318,19 @@ def test_attention_beside_a_strong_channel(ctx, T, dim):
                 delta = 0.125 * (16 * u * (np.abs(k) @ np.abs(x)) + held) + 2.0**-21 + u * (z.max() - z + 16)
                 bound = (w * delta) @ np.abs(v - r) / w.sum() + (4 * u + (m / 64 + 24) * u) * (w @ np.abs(v)) / w.sum()
                 assert (np.abs(got[0, t, h] - r) <= bound).all(), (strong, t, h, np.max(np.abs(got[0, t, h] - r) / bound))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_a_single_visible_value_of_any_magnitude(ctx, dim):
+    """The first row of a chunk sees one token and returns its value: 22 bits of the weight, four roundings."""
+    S = Setup(ctx, 1, 40, 16, 2, dim)
+    S.fill([40])
+    plain = S.scales[1].copy()
+    q = S.rng.standard_normal((1, 40, 4, dim)).astype(np.float32)
+    for f in (1e-30, 1e-10, 1, 1e10, 1e30, 1e37, 1e38):
+        S.scales[1][:] = plain * np.float32(f)
+        S.upload()
+        got = run_attention(S, q, [0], None, None, dim ** -0.5)
+        _, vc, _, vs = S.tokens(0, 1)
+        want = np.repeat(vc[0].astype(np.float64) * vs[0, :, None], 2, axis=0)
+        assert np.abs(got[0, 0] - want).max() <= 8 * 2.0**-24 * np.abs(want).max(), (f, np.abs(got[0, 0] - want).max() / np.abs(want).max())
