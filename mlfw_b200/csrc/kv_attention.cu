@@ -400,18 +400,18 @@ __global__ void __launch_bounds__(32 * Four<D>::WARPS, 1) kv_attention_four_kern
           lower = fminf((float)up, 80.0f);
         }
         if (__builtin_expect(__any_sync(0xffffffffu, m != 0.0f || (fabsf(top) > FAR && top > NEG_INF)), 0)) {
+          float raw[4];                                         // z - m is exact where it matters, from the scores themselves
 #pragma unroll
-          for (int j = 0; j < 4; j++) z[j] -= m;
-          top = top_of();
+          for (int j = 0; j < 4; j++) raw[j] = z[j];
           for (int k = 0; k < 8; k++) {                         // each round leaves a rounding of the one before: 2^-23 of it
+#pragma unroll
+            for (int j = 0; j < 4; j++) z[j] = raw[j] - m;
+            top = top_of();
             const bool far = top > FAR || (top < -FAR && top > NEG_INF && c_old < C_SEEN);
             if (!__any_sync(0xffffffffu, far)) break;
-            const float d = far ? top : 0.0f;
-#pragma unroll
-            for (int j = 0; j < 4; j++) z[j] -= d;
-            m += d;
-            c_old = fmaxf(c_old - d, C_NONE);
-            top = top_of();
+            const float m_old = m;
+            if (far) m += top;
+            c_old = fmaxf(c_old - (m - m_old), C_NONE);
           }
         }
         const float c_low = fmaxf(c_old - lower, C_NONE);

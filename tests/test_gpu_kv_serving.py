@@ -334,3 +334,31 @@ def test_a_single_visible_value_of_any_magnitude(ctx, dim):
         _, vc, _, vs = S.tokens(0, 1)
         want = np.repeat(vc[0].astype(np.float64) * vs[0, :, None], 2, axis=0)
         assert np.abs(got[0, 0] - want).max() <= 8 * 2.0**-24 * np.abs(want).max(), (f, np.abs(got[0, 0] - want).max() / np.abs(want).max())
+
+
+@pytest.mark.parametrize("T,dim", [(1, 64), (1, 128), (9, 64)])
+def test_equal_scores_weigh_the_same_wherever_they_are(ctx, T, dim):
+    """Three equal keys among many far below, in different tiles of long runs: the mean of their values at every size of the scores.
+    Many sequences over the same pages, so that a warp walks many tiles and meets the keys in the middle of its run."""
+    B, n, page = 300, 3000, 64
+    S = Setup(ctx, 1, n + T, page, 1, dim)
+    S.fill([n + T])
+    sign = S.rng.choice([-1, 1], dim)
+    q = np.broadcast_to(sign * S.rng.uniform(0.5, 2, dim), (B, T, 2, dim)).astype(np.float32)
+    table = ctx.to_device(np.ascontiguousarray(np.broadcast_to(S.table, (B, S.per))))
+    out = Guarded(ctx, (B * T, 2 * dim), np.float32, np.zeros((B * T, 2 * dim)))
+    plain = S.codes[0].copy()
+    for negative in (False, True):
+        for f in np.geomspace(1e4, 1e8, 17):
+            S.codes[0][:], S.scales[0][:] = plain, np.float32(0.02)
+            if negative:
+                S.codes[0][:] = -sign * (100 + S.rng.integers(0, 28, S.codes[0].shape[:-1])[..., None])
+            lead = S.rng.choice(n, 3, replace=False)
+            at = S.table[0, lead // page], 0, lead % page
+            S.codes[0][at] = sign * (-60 if negative else 127)
+            S.upload()
+            values = S.codes[1][at].astype(np.float64) * S.scales[1][at][:, None]
+            S.cache.attention(ctx.to_device((q * np.float32(f)).reshape(B * T, 2 * dim)), 2 * dim, B, T, 2, table, S.per, S.dev([n] * B), None, None,
+                              dim ** -0.5, out.ptr, 2 * dim)
+            err = np.abs(out.download().reshape(B, T, 2, dim) - values.mean(0)).max()
+            assert err <= 8 * 2.0**-24 * np.abs(values).max(), (negative, f, err / np.abs(values).max())
