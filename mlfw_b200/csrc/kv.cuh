@@ -23,8 +23,8 @@ struct KvBatch {
 };
 
 // Workspace of the attention: a counter and an item per block (one block per SM), then two slots per block for pieces of items
-// (128 rows of 128 with their sums: 20 MB on 148 SMs).  Its size depends on the GPU only, so a recording never finds it moved.
-constexpr int KV_SLOT_FLOATS = 128 * (128 + 2);
+// (128 rows of 128 and three numbers more in the room of four: 20 MB on 148 SMs).  Its size depends on the GPU only, so a recording never finds it moved.
+constexpr int KV_SLOT_FLOATS = 128 * (128 + 4);
 inline size_t kv_item_bytes(const b200q_ctx* ctx) { return (size_t)ctx->sm_count * 16; }
 inline size_t kv_counter_bytes(const b200q_ctx* ctx) { return ((size_t)ctx->sm_count * sizeof(uint32_t) + 255) & ~size_t(255); }
 int kv_workspace(b200q_ctx* ctx);

@@ -180,6 +180,96 @@ __device__ __forceinline__ int v_row(int L, int q) {
   return (L / W) * (D / 4) + (D == 64 ? r ^ (((L / W) & 1) * 4) : r);
 }
 
+// A row of a piece whose scores are not within FAR of zero, where binary32 has no room beside them for log2 scale_v: token by token, with
+// the scores relative to their maximum m and sums in binary64.  The tensor cores' path leaves such a row with a c outside
+// (-FAR, FAR] and whatever it came to; no real model has one, so this is made to be right, not fast.  A warp holds a
+// row's D / 4 pieces of four dimensions in neighbouring lanes (two rows for D = 64); v and sum in units of 2^(m + c), sum times L_UNIT.
+template <int D>
+struct FarRow {
+  float4 v;
+  float sum, c, m;
+};
+template <int D, int ROWS>
+__device__ __forceinline__ FarRow<D> far_row(const AttnArgs& a, int b, int head, int rb, int r, int tile0, int tile1, int p, bool asked) {
+  auto over_row = [](auto x, auto f) {
+#pragma unroll
+    for (int o = 1; o < D / 4; o <<= 1) x = f(x, __shfl_xor_sync(0xffffffffu, x, o));
+    return x;
+  };
+  FarRow<D> y;
+  y.v = make_float4(0.f, 0.f, 0.f, 0.f);
+  y.sum = 0.0f; y.c = -FAR; y.m = 0.0f;
+  // most rows that come here just see nothing of the piece: it begins behind them
+  int t;
+  const float* src = a.q + row_offset(a, b, head, rb * ROWS + r, a.ld_q, D, t);
+  const int64_t first = a.start[b], lo = (int64_t)tile0 * MT - first;
+  const int rows = kv_rows_in_use(a.count, b, a.T);
+  uint64_t seen = a.tree ? a.tree[(int64_t)b * a.T + t] : 0;
+  if (rows < 64) seen &= (1ull << rows) - 1;
+  if (!__any_sync(0xffffffffu, asked && (lo < 0 || (a.tree ? lo < 64 && (seen >> lo) != 0 : lo <= t)))) return y;
+  const float4 q = __ldcg(reinterpret_cast<const float4*>(src) + p);
+  const float big = over_row(fmaxf(fmaxf(fabsf(q.x), fabsf(q.y)), fmaxf(fabsf(q.z), fabsf(q.w))), [](float x, float y) { return fmaxf(x, y); });
+  const int ex = max(__float_as_int(big) >> 23, 24) - 127;
+  const float up = pow2(14 - ex), rs = a.scale_log2e * pow2(ex - 14);
+  const float x[4] = {q.x * up, q.y * up, q.z * up, q.w * up};
+  const int32_t* table = a.page_table + (int64_t)b * a.g.max_pages;
+  float m = NEG_INF;
+  double l = 0.0, n[4] = {0.0, 0.0, 0.0, 0.0};
+  const int64_t end = min((int64_t)tile1 * MT, kv_visible(a.g, first, rows, a.group, ROWS, rb, a.tree != nullptr));   // inside the page table
+#pragma unroll 1
+  for (int64_t pos = (int64_t)tile0 * MT; pos < end; pos += 4) {
+    const int page = __ldcg(table + (pos >> a.g.page_shift));
+    if ((uint32_t)page >= (uint32_t)a.g.pages) continue;
+    const int64_t cell = (((int64_t)page * a.g.heads + head) << a.g.page_shift) + (pos & ((1 << a.g.page_shift) - 1));
+    float z[4], vs[4], top = NEG_INF;
+    uint32_t vc[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const uint32_t k = __ldcg(reinterpret_cast<const uint32_t*>(a.k + (cell + i) * D) + p);
+      vc[i] = __ldcg(reinterpret_cast<const uint32_t*>(a.v + (cell + i) * D) + p);
+      const float ks = __ldcg(a.ks + cell + i);
+      vs[i] = __ldcg(a.vs + cell + i);
+      float dot = 0.0f;
+#pragma unroll
+      for (int c = 0; c < 4; c++) dot = fmaf(x[c], (float)(int8_t)(k >> (8 * c)), dot);
+      dot = over_row(dot, [](float y, float u) { return y + u; });
+      const int64_t j = pos + i - first;
+      const bool sees = pos + i < end && (j < 0 || (a.tree ? j < 64 && ((seen >> j) & 1) : j <= t));
+      z[i] = sees ? dot * (ks * rs) : NEG_INF;
+      top = fmaxf(top, z[i]);
+    }
+    if (top > m) {
+      const double f = ex2(m - top);
+      l *= f;
+#pragma unroll
+      for (int c = 0; c < 4; c++) n[c] *= f;
+      m = top;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      if (z[i] > NEG_INF) {
+        const float e = ex2(z[i] - m);
+        l += e;
+#pragma unroll
+        for (int c = 0; c < 4; c++) n[c] += (double)e * ((double)vs[i] * (double)(int8_t)(vc[i] >> (8 * c)));
+      }
+    }
+  }
+  int e = -2000;                                                 // exponent of the largest
+#pragma unroll
+  for (int c = 0; c < 4; c++) e = max(e, ((__double2hiint(n[c]) >> 20) & 0x7ff) - 1023);
+  e = over_row(e, [](int u, int v) { return max(u, v); });
+  if (m > NEG_INF) {
+    const int c = max(e - 24, -90);
+    const double s = __hiloint2double((1023 - c) << 20, 0);
+    y.v = make_float4((float)(n[0] * s), (float)(n[1] * s), (float)(n[2] * s), (float)(n[3] * s));
+    y.sum = (float)(l * s * (double)L_UNIT);
+    y.c = (float)c;
+    y.m = m;
+  }
+  return y;
+}
+
 template <int D, int CS>
 __global__ void __launch_bounds__(MANY_THREADS, 1) kv_attention_many_kernel(const AttnArgs a, const ManyParams mp) {
   using C = Many<D>;
@@ -282,7 +372,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv_attention_many_kernel(cons
         const int ex = max((int)(top >> 23), 24) - 127;
         // rs is kept positive, so that a masked x = -Inf stays -Inf: a negative scale turns the query's sign, a zero one zeroes it
         const float up = a.scale_log2e == 0.0f ? 0.0f : copysignf(pow2(14 - ex), a.scale_log2e);
-        rs = finite ? fmaxf(fabsf(a.scale_log2e) * pow2(ex - 14), 1e-37f) : __int_as_float(0x7fc00000);
+        rs = finite ? fmaxf(fabsf(a.scale_log2e) * pow2(ex - 14), 1e-45f) : __int_as_float(0x7fc00000);
 #pragma unroll
         for (int i = 0; i < QD / 4; i += 2) {                    // eight dimensions: 16 bytes of either half, in the order of staged K
           uint32_t h[4], l[4];
@@ -305,7 +395,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv_attention_many_kernel(cons
       float o[QD];                                               // outputs, in the order of the V tile's rows
 #pragma unroll
       for (int i = 0; i < QD; i++) o[i] = 0.0f;
-      float c_run = C_NONE, l_run = 0.0f, fold = 0.0f;           // fold: the factor that goes with the latest tile's O
+      float c_run = -FAR, l_run = 0.0f, fold = 0.0f;             // fold: the factor that goes with the latest tile's O
       auto take_outputs = [&](uint32_t t) -> bool {              // o = o * fold + O of tile t
         if (!__all_sync(0xffffffffu, wait(S::OUTPUTS + 8 * (t & 1), (t >> 1) & 1))) return false;
         fence_after();
@@ -445,9 +535,10 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv_attention_many_kernel(cons
       const bool whole = w.tile0 == 0 && w.tile1 == w.tiles;
       if (w.tile0 == 0 && !whole && tid == 0) a.items[blockIdx.x] = make_int4(w.e, w.head, kv_run_of(run.all, w.at + w.tiles - 1), 1);
       float* slot = a.slots + (int64_t)(2 * blockIdx.x + (w.tile0 == 0 ? 1 : 0)) * KV_SLOT_FLOATS;
-      for (int x = tid; x < w.rows_here * (D / 4); x += 32 * SOFT_WARPS) {
+      for (int x = tid; x - lane < w.rows_here * (D / 4); x += 32 * SOFT_WARPS) {   // whole warps: a row's D / 4 pieces are neighbouring lanes
         const int r = x / (D / 4), p = x % (D / 4);
-        float c_max = c_x[r], sum = 0.0f;
+        const bool used = r < w.rows_here;
+        float c_max = c_x[r], sum = 0.0f, m = 0.0f;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int k = 1; k < CS; k++) c_max = fmaxf(c_max, c_x[k * ROWS + r]);
@@ -458,13 +549,19 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) kv_attention_many_kernel(cons
           sum = fmaf((sum_x[0][ln] + sum_x[1][ln]) + (sum_x[2][ln] + sum_x[3][ln]), ex2(c_x[ln] - c_max), sum);
           v.x += y.x; v.y += y.y; v.z += y.z; v.w += y.w;
         }
+        const bool far = used && (c_max > FAR || (c_max <= -FAR && sum == sum));   // (sum NaN: the query has one, the row stays NaN)
+        if (__any_sync(0xffffffffu, far)) {
+          const FarRow<D> y = far_row<D, ROWS>(a, w.b, w.head, w.rb, used ? r : 0, w.tile0, w.tile1, p, far);
+          if (far) { v = y.v; sum = y.sum; c_max = y.c; m = y.m; }
+        }
+        if (!used) continue;
         if (whole) {
           const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
           int t;
           *reinterpret_cast<float4*>(a.out + row_offset(a, w.b, w.head, w.rb * ROWS + r, a.ld_o, D, t) + p * 4) = make_float4(v.x * L_UNIT * inv, v.y * L_UNIT * inv, v.z * L_UNIT * inv, v.w * L_UNIT * inv);
         } else {
           __stcg(reinterpret_cast<float4*>(slot + r * D) + p, v);
-          if (p == 0) { __stcg(slot + ROWS * D + r, c_max); __stcg(slot + ROWS * D + ROWS + r, sum); }
+          if (p == 0) __stcg(reinterpret_cast<float4*>(slot + ROWS * D) + r, make_float4(c_max, sum, m, 0.0f));
         }
       }
       alive = meet(S::SOFT, soft_phase);                         // Q's tiles are about to be written again
@@ -641,14 +738,27 @@ __global__ void __launch_bounds__(256) kv_attention_join_kernel(const AttnArgs a
   const int r0 = blockIdx.y * 16, r1 = min(rows_here, r0 + 16);
   for (int x = threadIdx.x; x < (r1 - r0) * P; x += 256) {
     const int r = r0 + x / P, p = x % P;
-    float c_max = C_NONE, sum = 0.0f;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int c = run0; c <= item.z; c++) c_max = fmaxf(c_max, __ldcg(a.slots + (int64_t)(2 * c + (c == run0)) * KV_SLOT_FLOATS + ROWS * D + r));
+    // pieces in units of 2^(m + c), against the largest m of one that has seen something and the largest c relative to it
+    auto piece = [&](int c) { return reinterpret_cast<const float4*>(a.slots + (int64_t)(2 * c + (c == run0)) * KV_SLOT_FLOATS); };
+    auto row = [&](int c) { return __ldcg(piece(c) + ROWS * P + r); };   // c, sum, m
+    float far = C_NONE, top = C_NONE, sum = 0.0f;
+    bool some = false;
     for (int c = run0; c <= item.z; c++) {
-      const float* s = a.slots + (int64_t)(2 * c + (c == run0)) * KV_SLOT_FLOATS;
-      const float f = ex2(__ldcg(s + ROWS * D + r) - c_max);
-      const float4 y = __ldcg(reinterpret_cast<const float4*>(s + r * D) + p);
-      sum = fmaf(__ldcg(s + ROWS * D + ROWS + r), f, sum);
+      const float4 x = row(c);
+      top = fmaxf(top, x.x);
+      far = fmaxf(far, x.x > -FAR ? x.z : C_NONE);
+      some |= x.z != 0.0f;
+    }
+    auto beside = [&](const float4& x) { return x.x > -FAR ? x.x + (x.z - far) : C_NONE; };
+    if (some) {
+      top = C_NONE;
+      for (int c = run0; c <= item.z; c++) top = fmaxf(top, beside(row(c)));
+    }
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int c = run0; c <= item.z; c++) {
+      const float4 x = row(c), y = __ldcg(piece(c) + r * P + p);
+      const float f = ex2((some ? beside(x) : x.x) - top);
+      sum = fmaf(x.y, f, sum);
       v.x = fmaf(y.x, f, v.x); v.y = fmaf(y.y, f, v.y); v.z = fmaf(y.z, f, v.z); v.w = fmaf(y.w, f, v.w);
     }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;

@@ -218,7 +218,8 @@ def test_attention_over_values_of_any_magnitude(ctx, T, dim):
     check_attention(S, q, [6000], None, None, dim ** -0.5)
 
 
-@pytest.mark.parametrize("T,dim,n", [(1, 64, 200), (1, 128, 5000), (9, 64, 3000), (9, 128, 150)])
+@pytest.mark.parametrize("T,dim,n", [(1, 64, 200), (1, 128, 5000), (9, 64, 3000), (9, 128, 150), (25, 64, 200), (25, 128, 4000), (70, 64, 3000),
+                                     (70, 128, 300)])
 def test_attention_scores_of_any_magnitude(ctx, T, dim, n):
     """Two equal keys lead all others by more than any weight survives, at opposite ends of the sequence: their values' mean, however
     large the scores are and whichever sign they have.  One exact addition and one division: off by a few roundings."""
@@ -336,11 +337,11 @@ def test_a_single_visible_value_of_any_magnitude(ctx, dim):
         assert np.abs(got[0, 0] - want).max() <= 8 * 2.0**-24 * np.abs(want).max(), (f, np.abs(got[0, 0] - want).max() / np.abs(want).max())
 
 
-@pytest.mark.parametrize("T,dim", [(1, 64), (1, 128), (9, 64)])
+@pytest.mark.parametrize("T,dim", [(1, 64), (1, 128), (9, 64), (24, 64), (20, 128), (67, 64)])
 def test_equal_scores_weigh_the_same_wherever_they_are(ctx, T, dim):
     """Three equal keys among many far below, in different tiles of long runs: the mean of their values at every size of the scores.
     Many sequences over the same pages, so that a warp walks many tiles and meets the keys in the middle of its run."""
-    B, n, page = 300, 3000, 64
+    B, n, page = 300 if T * 2 <= 36 else 40, 3000, 64
     S = Setup(ctx, 1, n + T, page, 1, dim)
     S.fill([n + T])
     sign = S.rng.choice([-1, 1], dim)
@@ -362,3 +363,39 @@ def test_equal_scores_weigh_the_same_wherever_they_are(ctx, T, dim):
                               dim ** -0.5, out.ptr, 2 * dim)
             err = np.abs(out.download().reshape(B, T, 2, dim) - values.mean(0)).max()
             assert err <= 8 * 2.0**-24 * np.abs(values).max(), (negative, f, err / np.abs(values).max())
+
+
+@pytest.mark.parametrize("T,H,dim,n", [(41, 1, 64, 700), (63, 3, 64, 150), (39, 1, 128, 2000), (64, 4, 128, 90), (11, 1, 64, 700), (33, 1, 128, 90)])
+def test_rows_with_large_scores_beside_ordinary_ones(ctx, T, H, dim, n):
+    """A drafted tree of which every third row has scores in the millions, of either sign, and some rows see only new tokens: the large ones
+    return the value of their largest score (the next is out of reach), the ordinary ones follow the formula, page ends and all."""
+    S = Setup(ctx, 2, n + T, 16, 1, dim)
+    start, count = [n, 0], [T, T - 2]
+    S.fill(np.array(start) + count)
+    q = S.rng.standard_normal((2, T, H, dim)).astype(np.float32)
+    q[:, ::3] *= np.float32(1e6)
+    q[:, 1::6] = 0
+    tree = random_tree(S.rng, 2, T)
+    tree[1, 4] = 0                                                # nothing at all
+    got = run_attention(S, q, start, count, tree, 0.3)
+    with np.errstate(over="ignore"):                              # the bound of the large rows says nothing
+        want, bound = attention_rows(S, q, start, count, tree, 0.3)
+    for b in range(2):
+        m = start[b] + count[b]
+        kc, vc, ks, vs = (a[:, 0] for a in S.tokens(b, m))
+        j = np.arange(m) - start[b]
+        for t in range(count[b]):
+            see = (j < 0) | ((tree[b, t] >> np.clip(j, 0, 63).astype(np.uint64)) & np.uint64(1)).astype(bool)
+            if not see.any():
+                assert (got[b, t] == 0).all()
+                continue
+            for h in range(H):
+                if t % 3:
+                    assert np.abs(got[b, t, h] - want[b, t, h]).max() <= bound[b, t, h]
+                    continue
+                z = np.where(see, 0.3 * ks.astype(np.float64) * (kc.astype(np.float64) @ q[b, t, h].astype(np.float64)), -np.inf)
+                first = int(np.argmax(z))
+                if see.sum() > 1 and z[first] - np.partition(z, -2)[-2] < 1e-4 * np.abs(z[see]).max():
+                    continue                                      # too near to tell in binary32
+                v = vc[first].astype(np.float64) * vs[first]
+                assert np.abs(got[b, t, h] - v).max() <= 8 * 2.0**-24 * np.abs(v).max(), (b, t, h)
