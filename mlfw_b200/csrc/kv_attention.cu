@@ -381,25 +381,26 @@ __global__ void __launch_bounds__(32 * Four<D>::WARPS, 1) kv_attention_four_kern
       float top = top_of();
       if (__any_sync(0xffffffffu, top > limit) || since == 1024) {
         float c_old = c_run, lower = 0.0f, g = 1.0f;
-        if (__builtin_expect(__any_sync(0xffffffffu, fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3])) > 0x1p60f), 0)) {   // another kappa; vs may be infinite
-          float big = 0.0f;
+        const bool big_vs = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3])) > 0x1p60f;
+        if (__builtin_expect(__any_sync(0xffffffffu, big_vs || m != 0.0f || (fabsf(top) > FAR && top > NEG_INF)), 0)) {
+          if (__any_sync(0xffffffffu, big_vs)) {                // another kappa; vs may be infinite
+            float big = 0.0f;
 #pragma unroll
-          for (int j = 0; j < 4; j++) {
-            vs[j] = vs[j] == 0.0f ? 0.0f : lds_f(s_src + here + (j >> 1) * C::GRAN + (j & 1) * 32 + 64);
-            big = fmaxf(big, vs[j]);
+            for (int j = 0; j < 4; j++) {
+              vs[j] = vs[j] == 0.0f ? 0.0f : lds_f(s_src + here + (j >> 1) * C::GRAN + (j & 1) * 32 + 64);
+              big = fmaxf(big, vs[j]);
+            }
+            const float kf_old = kf;
+            kf = kappa_of(big);
+#pragma unroll
+            for (int j = 0; j < 4; j++) vs[j] *= kf;
+            top = top_of();
+            // the integer sums are in units of 2^(c + kappa).  c goes down by what kappa goes up, so that a row that does not see the
+            // large values keeps its digits; by 2^80 at most, which the sums of p have room for
+            const int up = (__float_as_int(kf_old) - __float_as_int(kf)) >> 23;
+            g = up > 126 ? 0.0f : pow2(-up);
+            lower = fminf((float)up, 80.0f);
           }
-          const float kf_old = kf;
-          kf = kappa_of(big);
-#pragma unroll
-          for (int j = 0; j < 4; j++) vs[j] *= kf;
-          top = top_of();
-          // the integer sums are in units of 2^(c + kappa).  c goes down by what kappa goes up, so that a row that does not see the
-          // large values keeps its digits; by 2^80 at most, which the sums of p have room for
-          const int up = (__float_as_int(kf_old) - __float_as_int(kf)) >> 23;
-          g = up > 126 ? 0.0f : pow2(-up);
-          lower = fminf((float)up, 80.0f);
-        }
-        if (__builtin_expect(__any_sync(0xffffffffu, m != 0.0f || (fabsf(top) > FAR && top > NEG_INF)), 0)) {
           float raw[4];                                         // z - m is exact where it matters, from the scores themselves
 #pragma unroll
           for (int j = 0; j < 4; j++) raw[j] = z[j];
