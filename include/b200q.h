@@ -353,10 +353,16 @@ int b200q_kv_append(b200q_ctx* ctx, b200q_kv_cache* cache, const float* k, const
 int b200q_kv_read(b200q_ctx* ctx, b200q_kv_cache* cache, int64_t B, int64_t T, const int32_t* page_table, int64_t max_pages,
                   const int32_t* start, const int32_t* count, float* k_out, float* v_out, int64_t ld_k, int64_t ld_v);
 /* out = softmax(scale * q K^T) V over the cached rows for H query heads (a multiple of the cache's heads: H / heads
- * neighbouring heads share one), binary32 accuracy.  Row t sees every position below start[b] and, of the new ones (which
+ * neighbouring heads share one).  Row t sees every position below start[b] and, of the new ones (which
  * b200q_kv_append has written), j <= t when tree is null -- T = 1 is a decoding step, T > 1 a chunk of a prompt -- or those
  * j < count[b] whose bit is set in tree[b * T + t]: a drafted tree of at most 64 tokens, each row the set of its ancestors
- * and itself.  A row that sees nothing is zero. */
+ * and itself.  A row that sees nothing is zero; one with a NaN or an infinity in its query is NaN.
+ * Accuracy: as binary32 arithmetic, some 5e-7 of the largest output on ordinary rows; scores and V may have any finite
+ * magnitude.  Two things are held in fewer bits.  A query element: with up to 36 query rows per cache head (T * H / heads) to
+ * 2^-31 of its row's largest; with more, to 22 bits of its own and no finer than 2^-40 of the largest.  A weight times V's scale: with
+ * up to 36 rows to 2^-28 of the row's largest, rounded so that many smaller ones keep their sum; with more, to 22 bits of its own
+ * and no finer than 2^-40 of the largest.  The same call gives the same bits every time; another batch around a sequence, or another
+ * T, may change its last bits, since the work is cut over all sequences of a call. */
 int b200q_kv_attention(b200q_ctx* ctx, b200q_kv_cache* cache, const float* q, int64_t ld_q, int64_t B, int64_t T, int64_t H,
                        const int32_t* page_table, int64_t max_pages, const int32_t* start, const int32_t* count, const uint64_t* tree,
                        float scale, float* out, int64_t ld_out);

@@ -39,12 +39,12 @@ __device__ __forceinline__ uint32_t v_at(int t, int c) {
 // the row that is, so c stays small.  m, kappa and c change in a branch that is entered when a row's largest weight
 // leaves its window (`limit`), on every tile once m is not zero.
 //
-// About 550 instructions per warp and 32 tokens of 128 dimensions, 500 of 64 (conversion of the codes to binary16 for
-// m16n8k16, tried first, took 1300).  Bound by reading the cache: 5.4 TB/s of the 6.5 measured at 48 sequences of up to 6000
-// tokens, 32 heads on 8, 128 wide (75 us; 412 MB), launch, search of the runs and joining included.  One block per SM, eight
+// About 470 instructions per tile of 32 tokens of 128 dimensions, 450 of 64, all included (conversion of the codes to binary16 for
+// m16n8k16, tried first, took 1300).  Bound by reading the cache: 5.3 TB/s of the 6.5 measured at 48 sequences of up to 6000
+// tokens, 32 heads on 8, 128 wide (75 to 80 us from run to run, median 78; 412 MB), launch, search of the runs and joining included.  One block per SM, eight
 // warps (D = 128: 64 integer sums and 32 outputs per thread, which need more than the 168 registers that twelve warps leave)
-// with two tiles each in flight, or twelve (D = 64) with three.  Same case with 12 x 2: 85 us, 10 x 2: 83, 8 x 3: 77,
-// 6 x 3: 76, 4 x 4: 86; 64 wide, 64 sequences of up to 2000 tokens, 12 heads, 12 x 3: 34.9 us, 16 x 3: 38.9, 8 x 4: 37.1,
+// with two tiles each in flight, or twelve (D = 64) with three.  Where 8 x 2 took 75 us, 12 x 2 took 85, 10 x 2 83, 8 x 3 77,
+// 6 x 3 76, 4 x 4 86; 64 wide, 64 sequences of up to 2000 tokens, 12 heads, 12 x 3: 34.9 us, 16 x 3: 38.9, 8 x 4: 37.1,
 // 12 x 2: 35.1.
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int IT = 32;                                          // tokens of a tile: two runs of sixteen, each in one page
@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(32 * Four<D>::WARPS, 1) kv_attention_four_kern
   kv_after_previous();
   if (tid < WARPS) arrived[tid] = 0;
   // At least 8 tiles per run, or whole items: one sequence of 500 tokens, 12 heads of 64, 8.5 us (runs of 8 tiles 9.5), 2000 tokens
-  // 11.5 (whole items 12.6); 4 sequences of 1000 tokens, 32 heads on 8 of 128, 12.0 (12.3).
+  // 11.3 (whole items 12.6); 4 sequences of 1000 tokens, 32 heads on 8 of 128, 11.9 (12.3).
   const Run run = find_run<ROWS, IT, 8, true>(a, row_blocks);   // (its barriers publish `arrived`)
   if (run.begin == run.end) return;
   const KvRuns parts = kv_runs(run.end - run.begin, 1, WARPS);
@@ -574,8 +574,8 @@ int launch_kv_attention(b200q_ctx* ctx, const b200q_kv_cache& c, const KvBatch& 
                    ld_q, ld_o, s.B, s.T, H, H / c.heads, scale * 1.4426950408889634f, ctx->status_dev, (uint32_t*)ctx->ws_kv.ptr,
                    (float*)((uint8_t*)ctx->ws_kv.ptr + kv_counter_bytes(ctx) + kv_item_bytes(ctx)), (int4*)((uint8_t*)ctx->ws_kv.ptr + kv_counter_bytes(ctx))};
   // Query rows per cache head.  Measured on both sides of the border, 8 cache heads, 16 sequences of up to 3000 tokens, here and
-  // there: 24 rows 38 and 56 us (head dimension 64), 56 and 76 us (128); 36 rows 51 and 58, 78 and 79; 40 rows 57 and 58, 83 and
-  // 79; 64 rows 83 and 60, 128 and 88.  (With 4 sequences of up to 600 tokens both take 14 to 30 us, here the fewer.)
+  // there: 24 rows 39 and 56 us (head dimension 64), 59 and 78 us (128); 36 rows 53 and 58, 83 and 84; 40 rows 59 and 58, 89 and
+  // 84; 64 rows 87 and 60, 137 and 96.  (With 4 sequences of up to 600 tokens both take 12 to 33 us, here the fewer.)
   if ((int64_t)s.T * a.group > 36) return launch_kv_attention_many(ctx, a, c.head_dim);
   return c.head_dim == 64 ? launch_four<64>(ctx, a) : launch_four<128>(ctx, a);
 }

@@ -4,17 +4,21 @@
 // tree) or those whose bit is set in its row of ancestors.  Query heads h of a group H / heads share cache head h / (H / heads).
 //
 // The arithmetic.  A cached value is code * scale with an integer |code| <= 128.  The codes go into the tensor cores as they
-// are; queries and weights, which are binary32, are split into parts that the tensor cores take, so the result has binary32
-// accuracy and the cache is never dequantized.  Two forms:
+// are; queries and weights, which are binary32, are split into parts that the tensor cores take, so the cache is never dequantized
+// and the result is as near as binary32 arithmetic comes: 3e-7 to 8e-7 of the largest output against binary64 on
+// ordinary rows.  What each form holds in fewer bits is said with it:
 //   Many rows (kv_attention_umma.cu), binary16 products, two per contraction.  A query row is scaled by a power of two to
 //   x = q * 2^(14 - e) with 2^e <= max|q| < 2^(e+1), and an element is its rounding to binary16 and the rounding of what is left: 22
 //   bits of its own down to 2^-17 of the row's largest, 2^-40 of the largest below that (a fixed point against the largest, tried
 //   first, left an element beside one 2000 times as large 11 bits).  sum_d q_d code_d = 2^(e-14) * (sum lo code + sum hi code), in one
 //   binary32 sum with the small parts first.  A weight is split the same way, the largest below 2^15.
+//   Sums over tiles of 64 tokens are binary32 additions one after another, of the outputs and of p: n / 64 roundings.
 //   Few rows (kv_attention.cu), integer products: queries and weights as 32-bit fixed-point numbers in four 8-bit digits, sums
-//   in 32-bit integers, exact.
-// Either way a score carries the rounding of q (2^-23 of the row's largest element or better) and the one of adding the
-// parts.  With z the score in units of log2 and the row's running
+//   in 32-bit integers, exact.  An element of a query row is held to 2^-31 of the row's largest (an element 2^-10 of the largest has 21
+//   bits; below a largest of 1e-31 there are fewer), a weight times its scale to 2^-28 of the row's largest, with a rounding that keeps the
+//   sum of many smaller ones; sums of p carry their rounding along.
+// ex2.approx adds 2^-22 to a weight, and so does the rounding of z - c where c is 8 or more: c holds log2 of V's scale in the
+// form for many rows, which makes it 2.5e-6 for values of V near 1e37 or 1e-35.  With z the score in units of log2 and the row's running
 //     c = max over the keys of (z + log2 scale_v) - a constant,      p = 2^(z - c),      w = p * scale_v,
 // the row's result is sum w code / sum p, so one running number per row replaces the softmax's maximum and the weights'
 // exponent, and a key whose score is high but whose scale is small (or the other way round) costs no precision.  log2 of

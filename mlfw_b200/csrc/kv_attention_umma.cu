@@ -10,8 +10,8 @@ namespace {
 // One block per SM walks a run of 64-token tiles; an item is up to 128 rows, the 128 lanes of tensor memory.  Roles:
 //   three staging warps: K and V of a tile from the cache into a ring in shared memory as binary16 tiles of the tensor cores'
 //     layout (V transposed), with the tokens' scales beside them, in units of sixteen tokens, which always share a page
-//     (three, so that the block has 20 warps and 96 registers per thread: the first case below takes 108 us, with two
-//     staging warps 127, with four, which leave 80 registers, 126);
+//     (three, so that the block has 20 warps and 96 registers per thread: where the first case below took 108 us, two
+//     staging warps took 127, four, which leave 80 registers, 126);
 //   one thread issues the products: S = Q_lo K^T + Q_hi K^T (tcgen05.mma kind::f16, 128 x 64) of tile j + 1, then
 //     O = P_lo V + P_hi V of tile j with the weights read from tensor memory;
 //   sixteen softmax warps, four threads per row with sixteen tokens of a tile each: scores from tensor memory, the row's c
@@ -20,13 +20,16 @@ namespace {
 //     additions, not the tensor core's.
 // Scores and O are double-buffered (384 columns of tensor memory), so products, softmax and staging of neighbouring tiles
 // overlap.  Measured: two prompts' chunks of 512 rows behind up to 4000 cached tokens, 16 heads on 4, 128 wide (26 GFLOP, twice
-// that in binary16 products): 107 us with the join, whose 27 MB between L2 and the SMs take 9; eight drafted trees of 31 over
-// up to 5000 tokens, 32 heads on 8: 80 us.  Bound by the softmax warps: about 3150 cycles per tile of 64 tokens, of which
-// the products need 1200 (tensor pipe 25 % busy): 480 instructions per warp and tile, 0.56 issued per cycle, the rest their
-// latency (the scores' load from tensor memory, the row's meeting, the split and the store of the weights).  Not kept
-// (against 110 us on the same box): scores three tiles ahead 136 (the registers spill), Q in tensor memory with a
-// single O 117; the two parts of the scores in columns of their own, added by the softmax warps, is 110 against 107.7; a
-// hardware barrier for the row's meeting 107.0 against 107.7, not worth a wait without a limit.
+// that in binary16 products): 110 to 123 us from run to run (median 122) with the join, whose 27 MB between L2 and the SMs take 9;
+// the step with eight drafted trees of 31 over up to 5000 tokens, 32 heads on 8, 92 to 100 with its four other launches.  Bound by the softmax warps: 192 000
+// cycles of an SM for 45 tiles of 64 tokens, 4200 per tile with what a piece costs, in which the tensor pipe is busy for 24 %
+// (1000; the arithmetic alone is 512).  10 000 warp instructions per tile, 2.4 issued per cycle of an SM, the rest
+// their latency (the scores' load from tensor memory, the row's meeting, the split and the store of the weights).  The softmax role
+// has no registers left: for D = 128 the kernel spills 72 bytes of stores and 172 (176 with CS = 2) of loads.  Not kept
+// (against 110 us on the same box): scores three tiles ahead 136 (far more spills), Q in tensor memory with a
+// single O 117; the two parts of the scores in columns of their own, added by the softmax warps, 110 against 107.7; a
+// hardware barrier for the row's meeting 107.0 against 107.7, not worth a wait without a limit; two tokens per instruction
+// (f32x2) for scores, weights and outputs 120 against 114 (the pairs want aligned registers).
 //
 // With 64 or fewer rows (CS = 2) the lanes hold two copies of the rows, each copy takes half of a thread's tokens and has
 // weights of zero elsewhere, and the copies are joined at the end: the softmax work, which would leave lanes idle,

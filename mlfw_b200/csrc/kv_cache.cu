@@ -46,8 +46,9 @@ __device__ __forceinline__ double kv_row_scale(float mn_f, float mx_f) {
 // within 127.5 * 2^-21 of a tie, or a row with a NaN, an infinity, equal elements or a range the reciprocal does not represent,
 // takes the exact binary64 routine, so codes and scales are those of b200q_quantize_per_token on the same rows.
 // Bound by memory latency (four bytes read and one written per element, behind the chain count, start, page): 7000 tokens of
-// 8 heads of 128, 72 MB in 20 us (3.5 TB/s; with the read of the next kernel 27.8 us, where three blocks per SM instead of
-// four took 28.7, and K and V in warps of their own 28.0); a decoding step's 32 tokens are a launch, 4.6 us.
+// 8 heads of 128, 72 MB in 19 us (3.7 TB/s; with the read of the next kernel 28 to 29.5 us; where this took 27.8, three blocks per
+// SM instead of four took 28.7, and K and V in warps of their own 28.0); a decoding step's 32 tokens are a launch, 4.6 us.  Four blocks
+// leave 64 registers: for D = 128 one word spills.
 // ---------------------------------------------------------------------------
 template <int V4>   // float4 per lane: D = 32 * V4
 __device__ __forceinline__ void append_row(const float4 (&x)[V4], bool live, int sub, uint32_t* codes, float* scale) {
@@ -112,7 +113,7 @@ __global__ void __launch_bounds__(256, 4) kv_append_kernel(const KvArgs a, const
 // ---------------------------------------------------------------------------
 // Read: y = fround(code * scale).  The same split: eight lanes per row, four heads of a token per warp, K and V.  A row
 // whose position is outside the cache reads as zeros and sets the status bit.  Bound by memory: 8 x 4096 tokens of 8 heads of
-// 128, 337 MB in 55.7 us (6.06 TB/s of the 6.5 measured).
+// 128, 337 MB in 56.6 us (5.95 TB/s of the 6.5 measured).
 // ---------------------------------------------------------------------------
 template <int D>
 __global__ void __launch_bounds__(256) kv_read_kernel(const KvArgs a, float* __restrict__ k_out, float* __restrict__ v_out, int64_t ld_k,
