@@ -30,7 +30,7 @@ __device__ __forceinline__ uint32_t v_at(int t, int c) {
 // adding the digits, and the outputs are added up without rounding until a row's c changes (or 2^15 tokens have passed), when
 // they are converted, scaled and moved to binary32.  c = floor(top) - 28, an integer, so that moving is exact; 3.75 bits are left
 // before a larger weight (below 2^32) moves it.  The unit is thus 2^-28 of the row's largest weight or less.  Many weights below it
-// must neither vanish nor count double, so a weight is rounded down after adding `dither` in (0, 1), which goes round by the golden
+// must neither vanish nor count double, so a weight is rounded down after adding `dither` between 0 and 1, which goes round by the golden
 // ratio from tile to tile: over many tokens a unit's share of all weights is kept, and what is left of a token's rounding is noise.
 // The sum of p carries the rounding of each addition into the next one for the same reason.
 // Scales of V are taken relative to a power of two 2^kappa, that of the first tile's largest until one 2^60 times as large comes, so
@@ -430,10 +430,10 @@ __global__ void __launch_bounds__(32 * Four<D>::WARPS, 1) kv_attention_four_kern
       for (int j = 0; j < 4; j++) {
         const float p = ex2(z[j] - c_run);
         sum += p;
-        const uint32_t w = __float2uint_rz(fmaf(p, vs[j], (j & 1) ? 0.99999994f - dither : dither));
+        const uint32_t w = __float2uint_rz(fmaf(p, vs[j], (j & 1) ? 0.9999f - dither : dither));
         t[j] = __byte_perm(w, __shfl_xor_sync(0xffffffffu, w, 4), sel);   // digits (3, 3, 1, 1) or (2, 2, 0, 0) of two neighbouring tokens
       }
-      dither += dither < 1.0f - GOLDEN ? GOLDEN : GOLDEN - 1.0f;
+      dither += dither < 0.3819f ? GOLDEN : GOLDEN - 1.0f;      // within -0.0001 .. 0.9999, so that a weight of zero stays zero
       const float add = fmaf(sum, P_UNIT, -l_over), l_new = l + add;
       l_over = (l_new - l) - add;                               // what the sum is above the true one
       l = l_new;
