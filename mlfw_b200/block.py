@@ -19,7 +19,7 @@ Weights are quantized per output channel on the device when the block is built a
 """
 from __future__ import annotations
 
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 from typing import Dict, List, Optional
 
 import numpy as np
@@ -68,9 +68,10 @@ class QuantLinear:
 
 @dataclass
 class _Rows:
-    """Intermediate buffers of a block for up to ``rows`` rows, and whether a recorded call used them."""
+    """Intermediate buffers of a block for up to ``rows`` rows, their first rows by number, and whether a recorded call used them."""
     rows: int
     bufs: Dict[str, DeviceBuffer]
+    views: Dict[int, Dict[str, DeviceBuffer]] = field(default_factory=dict)
     recorded: bool = False
 
 
@@ -111,7 +112,8 @@ class GPTBlock:
 
     def _reserve_cached(self, M: int) -> Dict[str, DeviceBuffer]:
         """Buffers of M rows: the first rows of one set that grows.  A recording holds the addresses of the set it was made with,
-        so a set that a recorded call used is kept beside the larger one until the context has no recording left."""
+        so a set that a recorded call used is kept beside the larger one until the context has no recording left (those made
+        through its Context object: Context.graph_begin)."""
         c = self.ctx
         if not c.recording and c.recordings == 0:
             self._recorded.clear()
@@ -126,7 +128,10 @@ class GPTBlock:
             self._cached = _Rows(rows, self._buffers(rows))
         if c.recording:
             self._cached.recorded = True
-        return {name: b.head(M) for name, b in self._cached.bufs.items()}
+        views = self._cached.views.get(M)
+        if views is None:
+            views = self._cached.views[M] = {name: b.head(M) for name, b in self._cached.bufs.items()}
+        return views
 
     def forward(self, h: DeviceBuffer, B: int, S: int, out: DeviceBuffer, causal: bool = True) -> Dict[str, DeviceBuffer]:
         """h, out: f32 [B*S, D].  Returns the intermediate buffers (reused by the next call with the same size)."""
